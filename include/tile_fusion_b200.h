@@ -32,6 +32,9 @@ typedef enum {
   TF_ERR_NOMEM = -5
 } tf_status;
 
+/* Types of the values of the dense training operators (tf_layer_norm_*, tf_pack8_*, tf_linear_ce_*). */
+typedef enum { TF_F32 = 0, TF_BF16 = 1, TF_F16 = 2 } tf_dtype;
+
 const char *tf_last_error(void);
 const char *tf_version(void);
 
@@ -378,6 +381,29 @@ int tf_schedule_reordered_adj(const tf_schedule *s, int m, const int *ap, const 
  * reference's criterion and this library's gather tiles can fuse. */
 int tf_rcm_order(int m, const int *ap, const int *ai, int *perm);
 int tf_permute_csr(int m, const int *ap, const int *ai, const float *ax, const int *perm, int *b_ap, int *b_ai, float *b_ax);
+
+/* ------------------------------------------------------------------------- */
+/* Softmax cross entropy of a linear layer                                    */
+/* ------------------------------------------------------------------------- */
+/* loss_i = log sum_v exp(x_i . w_v) - x_i . w_target(i) for rows whose target is not `ignore_index`, without the logits in
+ * memory.  x [rows][cols] (ld_x values from row to row) and w [vocab][cols] of one tf_dtype, all pointers on the device.
+ * reduction 0: loss[rows], zero where a row does not count; 1: the mean over the rows that count (zero if none does);
+ * 2: their sum; the sums are taken in 64 bits, in a fixed order.  lse2[rows] receives log2 of the sums for the backward call.
+ *   A target outside [0, vocab) that is not `ignore_index` makes its row's loss NaN, and its gradients.
+ *   backward: grad[1] (reduction 1, 2) or grad[rows] (0) is the gradient of the loss; dx [rows][cols] and dw [vocab][cols],
+ * contiguous, of the operands' type, are overwritten; either may be NULL.  Rows that do not count have a gradient of zero and
+ * add nothing to dw, whatever they hold.
+ *   work: tf_linear_ce_work_bytes bytes, 256-byte aligned, of the caller's; two calls that may overlap need two.  The calls
+ * only enqueue work on `stream`; they allocate nothing and can be captured.  tf_linear_ce_status waits for `stream` and says
+ * whether a bounded wait of the last call with this work space ran out (the forward's loss is NaN then). */
+long long tf_linear_ce_work_bytes(int rows, int cols, int vocab, int dtype, int backward);
+int tf_linear_ce_fwd(const void *x, long long ld_x, const void *w, long long ld_w, int dtype, const long long *target, int rows,
+                     int cols, int vocab, long long ignore_index, int reduction, float *loss, float *lse2, void *work,
+                     long long work_bytes, void *stream);
+int tf_linear_ce_bwd(const void *x, long long ld_x, const void *w, long long ld_w, int dtype, const long long *target, int rows,
+                     int cols, int vocab, long long ignore_index, int reduction, const float *lse2, const float *grad, void *dx,
+                     void *dw, void *work, long long work_bytes, void *stream);
+int tf_linear_ce_status(const void *work, void *stream);
 
 /* ------------------------------------------------------------------------- */
 /* Matrix files                                                               */

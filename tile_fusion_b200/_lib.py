@@ -11,6 +11,7 @@ LIB_PATH = os.path.join(HERE, "libtilefusion_b200.so")
 
 TF_OK, TF_ERR_ARG, TF_ERR_UNSUPPORTED, TF_ERR_CUDA, TF_ERR_TIMEOUT, TF_ERR_NOMEM = 0, -1, -2, -3, -4, -5
 INSPECT_FIXED, INSPECT_VT_SPMM, INSPECT_VT_GEMM, INSPECT_VT_SPMM_THREADS = 1, 2, 3, 4
+F32, BF16, F16 = 0, 1, 2
 MODE_STREAM, MODE_SCHEDULE, MODE_UNFUSED = 0, 1, 2
 
 
@@ -48,6 +49,7 @@ EXPORTS = [
     "tf_comm_from_nccl", "tf_comm_free", "tf_multi_plan", "tf_multi_free", "tf_multi_info", "tf_multi_plan_handle",
     "tf_multi_exec", "tf_multi_status", "tf_multi_trace", "tf_partition_layout", "tf_read_matrix", "tf_read_dense_mtx",
     "tf_schedule_unfused_csr", "tf_schedule_reordered_adj", "tf_rcm_order", "tf_permute_csr",
+    "tf_linear_ce_work_bytes", "tf_linear_ce_fwd", "tf_linear_ce_bwd", "tf_linear_ce_status",
 ]
 
 _lib = None
@@ -137,6 +139,11 @@ def lib() -> C.CDLL:
     L.tf_permute_csr.argtypes = [i, vp, vp, vp, vp, vp, vp, vp]
     L.tf_read_matrix.argtypes = [C.c_char_p, i, ip, ip, C.POINTER(ll), C.POINTER(vp), C.POINTER(vp), C.POINTER(vp)]
     L.tf_read_dense_mtx.argtypes = [C.c_char_p, ip, ip, C.POINTER(vp)]
+    L.tf_linear_ce_work_bytes.argtypes = [i, i, i, i, i]
+    L.tf_linear_ce_work_bytes.restype = ll
+    L.tf_linear_ce_fwd.argtypes = [vp, ll, vp, ll, i, vp, i, i, i, ll, i, vp, vp, vp, ll, vp]
+    L.tf_linear_ce_bwd.argtypes = [vp, ll, vp, ll, i, vp, i, i, i, ll, i, vp, vp, vp, vp, vp, ll, vp]
+    L.tf_linear_ce_status.argtypes = [vp, vp]
     L.tf_lattice_preview.argtypes = [C.POINTER(Csr), i, i, i, ip, C.POINTER(vp), C.POINTER(vp), C.POINTER(vp), ip]
     _lib = L
     return L

@@ -29,7 +29,7 @@ from __future__ import annotations
 import numpy as np
 import torch
 
-from . import _lib, api
+from . import _lib, api, dense_ops
 
 _LIB = torch.library.Library("sw_gcn", "DEF")
 _plans: dict = {}
@@ -169,6 +169,7 @@ _LIB.define("fusedGeMMSpMM_vt_ro(Tensor adj, Tensor feature, Tensor weight, Tens
 _LIB.define("geMMSpMM_f_bw(Tensor adj, Tensor feature, Tensor weight, Tensor[] schedule, int num_threads) -> Tensor")
 _LIB.define("unfused_gcn_forward(Tensor adj, Tensor feature, Tensor weight, int num_threads) -> Tensor")
 _LIB.define("cachedSpMMGeMM(Tensor af, Tensor weight, int num_threads) -> Tensor")
+_LIB.define("linear_cross_entropy(Tensor x, Tensor weight, Tensor target, int ignore_index=-100, str reduction='mean') -> Tensor")
 
 # CompositeImplicitAutograd: the implementations call autograd Functions themselves, as the reference's ops do.
 _LIB.impl("inspect", _inspect, "CompositeImplicitAutograd")
@@ -179,3 +180,4 @@ _LIB.impl("fusedGeMMSpMM_vt_ro", lambda adj, f, w, sched, nt, mts: _FusedGeMMSpM
 _LIB.impl("geMMSpMM_f_bw", lambda adj, f, w, sched, nt: _FusedGeMMSpMM.apply(adj, f, w, False), "CompositeImplicitAutograd")
 _LIB.impl("unfused_gcn_forward", lambda adj, f, w, nt: _FusedGeMMSpMM.apply(adj, f, w, True), "CompositeImplicitAutograd")
 _LIB.impl("cachedSpMMGeMM", lambda af, w, nt: _CachedSpMMGeMM.apply(af, w), "CompositeImplicitAutograd")
+_LIB.impl("linear_cross_entropy", dense_ops.linear_cross_entropy, "CompositeImplicitAutograd")
