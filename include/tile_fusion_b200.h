@@ -383,6 +383,48 @@ int tf_rcm_order(int m, const int *ap, const int *ai, int *perm);
 int tf_permute_csr(int m, const int *ap, const int *ai, const float *ax, const int *perm, int *b_ap, int *b_ai, float *b_ax);
 
 /* ------------------------------------------------------------------------- */
+/* Layer norm                                                                 */
+/* ------------------------------------------------------------------------- */
+/* y = (x - mean) * rstd * weight + bias over the columns of each row, rstd = 1 / sqrt(variance + eps), and its gradients.  x, y, dy, dx:
+ * [rows][cols] of one tf_dtype, ld_ values from row to row; weight, bias and their gradients [cols] of w_dtype; weight and bias may
+ * be NULL (1 and 0).  At most 16 384 columns.  Device pointers; the calls only enqueue work on `stream`.
+ *   forward: mean[rows] and rstd[rows] (fp32) are written where not NULL; the backward pass needs them.  codes / exponents not
+ * NULL: x goes there in 8 bits as tf_pack8 would put it (ld_codes = cols rounded up to 32), and the backward pass may be given
+ * those instead of x.  y may be x.
+ *   backward: dx, dweight, dbias may each be NULL; work: tf_layer_norm_work_floats floats of the caller's (NULL if neither dweight nor
+ * dbias is asked for).  Sums over rows are fp32, in an order that depends on the sizes only. */
+long long tf_layer_norm_work_floats(int rows, int cols);
+int tf_layer_norm_fwd(const void *x, long long ld_x, int dtype, const void *weight, const void *bias, int w_dtype, int rows, int cols,
+                      float eps, void *y, long long ld_y, float *mean, float *rstd, signed char *codes, int ld_codes,
+                      unsigned char *exponents, void *stream);
+int tf_layer_norm_bwd(const void *x, long long ld_x, const signed char *codes, int ld_codes, const unsigned char *exponents, int dtype,
+                      const void *weight, int w_dtype, int rows, int cols, const float *mean, const float *rstd, const void *dy,
+                      long long ld_dy, void *dx, long long ld_dx, void *dweight, void *dbias, float *work, long long work_floats,
+                      void *stream);
+
+/* ------------------------------------------------------------------------- */
+/* Activations in 8 bits                                                      */
+/* ------------------------------------------------------------------------- */
+/* 32 neighbouring columns of a row share a power of two: e = floor(log2 max|x|) of the group, one more where the largest value
+ * would round to 128 steps, within [-120, 127]; code = x / 2^(e - 6) rounded to the nearest whole number, ties to even; the
+ * exponent's byte is e + 127, and 255 for a group that holds an infinity or a NaN (its values read back as NaN).
+ * codes [rows][ld_codes] (ld_codes a multiple of 32, 32-byte aligned; columns from `cols` on are written as zero),
+ * exponents [rows][ld_codes / 32].  relu: negative values become zero first, and -128 is the code of a positive value that
+ * rounds to zero (it reads back as zero).
+ *   tf_relu_grad8: grad (in place) becomes zero where the code is zero, i.e. where a value packed with relu was not positive.
+ *   tf_weight_grad8: out[na][nb] = G^T X for G [m][na] and the packed X [m][nb], in G's type; products are exact, sums fp32;
+ * work: tf_weight_grad8_work_floats floats of the caller's, 16-byte aligned; at most 2^26 entries.
+ * Device pointers; the calls only enqueue work on `stream`. */
+int tf_pack8(const void *x, long long ld, int dtype, int rows, int cols, int relu, signed char *codes, int ld_codes,
+             unsigned char *exponents, void *stream);
+int tf_unpack8(const signed char *codes, int ld_codes, const unsigned char *exponents, int dtype, int rows, int cols, void *out,
+               long long ld, void *stream);
+int tf_relu_grad8(const signed char *codes, int ld_codes, int dtype, int rows, int cols, void *grad, long long ld, void *stream);
+long long tf_weight_grad8_work_floats(int m, int na, int nb, int dtype);
+int tf_weight_grad8(const void *g, long long ld_g, int dtype, int na, const signed char *codes, int ld_codes,
+                    const unsigned char *exponents, int nb, int m, void *out, float *work, long long work_floats, void *stream);
+
+/* ------------------------------------------------------------------------- */
 /* Softmax cross entropy of a linear layer                                    */
 /* ------------------------------------------------------------------------- */
 /* loss_i = log sum_v exp(x_i . w_v) - x_i . w_target(i) for rows whose target is not `ignore_index`, without the logits in

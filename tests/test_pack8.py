@@ -1,0 +1,102 @@
+"""Activations in 8 bits (csrc/pack8.cu, pack8.cuh): every step but one rounding is exact, so codes and exponents are compared
+bit by bit with the definition in fp64; and the weight gradient from them (csrc/weight_grad8.cu): exact products, chains of at
+most 24 additions that cut off (2^-23 each) and fp32 sums of at most 2^13 of those: below 24 * 2^-23 + 2^-24 sqrt(2^13) of random
+terms < 5e-6, and half a step u of the result's type.
+"""
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+U = {"float32": 2.0 ** -24, "bfloat16": 2.0 ** -8, "float16": 2.0 ** -11}
+
+
+def reference(x, relu):
+    """Codes, exponent bytes and values by the definition."""
+    import torch
+    n, d = x.shape
+    x = x.double()
+    v = torch.where(x > 0, x, torch.where(x.isnan(), x, 0.0)) if relu else x
+    p = torch.nn.functional.pad(v, (0, -d % 32)).reshape(n, -1, 32)
+    bad = ~p.isfinite().all(2, keepdim=True)
+    top = torch.where(bad, 1.0, p).abs().amax(2, keepdim=True)
+    e = torch.floor(torch.log2(top.clamp(min=2.0 ** -120)))
+    e = torch.where(torch.round(top / torch.exp2(e - 6)) > 127, e + 1, e).clamp(max=127)
+    code = torch.round(torch.where(bad, 0.0, p) / torch.exp2(e - 6)).clamp(-127, 127)
+    value = torch.where(bad, float("nan"), code * torch.exp2(e - 6)).reshape(n, -1)[:, :d]
+    code = torch.where(bad, 0, code).reshape(n, -1)[:, :d]
+    if relu:
+        code = torch.where((x > 0) & (code == 0), -128, code)
+    return code.to(torch.int8), torch.where(bad, 255, e + 127).reshape(n, -1).to(torch.uint8), value
+
+
+def data(n, d, dtype, seed=0):
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(n, d, generator=g, device="cuda") * torch.exp(2 * torch.randn(n, 1, generator=g, device="cuda"))).to(getattr(torch, dtype))
+
+
+def check(x, relu):
+    import torch
+    from tile_fusion_b200 import sw_gcn  # noqa: F401
+    codes, exps = torch.ops.sw_gcn.pack8(x, relu)
+    code, exp, value = reference(x, relu)
+    finite = torch.nn.functional.pad(value, (0, -x.shape[1] % 32)).reshape(x.shape[0], -1, 32).isfinite().all(2) if x.numel() else exp == exp
+    assert torch.equal(exps, exp)
+    assert torch.equal(codes[value.isfinite()], code[value.isfinite()])
+    if relu:
+        assert torch.equal(codes != 0, x > 0)
+    for t in (torch.float32, torch.bfloat16, torch.float16):
+        got = torch.ops.sw_gcn.unpack8(codes, exps, t)
+        assert got.dtype == t
+        want = value.to(t)
+        assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got[~got.isnan()], want[~want.isnan()])
+    assert finite is not None
+
+
+@pytest.mark.parametrize("relu", [False, True])
+@pytest.mark.parametrize("dtype", list(U))
+@pytest.mark.parametrize("n,d", [(1, 1), (1, 32), (3, 33), (17, 100), (1000, 128), (333, 602), (5, 31), (70_001, 16), (2, 5000)])
+def test_codes(built_lib, relu, dtype, n, d):
+    check(data(n, d, dtype, n + d), relu)
+
+
+@pytest.mark.parametrize("relu", [False, True])
+def test_borders(built_lib, relu):
+    """Ties, the largest value next to 128 steps, subnormals, the ends of the range, infinities and NaN, groups of zeros."""
+    import torch
+    x = torch.zeros(12, 64, device="cuda")
+    x[0, :8] = torch.tensor([1.0, 0.5 / 64, 1.5 / 64, 2.5 / 64, -0.5 / 64, -1.5 / 64, 127.5 / 64 - 2 ** -20, 1e-9], device="cuda")
+    x[1, 0], x[1, 1] = 127.5 / 64, 1.5 / 64                        # rounds to 128 steps: one more
+    x[2, 0] = float(torch.tensor(127.5 / 64).nextafter(torch.tensor(0.0)))
+    x[3, 0], x[3, 1] = 2.0 ** -149, -(2.0 ** -149)
+    x[4, 0], x[4, 1] = 2.0 ** -120, 2.0 ** -126
+    x[5, 0], x[5, 1] = torch.finfo(torch.float32).max, -1e38
+    x[6, 0], x[6, 40] = float("inf"), 3.0
+    x[7, 0], x[7, 40] = float("nan"), -3.0
+    x[8, 63] = -float("inf")
+    x[9] = -1.0
+    x[10, 0], x[10, 1] = 2.0 ** -119, 2.0 ** -121
+    check(x, relu)
+
+
+@pytest.mark.parametrize("dtype", list(U))
+@pytest.mark.parametrize("m", [1, 31, 33, 129, 5003])
+@pytest.mark.parametrize("na,nb", [(47, 256), (256, 100), (7, 33), (128, 128), (130, 40), (300, 300), (64, 1), (1, 64), (512, 16)])
+def test_weight_grad(built_lib, dtype, m, na, nb):
+    import torch
+    from tile_fusion_b200 import sw_gcn  # noqa: F401
+    x, g = data(m, nb, dtype, m + na), data(m, na, dtype, nb)
+    codes, exps = torch.ops.sw_gcn.pack8(x, True)
+    want = g.double().t() @ torch.ops.sw_gcn.unpack8(codes, exps).double()
+    first = None
+    for _ in range(2):
+        got = torch.ops.sw_gcn.weight_grad8(g, codes, exps)
+        assert got.dtype == g.dtype and got.shape == (na, nb)
+        # sums beyond the type's range (fp16: some of 5 003 rows of these spreads) are infinities; next to its end either will do
+        top, got64 = torch.finfo(g.dtype).max, got.double()
+        assert torch.equal(got64[want.abs() > 1.001 * top], want[want.abs() > 1.001 * top].sign() * float("inf"))
+        inside = want.abs() < 0.999 * top
+        off = (got64 - want)[inside].norm().item()
+        assert off <= (U[dtype] + 5e-6) * want[inside].norm().item(), off / want[inside].norm().item()
+        assert first is None or torch.equal(got, first)
+        first = got

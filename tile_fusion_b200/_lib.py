@@ -49,7 +49,8 @@ EXPORTS = [
     "tf_comm_from_nccl", "tf_comm_free", "tf_multi_plan", "tf_multi_free", "tf_multi_info", "tf_multi_plan_handle",
     "tf_multi_exec", "tf_multi_status", "tf_multi_trace", "tf_partition_layout", "tf_read_matrix", "tf_read_dense_mtx",
     "tf_schedule_unfused_csr", "tf_schedule_reordered_adj", "tf_rcm_order", "tf_permute_csr",
-    "tf_linear_ce_work_bytes", "tf_linear_ce_fwd", "tf_linear_ce_bwd", "tf_linear_ce_status",
+    "tf_layer_norm_fwd", "tf_layer_norm_bwd", "tf_layer_norm_work_floats", "tf_pack8", "tf_unpack8", "tf_relu_grad8",
+    "tf_weight_grad8", "tf_weight_grad8_work_floats", "tf_linear_ce_work_bytes", "tf_linear_ce_fwd", "tf_linear_ce_bwd", "tf_linear_ce_status",
 ]
 
 _lib = None
@@ -139,6 +140,16 @@ def lib() -> C.CDLL:
     L.tf_permute_csr.argtypes = [i, vp, vp, vp, vp, vp, vp, vp]
     L.tf_read_matrix.argtypes = [C.c_char_p, i, ip, ip, C.POINTER(ll), C.POINTER(vp), C.POINTER(vp), C.POINTER(vp)]
     L.tf_read_dense_mtx.argtypes = [C.c_char_p, ip, ip, C.POINTER(vp)]
+    L.tf_layer_norm_work_floats.argtypes = [i, i]
+    L.tf_layer_norm_work_floats.restype = ll
+    L.tf_layer_norm_fwd.argtypes = [vp, ll, i, vp, vp, i, i, i, C.c_float, vp, ll, vp, vp, vp, i, vp, vp]
+    L.tf_layer_norm_bwd.argtypes = [vp, ll, vp, i, vp, i, vp, i, i, i, vp, vp, vp, ll, vp, ll, vp, vp, vp, ll, vp]
+    L.tf_pack8.argtypes = [vp, ll, i, i, i, i, vp, i, vp, vp]
+    L.tf_unpack8.argtypes = [vp, i, vp, i, i, i, vp, ll, vp]
+    L.tf_relu_grad8.argtypes = [vp, i, i, i, i, vp, ll, vp]
+    L.tf_weight_grad8_work_floats.argtypes = [i, i, i, i]
+    L.tf_weight_grad8_work_floats.restype = ll
+    L.tf_weight_grad8.argtypes = [vp, ll, i, i, vp, i, vp, i, i, vp, vp, ll, vp]
     L.tf_linear_ce_work_bytes.argtypes = [i, i, i, i, i]
     L.tf_linear_ce_work_bytes.restype = ll
     L.tf_linear_ce_fwd.argtypes = [vp, ll, vp, ll, i, vp, i, i, i, ll, i, vp, vp, vp, ll, vp]

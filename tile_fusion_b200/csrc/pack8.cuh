@@ -1,0 +1,57 @@
+// Activations in 8 bits: 32 neighbouring columns of a row share a power of two (the layout of the open MXINT8 format: one
+// exponent byte, e + 127, and signed bytes).
+//
+//   e     floor(log2 max|x|) of the group, in [-120, 127], one more where the largest value would round to 128 steps
+//   code  x / 2^(e - 6), rounded to the nearest whole number (ties to even), in [-127, 127]: off by at most half a step
+//   value code * 2^(e - 6).  Seven bits and a power of two: exact in bf16 and TF32, so that products on the tensor cores read the
+//         values as they are, and scaling by powers of two makes every step above exact in fp32: no rounding but the one.
+// A group that holds an infinity or a NaN has the byte 255, and all its values are NaN.
+// Behind a ReLU codes are never negative, and the byte -128 is free: it stands for a positive value that rounds to zero.  The
+// code says then whether the value was positive, which is what the ReLU's backward pass asks.
+#pragma once
+#include "values.cuh"
+
+namespace tfk {
+
+constexpr int kPackGroup = 32;
+
+__device__ __forceinline__ float pack8_power(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }  // e in [-126, 127]
+
+// The group's exponent from the bits of its largest |value|; 128 for a group that is not finite.
+__device__ __forceinline__ int pack8_exponent(unsigned top) {
+  const int e = (int)(top >> 23) - 127;
+  if (e == 128) return 128;
+  if (e < -120) return -120;
+  return min(127, e + ((top & 0x7fffffu) >= 0x7f0000u ? 1 : 0));
+}
+template <bool RELU> __device__ __forceinline__ float pack8_input(float x) { return RELU ? (x <= 0.f ? 0.f : x) : x; }  // (a NaN stays)
+template <bool RELU> __device__ __forceinline__ int pack8_code(float x, int e) {
+  int q = 0;
+  if (e != 128) q = max(-127, min(127, __float2int_rn(x * pack8_power(6 - e))));
+  return RELU && x > 0.f && q == 0 ? -128 : q;
+}
+__device__ __forceinline__ float unpack8_step(unsigned byte) {  // 2^(e - 6), NaN for 255
+  return byte == 255 ? __int_as_float(0x7fc00000) : __uint_as_float((byte - 6) << 23);
+}
+__device__ __forceinline__ float unpack8_value(int code, float step) { return (float)(code == -128 ? 0 : code) * step; }
+
+// A thread's N neighbouring values (N divides 32), the other lanes of the group holding the rest: codes, and the exponent.
+template <int N, bool RELU> __device__ __forceinline__ int pack8_lanes(const float (&v)[N], int (&code)[N]) {
+  unsigned top = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) top = max(top, __float_as_uint(pack8_input<RELU>(v[i])) & 0x7fffffffu);
+#pragma unroll
+  for (int k = kPackGroup / N / 2; k; k >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, k));
+  const int e = pack8_exponent(top);
+#pragma unroll
+  for (int i = 0; i < N; ++i) code[i] = pack8_code<RELU>(pack8_input<RELU>(v[i]), e);
+  return e;
+}
+template <int N> __device__ __forceinline__ void store_codes(signed char *p, const int (&code)[N]) {
+  Pack<signed char, N> a;
+#pragma unroll
+  for (int i = 0; i < N; ++i) a.v[i] = (signed char)code[i];
+  *reinterpret_cast<Pack<signed char, N> *>(p) = a;
+}
+
+}  // namespace tfk

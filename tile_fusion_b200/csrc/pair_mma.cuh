@@ -91,4 +91,16 @@ __device__ __forceinline__ void tmem_loaded(float (&v)[32]) {
   for (int i = 0; i < 32; ++i) asm volatile("" : "+f"(v[i]));
 }
 
+// 16 of them at a time, loaded when it returns: for kernels whose sums leave no registers for 32.
+__device__ __forceinline__ void tmem_load16(float (&v)[16], unsigned taddr) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+        "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+      : "r"(taddr) : "memory");
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 16; ++i) asm volatile("" : "+f"(v[i]));
+}
+
 }  // namespace tfk

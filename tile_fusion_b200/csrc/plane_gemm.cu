@@ -78,18 +78,6 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// 16 columns of a warp's 32 tensor-memory lanes (32 would leave no registers beside 128 sums).
-__device__ __forceinline__ void pg_tmem_load(float (&v)[16], unsigned taddr) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
-        "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
-      : "r"(taddr) : "memory");
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < 16; ++i) asm volatile("" : "+f"(v[i]));  // (not used before the wait)
-}
-
 struct PgTile { int m0, n0, split; };
 // Tiles of `group` row blocks go through all columns before the next group's: what runs at one time shares rows and columns.
 __device__ __forceinline__ PgTile pg_tile(const PlaneGemmParams &P, int t, int bn) {
@@ -260,7 +248,7 @@ plane_gemm_kernel(const __grid_constant__ CUtensorMap tm_ahi, const __grid_const
 #pragma unroll
         for (int c = 0; c < kCols; c += 16) {
           float v[16];
-          pg_tmem_load(v, lanes + (unsigned)(buf * 256 + c));
+          tmem_load16(v, lanes + (unsigned)(buf * 256 + c));
 #pragma unroll
           for (int q = 0; q < 16; ++q) acc[c + q] += v[q];
         }

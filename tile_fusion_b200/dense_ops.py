@@ -1,6 +1,25 @@
 """Dense operators of a training step beside the fused layers, registered under ``torch.ops.sw_gcn`` (:mod:`.sw_gcn`)::
 
+    torch.ops.sw_gcn.layer_norm(x, weight=None, bias=None, eps=1e-5, checkpoint=False)
+    torch.ops.sw_gcn.pack8(x, relu=False)                      -> codes, exponents
+    torch.ops.sw_gcn.unpack8(codes, exponents, dtype=None)     -> the values they stand for
+    torch.ops.sw_gcn.weight_grad8(grad, codes, exponents)      -> grad.T @ values
+    torch.ops.sw_gcn.fusedGeMMSpMM_ck8(adj, feature, weight, schedule, num_threads, relu=False)
     torch.ops.sw_gcn.linear_cross_entropy(x, weight, target, ignore_index=-100, reduction="mean")
+
+``layer_norm`` is over the last dimension, with the gradients of x, weight and bias; weight and bias have x's type or
+another of the three.  With ``checkpoint`` it keeps x in 8 bits for the backward pass (x itself can be freed): y is the
+same, the gradients are those of the formula at the kept values.
+
+``pack8`` puts activations [rows, columns] into 8 bits: 32 neighbouring columns share a power of two, a value is a whole
+number of steps of its 64th part, the nearest one, at most 127 of them.  ``codes`` is int8 [rows, columns] with rows that
+start on multiples of 32, ``exponents`` uint8 [rows, columns / 32 rounded up]; a group that holds an infinity or a NaN reads
+back as NaN.  With ``relu`` negative values become zero first, and a code of -128 is a positive value that rounds to zero, so
+that ``codes != 0`` says where the value was positive.  ``weight_grad8`` is the weight gradient of a layer whose input was
+packed, in grad's type.  These three carry no graph; ``fusedGeMMSpMM_ck8`` is the layer that uses them:
+``adj @ (h @ weight.T)`` with ``h = feature``, or with ``relu`` ``h = max(feature, 0)``, of which it keeps the 8 bits instead of
+the 32; the forward result and the gradient of feature are those of ``fusedGeMMSpMM``, the weight's gradient is taken at the
+kept values.
 
 ``linear_cross_entropy`` is the softmax cross entropy of ``x @ weight.T`` (weight stored ``[out, in]``, as in the layers)
 against class indices, without the logits in memory, with the gradients of both operands.  Rows whose target is
@@ -43,6 +62,157 @@ def _rows(t):
 def _ld(t):
     """Values from one row to the next (of a single row any number: its own length)."""
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _same_device(name, *tensors):
+    if len({t.device for t in tensors if t is not None}) > 1:
+        raise ValueError(f"sw_gcn.{name}: the tensors must be on one device")
+
+
+def _ptr(t):
+    return t.data_ptr() if t is not None else None
+
+
+def _pack(x, relu):
+    """Codes [rows, columns rounded up to 32] and exponents of a matrix."""
+    n, d = x.shape
+    ld = -(-d // 32) * 32
+    guard, stream = _on(x)
+    with guard:
+        codes = torch.empty((n, ld), device=x.device, dtype=torch.int8)
+        exponents = torch.empty((n, ld // 32), device=x.device, dtype=torch.uint8)
+        _lib.check(_lib.lib().tf_pack8(x.data_ptr(), _ld(x), _DTYPES[x.dtype], n, d, int(relu), codes.data_ptr(), ld, exponents.data_ptr(),
+                                       stream()))
+    return codes, exponents
+
+
+def _packed(name, codes, exponents):
+    """Codes as the library reads them: rows of whole groups of 32 that start on multiples of 32 bytes, and their length."""
+    if not codes.is_cuda or codes.dtype != torch.int8 or codes.dim() != 2 or exponents.dtype != torch.uint8:
+        raise ValueError(f"sw_gcn.{name}: codes must be a CUDA int8 matrix and exponents a uint8 one, as pack8 gives them")
+    n, d = codes.shape
+    ld = -(-d // 32) * 32
+    if d == 0 or tuple(exponents.shape) != (n, ld // 32):
+        raise ValueError(f"sw_gcn.{name}: codes {tuple(codes.shape)} need exponents [{n}, {ld // 32}], not {list(exponents.shape)}")
+    _same_device(name, codes, exponents)
+    room = codes.untyped_storage().nbytes() - codes.storage_offset()
+    if codes.stride(1) != 1 or _ld(codes) < (ld if n > 1 else 0) or (n > 1 and codes.stride(0) != ld) or codes.data_ptr() % 32 or room < n * ld:
+        codes = torch.nn.functional.pad(codes, (0, ld - d)).contiguous()
+    return codes, exponents.contiguous(), ld
+
+
+def pack8(x, relu=False):
+    _check_values("pack8", "x", x)
+    if x.dim() != 2 or x.shape[1] == 0:
+        raise ValueError(f"sw_gcn.pack8: x must be a matrix of at least one column, not {tuple(x.shape)}")
+    codes, exponents = _pack(_rows(x.detach()), relu)
+    return codes[:, :x.shape[1]], exponents
+
+
+def unpack8(codes, exponents, dtype=None):
+    dtype = torch.float32 if dtype is None else dtype
+    if dtype not in _DTYPES:
+        raise ValueError(f"sw_gcn.unpack8: dtype must be float32, bfloat16 or float16, not {dtype}")
+    n, d = codes.shape[0], codes.shape[-1]
+    codes, exponents, ld = _packed("unpack8", codes, exponents)
+    guard, stream = _on(codes)
+    with guard:
+        out = torch.empty((n, d), device=codes.device, dtype=dtype)
+        _lib.check(_lib.lib().tf_unpack8(codes.data_ptr(), ld, exponents.data_ptr(), _DTYPES[dtype], n, d, out.data_ptr(), d, stream()))
+    return out
+
+
+def weight_grad8(grad, codes, exponents):
+    name = "weight_grad8"
+    _check_values(name, "grad", grad)
+    if grad.dim() != 2 or codes.dim() != 2 or grad.shape[0] != codes.shape[0] or grad.shape[1] == 0:
+        raise ValueError(f"sw_gcn.{name}: grad {tuple(grad.shape)} and codes {tuple(codes.shape)} do not chain")
+    m, nb = codes.shape
+    codes, exponents, ld = _packed(name, codes, exponents)
+    _same_device(name, grad, codes)
+    L = _lib.lib()
+    g = _rows(grad.detach())
+    na, code = g.shape[1], _DTYPES[g.dtype]
+    guard, stream = _on(g)
+    with guard:
+        out = torch.empty((na, nb), device=g.device, dtype=g.dtype)
+        work = torch.empty(L.tf_weight_grad8_work_floats(m, na, nb, code), device=g.device, dtype=torch.float32)
+        _lib.check(L.tf_weight_grad8(g.data_ptr(), _ld(g), code, na, codes.data_ptr(), ld, exponents.data_ptr(), nb, m, out.data_ptr(),
+                                     work.data_ptr(), work.numel(), stream()))
+    return out
+
+
+def relu_grad8_(grad, codes):
+    """grad (a contiguous matrix, in place) where the packed value was positive, zero elsewhere."""
+    n, d = grad.shape
+    guard, stream = _on(grad)
+    with guard:
+        _lib.check(_lib.lib().tf_relu_grad8(codes.data_ptr(), codes.shape[1], _DTYPES[grad.dtype], n, d, grad.data_ptr(), d, stream()))
+    return grad
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, checkpoint):
+        L = _lib.lib()
+        xr = _rows(x)
+        w, b = (t.contiguous() if t is not None else None for t in (weight, bias))
+        n, d = xr.shape
+        w_code = _DTYPES[(w if w is not None else b if b is not None else x).dtype]
+        back = any(ctx.needs_input_grad[:3])
+        keep = checkpoint and (ctx.needs_input_grad[0] or ctx.needs_input_grad[1])
+        guard, stream = _on(x)
+        with guard:
+            y = torch.empty((n, d), device=x.device, dtype=x.dtype)
+            mean, rstd = torch.empty((2, n), device=x.device, dtype=torch.float32) if back else (None, None)
+            ld = -(-d // 32) * 32
+            codes = torch.empty((n, ld), device=x.device, dtype=torch.int8) if keep else None
+            exponents = torch.empty((n, ld // 32), device=x.device, dtype=torch.uint8) if keep else None
+            _lib.check(L.tf_layer_norm_fwd(xr.data_ptr(), _ld(xr), _DTYPES[x.dtype], _ptr(w), _ptr(b), w_code, n, d, eps, y.data_ptr(), d,
+                                           _ptr(mean), _ptr(rstd), _ptr(codes), ld, _ptr(exponents), stream()))
+        if back:
+            ctx.save_for_backward(None if keep else xr, codes, exponents, w, mean, rstd)
+        ctx.args = (x.shape, x.dtype, w_code, weight is not None, bias is not None)
+        return y.reshape(x.shape)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        L = _lib.lib()
+        x, codes, exponents, w, mean, rstd = ctx.saved_tensors
+        shape, dtype, w_code, has_w, has_b = ctx.args
+        g = _rows(grad)
+        n, d = g.shape
+        want = ctx.needs_input_grad
+        guard, stream = _on(g)
+        with guard:
+            dx = torch.empty((n, d), device=g.device, dtype=dtype) if want[0] else None
+            w_dtype = next(t for t, c in _DTYPES.items() if c == w_code)
+            dw = torch.empty(d, device=g.device, dtype=w_dtype) if has_w and want[1] else None
+            db = torch.empty(d, device=g.device, dtype=w_dtype) if has_b and want[2] else None
+            sums = dw is not None or db is not None
+            work = torch.empty(L.tf_layer_norm_work_floats(n, d), device=g.device, dtype=torch.float32) if sums else None
+            _lib.check(L.tf_layer_norm_bwd(_ptr(x), _ld(x) if x is not None else d, _ptr(codes), codes.shape[1] if codes is not None else 0,
+                                           _ptr(exponents), _DTYPES[dtype], _ptr(w), w_code, n, d, mean.data_ptr(), rstd.data_ptr(),
+                                           g.data_ptr(), _ld(g), _ptr(dx), d, _ptr(dw), _ptr(db), _ptr(work),
+                                           work.numel() if sums else 0, stream()))
+        return dx.reshape(shape) if dx is not None else None, dw, db, None, None
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, checkpoint=False):
+    name = "layer_norm"
+    _check_values(name, "x", x)
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise ValueError(f"sw_gcn.{name}: x must have a last dimension of at least one value, not {tuple(x.shape)}")
+    for what, t in (("weight", weight), ("bias", bias)):
+        if t is not None:
+            _check_values(name, what, t)
+            if tuple(t.shape) != (x.shape[-1],):
+                raise ValueError(f"sw_gcn.{name}: {what} must have {x.shape[-1]} values, not {tuple(t.shape)}")
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise ValueError(f"sw_gcn.{name}: weight is {weight.dtype}, bias {bias.dtype}")
+    _same_device(name, x, weight, bias)
+    return _LayerNorm.apply(x, weight, bias, float(eps), bool(checkpoint))
 
 
 class _LinearCrossEntropy(torch.autograd.Function):

@@ -11,6 +11,9 @@ Importing this module registers, under the same names and with the same argument
     torch.ops.sw_gcn.unfused_gcn_forward(adj, feature, weight, threads)
     torch.ops.sw_gcn.cachedSpMMGeMM(af, weight, threads)                          -> af @ weight.T
 
+and, beside those of the reference, the dense operators of a training step that :mod:`.dense_ops` describes: ``layer_norm``,
+``pack8`` / ``unpack8`` / ``weight_grad8``, ``fusedGeMMSpMM_ck8`` and ``linear_cross_entropy``.
+
 ``adj`` is a torch sparse-CSR tensor (int32 indices, fp32 values), ``weight`` is stored ``[out, in]`` as the
 reference's layers do (``gcn-e2e-training/FusedGCNLayer.py:10-11``), everything lives on the GPU and the results
 take part in autograd: the backward is the reference's (``src/Functions.cpp:819-1043``, ``:1192-1244``),
@@ -28,6 +31,7 @@ from __future__ import annotations
 
 import numpy as np
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib, api, dense_ops
 
@@ -126,6 +130,42 @@ class _FusedGeMMSpMM(torch.autograd.Function):
         return None, grad_x, grad_w, None
 
 
+class _FusedGeMMSpMMCk8(torch.autograd.Function):
+    """As _FusedGeMMSpMM, optionally behind a ReLU, keeping the layer's input in 8 bits for the weight's gradient."""
+
+    @staticmethod
+    def forward(ctx, adj, feature, weight, relu):
+        x = feature.contiguous().float()
+        if relu:
+            x = torch.relu(x)
+        w = weight.contiguous().float()
+        out = torch.empty((adj.shape[0], w.shape[0]), device=x.device, dtype=torch.float32)
+        _plan(adj, x.shape[1], w.shape[0]).gemm_spmm(x, w, out, w_transposed=True)
+        ctx.adj, ctx.relu = adj, relu
+        keep = ctx.needs_input_grad[2] or (relu and ctx.needs_input_grad[1])
+        ctx.save_for_backward(w, *(dense_ops._pack(feature.contiguous().float(), relu) if keep else (None, None)))
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out):
+        w, codes, exponents = ctx.saved_tensors
+        k = w.shape[1]
+        ag = _spmm(_plan(ctx.adj, k, w.shape[0]), grad_out)
+        grad_x = ag @ w if ctx.needs_input_grad[1] else None
+        if grad_x is not None and ctx.relu:
+            dense_ops.relu_grad8_(grad_x, codes)
+        grad_w = dense_ops.weight_grad8(ag, codes[:, :k], exponents) if ctx.needs_input_grad[2] else None
+        return None, grad_x, grad_w, None
+
+
+def _ck8(adj, feature, weight, schedule, num_threads, relu=False):
+    if feature.dim() != 2 or weight.dim() != 2 or feature.shape[1] != weight.shape[1] or adj.shape[1] != feature.shape[0]:
+        raise ValueError(f"sw_gcn.fusedGeMMSpMM_ck8: adj {tuple(adj.shape)}, feature {tuple(feature.shape)} and weight "
+                         f"{tuple(weight.shape)} do not chain")
+    return _FusedGeMMSpMMCk8.apply(adj, feature, weight, bool(relu))
+
+
 class _CachedSpMMGeMM(torch.autograd.Function):
     """ForwardCachingAF (binding-project/src/Functions.cpp): out = AF W^T for a first layer whose A X is cached."""
 
@@ -169,6 +209,11 @@ _LIB.define("fusedGeMMSpMM_vt_ro(Tensor adj, Tensor feature, Tensor weight, Tens
 _LIB.define("geMMSpMM_f_bw(Tensor adj, Tensor feature, Tensor weight, Tensor[] schedule, int num_threads) -> Tensor")
 _LIB.define("unfused_gcn_forward(Tensor adj, Tensor feature, Tensor weight, int num_threads) -> Tensor")
 _LIB.define("cachedSpMMGeMM(Tensor af, Tensor weight, int num_threads) -> Tensor")
+_LIB.define("fusedGeMMSpMM_ck8(Tensor adj, Tensor feature, Tensor weight, Tensor[] schedule, int num_threads, bool relu=False) -> Tensor")
+_LIB.define("layer_norm(Tensor x, Tensor? weight=None, Tensor? bias=None, float eps=1e-05, bool checkpoint=False) -> Tensor")
+_LIB.define("pack8(Tensor x, bool relu=False) -> (Tensor, Tensor)")
+_LIB.define("unpack8(Tensor codes, Tensor exponents, ScalarType? dtype=None) -> Tensor")
+_LIB.define("weight_grad8(Tensor grad, Tensor codes, Tensor exponents) -> Tensor")
 _LIB.define("linear_cross_entropy(Tensor x, Tensor weight, Tensor target, int ignore_index=-100, str reduction='mean') -> Tensor")
 
 # CompositeImplicitAutograd: the implementations call autograd Functions themselves, as the reference's ops do.
@@ -180,4 +225,9 @@ _LIB.impl("fusedGeMMSpMM_vt_ro", lambda adj, f, w, sched, nt, mts: _FusedGeMMSpM
 _LIB.impl("geMMSpMM_f_bw", lambda adj, f, w, sched, nt: _FusedGeMMSpMM.apply(adj, f, w, False), "CompositeImplicitAutograd")
 _LIB.impl("unfused_gcn_forward", lambda adj, f, w, nt: _FusedGeMMSpMM.apply(adj, f, w, True), "CompositeImplicitAutograd")
 _LIB.impl("cachedSpMMGeMM", lambda af, w, nt: _CachedSpMMGeMM.apply(af, w), "CompositeImplicitAutograd")
+_LIB.impl("fusedGeMMSpMM_ck8", _ck8, "CompositeImplicitAutograd")
+_LIB.impl("layer_norm", dense_ops.layer_norm, "CompositeImplicitAutograd")
+_LIB.impl("pack8", dense_ops.pack8, "CompositeImplicitAutograd")
+_LIB.impl("unpack8", dense_ops.unpack8, "CompositeImplicitAutograd")
+_LIB.impl("weight_grad8", dense_ops.weight_grad8, "CompositeImplicitAutograd")
 _LIB.impl("linear_cross_entropy", dense_ops.linear_cross_entropy, "CompositeImplicitAutograd")
