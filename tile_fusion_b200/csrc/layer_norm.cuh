@@ -1,0 +1,178 @@
+// What the two passes of the layer norm share (layer_norm.cu, layer_norm_grad.cu): how a row lies over threads.
+//
+// A thread holds N neighbouring columns (16 bytes of values) NV times, whatever the rows' alignment: they come and go in pieces of
+// AL values, all N where every row starts on 16 bytes, else two, else one.
+#pragma once
+#include "pack8.cuh"
+#include "tf_internal.h"
+
+namespace tfk {
+
+constexpr int kLnWarpThreads = 256;            // CTAs whose rows have a warp or less
+constexpr int kLnRowThreads = 512;             // the largest CTA of a row: 128 registers a thread
+constexpr int kLnMaxCols = 16384;              // 32 values to each of them
+constexpr int kLnMaxCtas = 148 * 8;
+
+struct LnParams {
+  const void *x; long long ld_x;
+  const void *w, *b; int w_dtype; bool w_whole;  // w_whole: both start on 16 bytes
+  int rows, cols; float eps;
+  void *y; long long ld_y;
+  float *mean, *rstd;
+  signed char *codes; int ld_codes; unsigned char *exps;   // forward: written (null: not); backward: read instead of x
+  const void *dy; long long ld_dy;
+  void *dx; long long ld_dx;
+  float *part;                                             // [CTA][2][cols]
+};
+
+template <class T> constexpr int kLnN = 16 / (int)sizeof(T);
+
+template <class T, int AL> __device__ __forceinline__ Pack<T, kLnN<T>> ln_load(const T *row, int col, int cols, bool in) {
+  constexpr int N = kLnN<T>;
+  Pack<T, N> v;
+#pragma unroll
+  for (int p = 0; p < N; p += AL) {
+    Pack<T, AL> a;
+#pragma unroll
+    for (int k = 0; k < AL; ++k) a.v[k] = from_float<T>(0.f);
+    if (in && col + p < cols) a = *reinterpret_cast<const Pack<T, AL> *>(row + col + p);
+#pragma unroll
+    for (int k = 0; k < AL; ++k) v.v[p + k] = a.v[k];
+  }
+  return v;
+}
+template <class T, int AL> __device__ __forceinline__ void ln_store(T *row, int col, int cols, const float (&v)[kLnN<T>]) {
+  constexpr int N = kLnN<T>;
+#pragma unroll
+  for (int p = 0; p < N; p += AL) {
+    if (col + p >= cols) break;
+    float a[AL];
+#pragma unroll
+    for (int k = 0; k < AL; ++k) a[k] = v[p + k];
+    store_pack<T, AL>(row + col + p, a);
+  }
+}
+// N weights from `col` on, `none` where there are none.
+template <class T> __device__ __forceinline__ void ln_weight(const void *w, const LnParams &P, int col, float none, float (&v)[kLnN<T>]) {
+  constexpr int N = kLnN<T>;
+  if (w && P.w_whole && col + N <= P.cols) {
+    if (P.w_dtype == TF_F32) {
+#pragma unroll
+      for (int k = 0; k < N; k += 4) {
+        const float4 q = __ldg(reinterpret_cast<const float4 *>(static_cast<const float *>(w) + col + k));
+        v[k] = q.x; v[k + 1] = q.y; v[k + 2] = q.z; v[k + 3] = q.w;
+      }
+      return;
+    }
+    const unsigned *u = reinterpret_cast<const unsigned *>(static_cast<const unsigned short *>(w) + col);
+#pragma unroll
+    for (int k = 0; k < N; k += 2) {
+      const unsigned q = __ldg(u + k / 2);
+      if (P.w_dtype == TF_BF16) { v[k] = __uint_as_float(q << 16); v[k + 1] = __uint_as_float(q & 0xffff0000u); }
+      else { const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&q)); v[k] = f.x; v[k + 1] = f.y; }
+    }
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < N; ++k) v[k] = w && col + k < P.cols ? load_value(w, P.w_dtype, col + k) : none;
+}
+
+// K sums over LANES lanes, or (LANES == 0) over the CTA; `slot` alternates between two scratch arrays.
+template <int LANES, int K> __device__ __forceinline__ void ln_sum(float (&v)[K], float (*scratch)[kLnRowThreads / 32][K], int &slot) {
+#pragma unroll
+  for (int k = (LANES ? LANES : 32) / 2; k; k >>= 1)
+#pragma unroll
+    for (int i = 0; i < K; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], k);
+  if (LANES == 0 && blockDim.x > 32) {
+    const int warps = blockDim.x / 32, lane = threadIdx.x & (kLnRowThreads / 32 - 1);  // (both halves of a warp add up all warps)
+    if ((threadIdx.x & 31) == 0)
+#pragma unroll
+      for (int i = 0; i < K; ++i) scratch[slot][threadIdx.x >> 5][i] = v[i];
+    __syncthreads();  // (one to a sum: the scratch array of the sum before last has been read by then)
+#pragma unroll
+    for (int i = 0; i < K; ++i) v[i] = lane < warps ? scratch[slot][lane][i] : 0.f;
+#pragma unroll
+    for (int k = kLnRowThreads / 64; k; k >>= 1)
+#pragma unroll
+      for (int i = 0; i < K; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], k);
+    slot ^= 1;
+  }
+}
+
+// ---- a CTA to a row, several rows a turn, the rows of later turns on their way into shared memory ----
+template <int NV> __host__ __device__ constexpr int ln_rows_at_once() { return NV >= 4 ? 1 : 4 / NV; }
+// turns of rows in flight behind the one at hand (rows of 8 accesses a thread fill the shared memory)
+template <int NV> __host__ __device__ constexpr int ln_ahead() { return NV >= 8 ? 0 : 2; }
+
+// Copies of AL values of a thread into its own shared memory, zeros where there are none.  Below four bytes there is no asynchronous copy.
+template <class T, int AL> __device__ __forceinline__ void ln_copy(Pack<T, kLnN<T>> *to, const T *row, int col, int cols, bool in) {
+  constexpr int N = kLnN<T>, BYTES = AL * (int)sizeof(T);
+  if constexpr (BYTES < 4) *to = ln_load<T, AL>(row, col, cols, in);
+  else {
+    const unsigned dst = (unsigned)__cvta_generic_to_shared(to);
+#pragma unroll
+    for (int p = 0; p < N; p += AL) {
+      const bool here = in && col + p < cols;
+      const T *src = here ? row + col + p : row;  // (nothing is read for a size of zero)
+      if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(here ? 16 : 0) : "memory");
+      else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst + p * (int)sizeof(T)), "l"(src), "n"(BYTES), "r"(here ? BYTES : 0) : "memory");
+    }
+  }
+}
+
+// The rows of a thread that has a warp or less of company, and its columns.
+template <class T, int LANES> struct LnPlace {
+  int t;
+  long long row, step;
+  __device__ LnPlace() {
+    t = threadIdx.x % LANES;
+    row = blockIdx.x * (long long)(blockDim.x / LANES) + threadIdx.x / LANES;
+    step = (long long)gridDim.x * (blockDim.x / LANES);
+  }
+  __device__ int col(int i) const { return (i * LANES + t) * kLnN<T>; }
+  // rows of a warp's lanes end at different times: it goes on as one
+  __device__ bool more(int rows) const { return LANES < 32 ? __any_sync(0xffffffffu, row < rows) : row < rows; }
+};
+
+struct LnShape { int al, nv, lanes, threads; };  // lanes 0: a CTA to a row
+
+inline int ln_align(int cols, int bytes, std::initializer_list<std::pair<const void *, long long>> operands) {
+  for (int al : {16 / bytes, 2}) {
+    bool whole = cols % al == 0;
+    for (const auto &o : operands) whole = whole && (!o.first || (o.second % al == 0 && reinterpret_cast<uintptr_t>(o.first) % (al * bytes) == 0));
+    if (whole) return al;
+  }
+  return 1;
+}
+// Eight lanes to a row where they hold it with 16 values each, a warp where it does (512 columns), a CTA beyond: of as few threads as
+// hold it with one access each up to 256 threads, two or four (fp32 eight) up to 512.
+inline LnShape ln_shape(int al, int cols, int bytes) {
+  const int n = 16 / bytes, vecs = (cols + n - 1) / n, most = 16 / n;
+  auto least = [&](int lanes) { int nv = 1; while (lanes * nv < vecs) nv *= 2; return nv; };
+  if (vecs <= 8 * most) return {al, least(8), 8, kLnWarpThreads};
+  if (vecs <= 32 * most) return {al, least(32), 32, kLnWarpThreads};
+  int nv = 1;
+  while ((vecs + nv - 1) / nv > (nv == 1 ? 256 : kLnRowThreads)) nv *= 2;
+  return {al, nv, 0, ((vecs + nv - 1) / nv + 31) / 32 * 32};
+}
+// CTAs of a launch: as many as fit the device at one time, or as have rows.
+template <class F> cudaError_t ln_ctas(F f, int threads, size_t smem, int rows, int rows_cta, int &ctas) {
+  int each = 1;
+  const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&each, (const void *)f, threads, smem);
+  ctas = std::max(1, std::min((rows + rows_cta - 1) / rows_cta, std::min(kLnMaxCtas, 148 * std::max(1, each))));
+  return e;
+}
+
+// Launches f with as many CTAs as fit the device at one time, or as have rows.
+template <class F> cudaError_t ln_go(F f, const LnShape &s, const LnParams &P, int rows_cta, size_t smem, int &ctas, cudaStream_t st) {
+  cudaError_t e = cudaSuccess;
+  if (smem > 32 * 1024) e = cudaFuncSetAttribute((const void *)f, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+  if (e == cudaSuccess) e = ln_ctas(f, s.threads, smem, P.rows, rows_cta, ctas);
+  if (e != cudaSuccess) return e;
+  f<<<ctas, s.threads, smem, st>>>(P);
+  return cudaGetLastError();
+}
+
+int ln_check(const char *who, int rows, int cols, int dtype, int w_dtype, const void *codes, int ld_codes, const void *exps);
+
+}  // namespace tfk

@@ -12,73 +12,80 @@ namespace {
 
 constexpr int kPackThreads = 256, kPackUnroll = 4;
 
-// The places of a thread in [rows][quads] walked with one stride, without a division at each step.
-struct Walk {
-  long long row;
-  int quad, quads, d_row, d_quad;
-  __device__ Walk(int quads_) : quads(quads_) {
+// The places of a thread in [rows][quads] walked with one stride, without a division at each step.  FLAT: one long row.
+template <bool FLAT> struct Walk {
+  long long row, quad, quads, d_row, d_quad;
+  __device__ Walk(long long quads_) : quads(quads_) {
     const long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x, step = (long long)gridDim.x * blockDim.x;
-    row = i / quads; quad = (int)(i - row * quads);
-    d_row = (int)(step / quads); d_quad = (int)(step - (long long)d_row * quads);
+    if (FLAT) { row = 0; quad = i; d_row = 0; d_quad = step; return; }
+    row = i / quads; quad = i - row * quads;
+    d_row = step / quads; d_quad = step - d_row * quads;
   }
+  __device__ bool in(int rows) const { return FLAT ? quad < quads : row < rows; }
   __device__ void next() {
-    row += d_row; quad += d_quad;
+    quad += d_quad;
+    if (FLAT) return;
+    row += d_row;
     if (quad >= quads) { quad -= quads; ++row; }
   }
 };
 
 // N values a thread; codes [rows][ld_codes], exponents [rows][ld_codes / 32]; columns from `cols` on become zero.
-template <class T, int N, bool RELU>
+// FLAT: rows of whole groups with nothing between them, one row of rows * cols values.
+template <class T, int N, bool RELU, bool FLAT>
 __global__ void __launch_bounds__(kPackThreads)
-pack8_kernel(const T *__restrict__ x, long long ld, int rows, int cols, signed char *__restrict__ codes, int ld_codes, unsigned char *__restrict__ exps) {
-  Walk w(ld_codes / N);
+pack8_kernel(const T *__restrict__ x, long long ld, int rows, long long cols, signed char *__restrict__ codes, long long ld_codes,
+             unsigned char *__restrict__ exps) {
+  Walk<FLAT> w(ld_codes / N);
   // (a warp leaves as one: the lanes of a group are in one row)
-  while (__any_sync(0xffffffffu, w.row < rows)) {
-    long long row[kPackUnroll];
-    int col[kPackUnroll];
-    float v[kPackUnroll][N];
+  while (__any_sync(0xffffffffu, w.in(rows))) {
+    long long to[kPackUnroll];  // where the codes go, or -1
+    Pack<T, N> v[kPackUnroll];
 #pragma unroll
     for (int u = 0; u < kPackUnroll; ++u, w.next()) {
-      row[u] = w.row; col[u] = w.quad * N;
+      const bool in = w.in(rows);
+      const long long col = w.quad * N;
+      to[u] = in ? (FLAT ? col : w.row * ld_codes + col) : -1;
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[u][i] = 0.f;
-      if (row[u] < rows && col[u] < cols) load_pack<T, N>(x + row[u] * ld + col[u], v[u]);
+      for (int i = 0; i < N; ++i) v[u].v[i] = from_float<T>(0.f);
+      if (in && (FLAT || col < cols)) v[u] = *reinterpret_cast<const Pack<T, N> *>(x + (FLAT ? col : w.row * ld + col));
     }
 #pragma unroll
     for (int u = 0; u < kPackUnroll; ++u) {
-      int code[N];
-      const int e = pack8_lanes<N, RELU>(v[u], code);
-      if (row[u] >= rows) continue;
-      store_codes<N>(codes + row[u] * ld_codes + col[u], code);
-      if (col[u] % kPackGroup == 0) exps[row[u] * (ld_codes / kPackGroup) + col[u] / kPackGroup] = (unsigned char)(e + 127);
+      float f[N];
+      unsigned code[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) f[i] = to_float(v[u].v[i]);
+      const int e = pack8_lanes<N, RELU>(f, code);
+      if (to[u] < 0) continue;
+      store_codes<N>(codes + to[u], code);
+      if (to[u] % kPackGroup == 0) exps[to[u] / kPackGroup] = (unsigned char)(e + 127);  // (rows of codes are whole groups)
     }
   }
 }
 
-template <class T, int N>
+template <class T, int N, bool FLAT>
 __global__ void __launch_bounds__(kPackThreads)
-unpack8_kernel(const signed char *__restrict__ codes, int ld_codes, const unsigned char *__restrict__ exps, int rows, int cols, T *__restrict__ out,
-               long long ld) {
-  for (Walk w((cols + N - 1) / N); w.row < rows;) {
-    long long row[kPackUnroll];
-    int col[kPackUnroll];
+unpack8_kernel(const signed char *__restrict__ codes, long long ld_codes, const unsigned char *__restrict__ exps, int rows, long long cols,
+               T *__restrict__ out, long long ld) {
+  for (Walk<FLAT> w(cols / N); w.in(rows);) {
+    long long to[kPackUnroll];
     Pack<signed char, N> c[kPackUnroll];
     unsigned e[kPackUnroll];
 #pragma unroll
     for (int u = 0; u < kPackUnroll; ++u, w.next()) {
-      row[u] = w.row; col[u] = w.quad * N;
-      if (row[u] >= rows) continue;
-      c[u] = *reinterpret_cast<const Pack<signed char, N> *>(codes + row[u] * ld_codes + col[u]);
-      e[u] = __ldg(exps + row[u] * (ld_codes / kPackGroup) + col[u] / kPackGroup);
+      const long long col = w.quad * N, at = FLAT ? col : w.row * ld_codes + col;
+      to[u] = w.in(rows) ? (FLAT ? col : w.row * ld + col) : -1;
+      if (to[u] < 0) continue;
+      c[u] = *reinterpret_cast<const Pack<signed char, N> *>(codes + at);
+      e[u] = __ldg(exps + at / kPackGroup);
     }
 #pragma unroll
     for (int u = 0; u < kPackUnroll; ++u) {
-      if (row[u] >= rows) continue;
-      const float step = unpack8_step(e[u]);
+      if (to[u] < 0) continue;
       float v[N];
-#pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = unpack8_value(c[u].v[i], step);
-      store_pack<T, N>(out + row[u] * ld + col[u], v);
+      unpack8_values<N>(c[u], unpack8_step(e[u]), v);
+      store_pack<T, N>(out + to[u], v);
     }
   }
 }
@@ -87,25 +94,24 @@ unpack8_kernel(const signed char *__restrict__ codes, int ld_codes, const unsign
 template <class T, int N>
 __global__ void __launch_bounds__(kPackThreads)
 mask8_kernel(const signed char *__restrict__ codes, int ld_codes, int rows, int cols, T *__restrict__ grad, long long ld) {
-  for (Walk w((cols + N - 1) / N); w.row < rows;) {
-    long long row[kPackUnroll];
-    int col[kPackUnroll];
+  for (Walk<false> w(cols / N); w.in(rows);) {
+    long long to[kPackUnroll];
     Pack<signed char, N> c[kPackUnroll];
     Pack<T, N> g[kPackUnroll];
 #pragma unroll
     for (int u = 0; u < kPackUnroll; ++u, w.next()) {
-      row[u] = w.row; col[u] = w.quad * N;
-      if (row[u] >= rows) continue;
-      c[u] = *reinterpret_cast<const Pack<signed char, N> *>(codes + row[u] * ld_codes + col[u]);
-      g[u] = *reinterpret_cast<const Pack<T, N> *>(grad + row[u] * ld + col[u]);
+      to[u] = w.in(rows) ? w.row * ld + w.quad * N : -1;
+      if (to[u] < 0) continue;
+      c[u] = *reinterpret_cast<const Pack<signed char, N> *>(codes + w.row * ld_codes + w.quad * N);
+      g[u] = *reinterpret_cast<const Pack<T, N> *>(grad + to[u]);
     }
 #pragma unroll
     for (int u = 0; u < kPackUnroll; ++u) {
-      if (row[u] >= rows) continue;
+      if (to[u] < 0) continue;
 #pragma unroll
       for (int i = 0; i < N; ++i)
         if (c[u].v[i] == 0) g[u].v[i] = from_float<T>(0.f);
-      *reinterpret_cast<Pack<T, N> *>(grad + row[u] * ld + col[u]) = g[u];
+      *reinterpret_cast<Pack<T, N> *>(grad + to[u]) = g[u];
     }
   }
 }
@@ -136,15 +142,22 @@ int check(const char *who, const void *values, long long ld, int dtype, int rows
 template <class T, int N> void launch_pack(const void *x, long long ld, int rows, int cols, signed char *codes, int ld_codes, unsigned char *exps, bool relu,
                                            cudaStream_t s) {
   const unsigned grid = pack_grid((long long)rows * (ld_codes / N));
-  if (relu) pack8_kernel<T, N, true><<<grid, kPackThreads, 0, s>>>((const T *)x, ld, rows, cols, codes, ld_codes, exps);
-  else pack8_kernel<T, N, false><<<grid, kPackThreads, 0, s>>>((const T *)x, ld, rows, cols, codes, ld_codes, exps);
+  if (N >= 4 && ld == cols && cols == ld_codes) {
+    const long long all = (long long)rows * cols;
+    if (relu) pack8_kernel<T, N, true, true><<<grid, kPackThreads, 0, s>>>((const T *)x, all, 1, all, codes, all, exps);
+    else pack8_kernel<T, N, false, true><<<grid, kPackThreads, 0, s>>>((const T *)x, all, 1, all, codes, all, exps);
+  } else if (relu) pack8_kernel<T, N, true, false><<<grid, kPackThreads, 0, s>>>((const T *)x, ld, rows, cols, codes, ld_codes, exps);
+  else pack8_kernel<T, N, false, false><<<grid, kPackThreads, 0, s>>>((const T *)x, ld, rows, cols, codes, ld_codes, exps);
 }
 template <class T, int N> void launch_unpack(const signed char *codes, int ld_codes, const unsigned char *exps, int rows, int cols, void *out, long long ld,
                                              cudaStream_t s) {
-  unpack8_kernel<T, N><<<pack_grid((long long)rows * ((cols + N - 1) / N)), kPackThreads, 0, s>>>(codes, ld_codes, exps, rows, cols, (T *)out, ld);
+  const unsigned grid = pack_grid((long long)rows * (cols / N));
+  const long long all = (long long)rows * cols;
+  if (N >= 4 && ld == cols && cols == ld_codes) unpack8_kernel<T, N, true><<<grid, kPackThreads, 0, s>>>(codes, all, exps, 1, all, (T *)out, all);
+  else unpack8_kernel<T, N, false><<<grid, kPackThreads, 0, s>>>(codes, ld_codes, exps, rows, cols, (T *)out, ld);
 }
 template <class T, int N> void launch_mask(const signed char *codes, int ld_codes, int rows, int cols, void *grad, long long ld, cudaStream_t s) {
-  mask8_kernel<T, N><<<pack_grid((long long)rows * ((cols + N - 1) / N)), kPackThreads, 0, s>>>(codes, ld_codes, rows, cols, (T *)grad, ld);
+  mask8_kernel<T, N><<<pack_grid((long long)rows * (cols / N)), kPackThreads, 0, s>>>(codes, ld_codes, rows, cols, (T *)grad, ld);
 }
 
 }  // namespace

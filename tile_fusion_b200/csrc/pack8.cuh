@@ -25,33 +25,63 @@ __device__ __forceinline__ int pack8_exponent(unsigned top) {
   return min(127, e + ((top & 0x7fffffu) >= 0x7f0000u ? 1 : 0));
 }
 template <bool RELU> __device__ __forceinline__ float pack8_input(float x) { return RELU ? (x <= 0.f ? 0.f : x) : x; }  // (a NaN stays)
-template <bool RELU> __device__ __forceinline__ int pack8_code(float x, int e) {
-  int q = 0;
-  if (e != 128) q = max(-127, min(127, __float2int_rn(x * pack8_power(6 - e))));
-  return RELU && x > 0.f && q == 0 ? -128 : q;
+// The byte of x's code, by adding 1.5 * 2^23: the sum's last bits are the nearest whole number, ties to even (a conversion
+// instruction runs at a quarter of the rate).  `power`: 2^(6 - e).
+template <bool RELU> __device__ __forceinline__ unsigned pack8_code(float x, float power) {
+  const unsigned u = __float_as_uint(fminf(fmaxf(x * power, -127.f), 127.f) + 12582912.f) & 0xffu;
+  return RELU && u == 0 && x > 0.f ? 0x80u : u;
 }
 __device__ __forceinline__ float unpack8_step(unsigned byte) {  // 2^(e - 6), NaN for 255
   return byte == 255 ? __int_as_float(0x7fc00000) : __uint_as_float((byte - 6) << 23);
 }
 __device__ __forceinline__ float unpack8_value(int code, float step) { return (float)(code == -128 ? 0 : code) * step; }
+// Four codes at a time: the byte c as the float 2^23 + 128 + c, less 2^23 + 128 (exact), times the step (exact).
+__device__ __forceinline__ void unpack8_word(unsigned w, float step, float *v) {
+  w = (w & ~__vcmpeq4(w, 0x80808080u)) ^ 0x80808080u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = (__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 + i)) - 8388736.f) * step;
+}
+template <int N> __device__ __forceinline__ void unpack8_values(const Pack<signed char, N> &c, float step, float (&v)[N]) {
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) unpack8_word(*reinterpret_cast<const unsigned *>(&c.v[i]), step, &v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = unpack8_value(c.v[i], step);
+  }
+}
 
 // A thread's N neighbouring values (N divides 32), the other lanes of the group holding the rest: codes, and the exponent.
-template <int N, bool RELU> __device__ __forceinline__ int pack8_lanes(const float (&v)[N], int (&code)[N]) {
+template <int N, bool RELU> __device__ __forceinline__ int pack8_lanes(const float (&v)[N], unsigned (&code)[N]) {
   unsigned top = 0;
 #pragma unroll
   for (int i = 0; i < N; ++i) top = max(top, __float_as_uint(pack8_input<RELU>(v[i])) & 0x7fffffffu);
 #pragma unroll
   for (int k = kPackGroup / N / 2; k; k >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, k));
   const int e = pack8_exponent(top);
+  if (e == 128) {  // the codes say what was positive, no more
 #pragma unroll
-  for (int i = 0; i < N; ++i) code[i] = pack8_code<RELU>(pack8_input<RELU>(v[i]), e);
+    for (int i = 0; i < N; ++i) code[i] = RELU && v[i] > 0.f ? 0x80u : 0u;
+  } else {
+    const float power = pack8_power(6 - e);
+#pragma unroll
+    for (int i = 0; i < N; ++i) code[i] = pack8_code<RELU>(pack8_input<RELU>(v[i]), power);
+  }
   return e;
 }
-template <int N> __device__ __forceinline__ void store_codes(signed char *p, const int (&code)[N]) {
-  Pack<signed char, N> a;
+template <int N> __device__ __forceinline__ void store_codes(signed char *p, const unsigned (&code)[N]) {
+  if constexpr (N % 4 == 0) {
+    Pack<unsigned, N / 4> a;
 #pragma unroll
-  for (int i = 0; i < N; ++i) a.v[i] = (signed char)code[i];
-  *reinterpret_cast<Pack<signed char, N> *>(p) = a;
+    for (int i = 0; i < N / 4; ++i)
+      a.v[i] = __byte_perm(__byte_perm(code[4 * i], code[4 * i + 1], 0x0040), __byte_perm(code[4 * i + 2], code[4 * i + 3], 0x0040), 0x5410);
+    *reinterpret_cast<Pack<unsigned, N / 4> *>(p) = a;
+  } else {
+    Pack<unsigned char, N> a;
+#pragma unroll
+    for (int i = 0; i < N; ++i) a.v[i] = (unsigned char)code[i];
+    *reinterpret_cast<Pack<unsigned char, N> *>(p) = a;
+  }
 }
 
 }  // namespace tfk

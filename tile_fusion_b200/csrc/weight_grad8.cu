@@ -217,13 +217,12 @@ __global__ void __launch_bounds__(kWgThreads, 1) weight_grad8_kernel(const WgPar
       for (int i = 0; i < QX; ++i) {
         const int q = tid + i * 512, r = q / (NT / 8), chunk = q % (NT / 8);
         const float step = unpack8_step(e[i]);
+        float v[8];
+        unpack8_word(x[i].x, step, v);
+        unpack8_word(x[i].y, step, v + 4);
         unsigned u[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const unsigned w = k < 2 ? x[i].x : x[i].y;
-          const int lo = (int)(signed char)(w >> (k & 1) * 16), hi = (int)(signed char)(w >> (k & 1) * 16 + 8);
-          u[k] = pack_pair(unpack8_value(lo, step), unpack8_value(hi, step), false);
-        }
+        for (int k = 0; k < 4; ++k) u[k] = pack_pair(v[2 * k], v[2 * k + 1], false);
         *reinterpret_cast<uint4 *>(base + PLANES * kPlane + chunk / 8 * kWgBlock + r * 128 + ((chunk & 7) ^ (r & 7)) * 16) =
             make_uint4(u[0], u[1], u[2], u[3]);
       }
