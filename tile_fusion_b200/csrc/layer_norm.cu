@@ -58,10 +58,18 @@ template <class T, int NV, class Value, class Col> __device__ __forceinline__ fl
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const Pack<T, kLnN<T>> v = x(i);
+    if (col(i) + kLnN<T> <= cols) {
 #pragma unroll
-    for (int k = 0; k < kLnN<T>; ++k) {
-      const float c = col(i) + k < cols ? to_float(v.v[k]) - mean : 0.f;
-      s = fmaf(c, c, s);
+      for (int k = 0; k < kLnN<T>; ++k) {
+        const float c = to_float(v.v[k]) - mean;
+        s = fmaf(c, c, s);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < kLnN<T>; ++k) {
+        const float c = col(i) + k < cols ? to_float(v.v[k]) - mean : 0.f;
+        s = fmaf(c, c, s);
+      }
     }
   }
   return s;

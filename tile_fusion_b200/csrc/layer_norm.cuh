@@ -100,7 +100,7 @@ template <int LANES, int K> __device__ __forceinline__ void ln_sum(float (&v)[K]
 }
 
 // ---- a CTA to a row, several rows a turn, the rows of later turns on their way into shared memory ----
-template <int NV> __host__ __device__ constexpr int ln_rows_at_once() { return NV >= 4 ? 1 : 4 / NV; }
+template <int NV> __host__ __device__ constexpr int ln_rows_at_once() { return NV >= 4 ? 1 : NV == 2 ? 2 : 4; }
 // turns of rows in flight behind the one at hand (rows of 8 accesses a thread fill the shared memory)
 template <int NV> __host__ __device__ constexpr int ln_ahead() { return NV >= 8 ? 0 : 2; }
 
@@ -144,8 +144,9 @@ inline int ln_align(int cols, int bytes, std::initializer_list<std::pair<const v
   }
   return 1;
 }
-// Eight lanes to a row where they hold it with 16 values each, a warp where it does (512 columns), a CTA beyond: of as few threads as
-// hold it with one access each up to 256 threads, two or four (fp32 eight) up to 512.
+// Eight lanes to a row where they hold it with 16 values each, a warp where it does (512 columns), a CTA beyond: of as many threads as
+// hold it with one access each up to 256, with two, four or (fp32) eight up to 512 (16 384 x 4 096 bf16, forward and backward: 256
+// threads with two 67 and 98 us, 512 with one 74 and 108).
 inline LnShape ln_shape(int al, int cols, int bytes) {
   const int n = 16 / bytes, vecs = (cols + n - 1) / n, most = 16 / n;
   auto least = [&](int lanes) { int nv = 1; while (lanes * nv < vecs) nv *= 2; return nv; };

@@ -114,12 +114,13 @@ __global__ void __launch_bounds__(kLnWarpThreads) ln_backward_kernel(const LnPar
 }
 
 // A CTA to a row, R rows a turn.  Shared memory: [turn][row][NV][thread] of (x or codes), then of dy.
+template <int NV> __host__ __device__ constexpr int ln_grad_rows() { return NV >= 4 ? 1 : 2; }
 template <class T, int NV, bool KEEP8> __host__ __device__ constexpr int ln_turn_bytes(int threads) {
-  return ln_rows_at_once<NV>() * NV * threads * (16 + (KEEP8 ? kLnN<T> : 16));
+  return ln_grad_rows<NV>() * NV * threads * (16 + (KEEP8 ? kLnN<T> : 16));
 }
 template <class T, int AL, int NV, bool KEEP8>
 __global__ void __launch_bounds__(kLnRowThreads, 1) ln_backward_rows_kernel(const LnParams P) {
-  constexpr int N = kLnN<T>, R = ln_rows_at_once<NV>(), AHEAD = ln_ahead<NV>(), TURNS = AHEAD + 1;
+  constexpr int N = kLnN<T>, R = ln_grad_rows<NV>(), AHEAD = ln_ahead<NV>(), TURNS = AHEAD + 1;
   extern __shared__ float4 rows_smem[];
   __shared__ float scratch[2][kLnRowThreads / 32][2 * R];
   using Kept = Pack<signed char, N>;
@@ -161,18 +162,33 @@ __global__ void __launch_bounds__(kLnRowThreads, 1) ln_backward_rows_kernel(cons
 #pragma unroll
   for (int k = 0; k < AHEAD; ++k) fetch(row + k * step, k);
   int turn = 0;
+  // what a row has besides its values comes a turn ahead too
+  float next_mean[R], next_rstd[R];
+  unsigned char next_e[KEEP8 ? R : 1][NV];
+  auto fetch_stats = [&](long long row) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const bool in = row + r < P.rows;
+      next_mean[r] = in ? __ldg(P.mean + row + r) : 0.f;
+      next_rstd[r] = in ? __ldg(P.rstd + row + r) : 0.f;
+      if (KEEP8)
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+          next_e[r][i] = in && col(i) < P.cols ? __ldg(P.exps + (row + r) * (P.ld_codes / kPackGroup) + col(i) / kPackGroup) : 127;
+    }
+  };
+  fetch_stats(row);
   for (; row < P.rows; row += step) {
     float mean[R], rstd[R], unit[KEEP8 ? R : 1][NV], sum[2 * R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const bool in = row + r < P.rows;
-      mean[r] = in ? __ldg(P.mean + row + r) : 0.f;
-      rstd[r] = in ? __ldg(P.rstd + row + r) : 0.f;
+      mean[r] = next_mean[r];
+      rstd[r] = next_rstd[r];
       if (KEEP8)
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
-          unit[r][i] = in && col(i) < P.cols ? unpack8_step(__ldg(P.exps + (row + r) * (P.ld_codes / kPackGroup) + col(i) / kPackGroup)) : 0.f;
+        for (int i = 0; i < NV; ++i) unit[r][i] = unpack8_step(next_e[r][i]);
     }
+    fetch_stats(row + step);
     fetch(row + AHEAD * step, turn == 0 ? AHEAD : turn - 1);  // (a thread has read its part of that turn)
     asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD) : "memory");
     auto hats = [&](int r, int i, float (&xh)[N]) {
@@ -258,7 +274,7 @@ template <class T, int AL, bool KEEP8> cudaError_t ln_by_nv(const LnShape &s, co
 #define TF_LN(NV)                                                                                                                                  \
   if (s.nv == NV) {                                                                                                                                \
     if (s.lanes == 0)                                                                                                                              \
-      return ln_go(ln_backward_rows_kernel<T, AL, NV, KEEP8>, s, P, ln_rows_at_once<NV>(), (ln_ahead<NV>() + 1) * ln_turn_bytes<T, NV, KEEP8>(s.threads), ctas, st); \
+      return ln_go(ln_backward_rows_kernel<T, AL, NV, KEEP8>, s, P, ln_grad_rows<NV>(), (ln_ahead<NV>() + 1) * ln_turn_bytes<T, NV, KEEP8>(s.threads), ctas, st); \
     if constexpr (NV <= 16 / kLnN<T>) {                                                                                                            \
       if (s.lanes == 32) return ln_go(ln_backward_kernel<T, AL, NV, 32, KEEP8>, s, P, kLnWarpThreads / 32, joined, ctas, st);                       \
       return ln_go(ln_backward_kernel<T, AL, NV, 8, KEEP8>, s, P, kLnWarpThreads / 8, joined, ctas, st);                                           \

@@ -24,12 +24,11 @@ __device__ __forceinline__ int pack8_exponent(unsigned top) {
   if (e < -120) return -120;
   return min(127, e + ((top & 0x7fffffu) >= 0x7f0000u ? 1 : 0));
 }
-template <bool RELU> __device__ __forceinline__ float pack8_input(float x) { return RELU ? (x <= 0.f ? 0.f : x) : x; }  // (a NaN stays)
-// The byte of x's code, by adding 1.5 * 2^23: the sum's last bits are the nearest whole number, ties to even (a conversion
-// instruction runs at a quarter of the rate).  `power`: 2^(6 - e).
-template <bool RELU> __device__ __forceinline__ unsigned pack8_code(float x, float power) {
-  const unsigned u = __float_as_uint(fminf(fmaxf(x * power, -127.f), 127.f) + 12582912.f) & 0xffu;
-  return RELU && u == 0 && x > 0.f ? 0x80u : u;
+// A code in the low byte of the result, from x in steps of its group, at most 128 of them: adding 1.5 * 2^23 leaves the nearest whole
+// number in the last bits, ties to even (a conversion instruction runs at a quarter of the rate).
+template <bool RELU> __device__ __forceinline__ unsigned pack8_code(float steps) {
+  if (!RELU) return __float_as_uint(steps + 12582912.f);
+  return steps > 0.f && steps <= 0.5f ? 0x80u : __float_as_uint(fmaxf(steps, 0.f) + 12582912.f);
 }
 __device__ __forceinline__ float unpack8_step(unsigned byte) {  // 2^(e - 6), NaN for 255
   return byte == 255 ? __int_as_float(0x7fc00000) : __uint_as_float((byte - 6) << 23);
@@ -51,21 +50,28 @@ template <int N> __device__ __forceinline__ void unpack8_values(const Pack<signe
   }
 }
 
-// A thread's N neighbouring values (N divides 32), the other lanes of the group holding the rest: codes, and the exponent.
+// A thread's N neighbouring values (N divides 32), the other lanes of the group holding the rest: codes in the low bytes, and the
+// exponent.
 template <int N, bool RELU> __device__ __forceinline__ int pack8_lanes(const float (&v)[N], unsigned (&code)[N]) {
-  unsigned top = 0;
+  float m = 0.f;
+  if constexpr (N == 1) m = RELU ? max3(m, v[0], v[0]) : max3_abs(m, v[0], v[0]);
+  else {
 #pragma unroll
-  for (int i = 0; i < N; ++i) top = max(top, __float_as_uint(pack8_input<RELU>(v[i])) & 0x7fffffffu);
+    for (int i = 0; i < N; i += 2) m = RELU ? max3(m, v[i], v[i + 1]) : max3_abs(m, v[i], v[i + 1]);
+  }
+  unsigned top = __float_as_uint(m) & 0x7fffffffu;  // (a NaN is above the infinity)
 #pragma unroll
   for (int k = kPackGroup / N / 2; k; k >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, k));
   const int e = pack8_exponent(top);
-  if (e == 128) {  // the codes say what was positive, no more
+  if (e >= 127) {  // rare: the last power of two, where 128 steps stay 127, or a group that is not finite: its codes say what was positive
+    const float power = e == 127 ? pack8_power(6 - e) : 0.f;
 #pragma unroll
-    for (int i = 0; i < N; ++i) code[i] = RELU && v[i] > 0.f ? 0x80u : 0u;
+    for (int i = 0; i < N; ++i)
+      code[i] = e == 127 ? pack8_code<RELU>(fminf(fmaxf(v[i] * power, -127.f), 127.f)) : RELU && v[i] > 0.f ? 0x80u : 0u;
   } else {
     const float power = pack8_power(6 - e);
 #pragma unroll
-    for (int i = 0; i < N; ++i) code[i] = pack8_code<RELU>(pack8_input<RELU>(v[i]), power);
+    for (int i = 0; i < N; ++i) code[i] = pack8_code<RELU>(v[i] * power);
   }
   return e;
 }

@@ -55,4 +55,33 @@ template <class T, int N> __device__ __forceinline__ void store_pack(T *p, const
   *reinterpret_cast<Pack<T, N> *>(p) = a;
 }
 
+// As they lie in memory, up to 32 bytes at a time.
+template <class T, int N> __device__ __forceinline__ Pack<T, N> load_raw(const T *p) {
+  if constexpr (sizeof(T) * N == 32) {
+    Pack<T, N> a;
+    unsigned *u = reinterpret_cast<unsigned *>(&a);
+    asm("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+        : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]) : "l"(p));
+    return a;
+  } else return *reinterpret_cast<const Pack<T, N> *>(p);
+}
+template <class T, int N> __device__ __forceinline__ void store_raw(T *p, const Pack<T, N> &a) {
+  if constexpr (sizeof(T) * N == 32) {
+    const unsigned *u = reinterpret_cast<const unsigned *>(&a);
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]),
+                 "r"(u[6]), "r"(u[7]) : "memory");
+  } else *reinterpret_cast<Pack<T, N> *>(p) = a;
+}
+// The largest of |a|, |b|, |c|, or a NaN if one of them is; and of a, b, c.
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {
+  float d;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 }  // namespace tfk
