@@ -1,6 +1,7 @@
 // Activations into 8 bits and back (pack8.cuh), and the ReLU's gradient from the codes.  One pass each, bound by what it reads
 // and writes: a thread takes up to 32 bytes of values at a time, four such in flight.
 #include <algorithm>
+#include <initializer_list>
 #include <string>
 
 #include "pack8.cuh"
@@ -119,9 +120,9 @@ mask8_kernel(const signed char *__restrict__ codes, int ld_codes, int rows, int 
   }
 }
 
-// Values that one access of a thread takes: as many as fill 32 bytes where rows and widths are whole multiples of that, two, or one.
+// Values that one access of a thread takes: as many as fill 32 or 16 bytes where rows and widths are whole multiples of that, two, or one.
 int pack_width(const void *p, long long ld, int cols, int bytes) {
-  for (int n = 32 / bytes; n > 1; n = n > 2 ? 2 : 1)
+  for (int n : {32 / bytes, 16 / bytes, 2})
     if (cols % n == 0 && ld % n == 0 && reinterpret_cast<uintptr_t>(p) % (n * bytes) == 0) return n;
   return 1;
 }
@@ -172,10 +173,10 @@ using namespace tfk;
 // f<type, values of a thread>(arguments) for the operand's type and width
 #define TF_BY_TYPE(f, dtype, n, ...)                                                                              \
   do {                                                                                                            \
-    if (dtype == TF_F32) n == 8 ? f<float, 8>(__VA_ARGS__) : n == 2 ? f<float, 2>(__VA_ARGS__) : f<float, 1>(__VA_ARGS__); \
+    if (dtype == TF_F32) n == 8 ? f<float, 8>(__VA_ARGS__) : n == 4 ? f<float, 4>(__VA_ARGS__) : n == 2 ? f<float, 2>(__VA_ARGS__) : f<float, 1>(__VA_ARGS__); \
     else if (dtype == TF_BF16)                                                                                    \
-      n == 16 ? f<__nv_bfloat16, 16>(__VA_ARGS__) : n == 2 ? f<__nv_bfloat16, 2>(__VA_ARGS__) : f<__nv_bfloat16, 1>(__VA_ARGS__); \
-    else n == 16 ? f<__half, 16>(__VA_ARGS__) : n == 2 ? f<__half, 2>(__VA_ARGS__) : f<__half, 1>(__VA_ARGS__);       \
+      n == 16 ? f<__nv_bfloat16, 16>(__VA_ARGS__) : n == 8 ? f<__nv_bfloat16, 8>(__VA_ARGS__) : n == 2 ? f<__nv_bfloat16, 2>(__VA_ARGS__) : f<__nv_bfloat16, 1>(__VA_ARGS__); \
+    else n == 16 ? f<__half, 16>(__VA_ARGS__) : n == 8 ? f<__half, 8>(__VA_ARGS__) : n == 2 ? f<__half, 2>(__VA_ARGS__) : f<__half, 1>(__VA_ARGS__);       \
   } while (0)
 
 extern "C" int tf_pack8(const void *x, long long ld, int dtype, int rows, int cols, int relu, signed char *codes, int ld_codes,

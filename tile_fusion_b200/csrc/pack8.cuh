@@ -34,16 +34,33 @@ __device__ __forceinline__ float unpack8_step(unsigned byte) {  // 2^(e - 6), Na
   return byte == 255 ? __int_as_float(0x7fc00000) : __uint_as_float((byte - 6) << 23);
 }
 __device__ __forceinline__ float unpack8_value(int code, float step) { return (float)(code == -128 ? 0 : code) * step; }
-// Four codes at a time: the byte c as the float 2^23 + 128 + c, less 2^23 + 128 (exact), times the step (exact).
-__device__ __forceinline__ void unpack8_word(unsigned w, float step, float *v) {
-  w = (w & ~__vcmpeq4(w, 0x80808080u)) ^ 0x80808080u;
+// Four codes at a time.  With c + 128 in a byte (128 where it was zero, which stands for the code zero), that byte behind 2^23 is the
+// float 2^23 + 128 + c; one multiplication and addition leaves c steps, exactly.  The step times 2^23 must be a number: SMALL is for
+// steps up to 2^96; larger ones take the subtraction first.
+__device__ __forceinline__ unsigned unpack8_biased(unsigned w) {
+  w ^= 0x80808080u;
+  const unsigned any = (w & 0x7f7f7f7fu) + 0x7f7f7f7fu;  // top bit of a byte: one of the lower seven is set
+  return w | (~(any | w) & 0x80808080u);
+}
+template <bool SMALL> __device__ __forceinline__ void unpack8_word(unsigned w, float step, float *v) {
+  w = unpack8_biased(w);
+  const float less = -8388736.f * step;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = (__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 + i)) - 8388736.f) * step;
+  for (int i = 0; i < 4; ++i) {
+    const float f = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 + i));
+    v[i] = SMALL ? fmaf(f, step, less) : (f - 8388736.f) * step;
+  }
 }
 template <int N> __device__ __forceinline__ void unpack8_values(const Pack<signed char, N> &c, float step, float (&v)[N]) {
   if constexpr (N % 4 == 0) {
+    const unsigned *w = reinterpret_cast<const unsigned *>(&c);
+    if (fabsf(step) <= 0x1p96f) {  // (a NaN is not)
 #pragma unroll
-    for (int i = 0; i < N; i += 4) unpack8_word(*reinterpret_cast<const unsigned *>(&c.v[i]), step, &v[i]);
+      for (int i = 0; i < N; i += 4) unpack8_word<true>(w[i / 4], step, &v[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; i += 4) unpack8_word<false>(w[i / 4], step, &v[i]);
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = unpack8_value(c.v[i], step);

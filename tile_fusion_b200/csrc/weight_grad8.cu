@@ -3,15 +3,16 @@
 //
 //   * The rows are cut into as many ranges as the device holds CTAs; each adds up a tile of 128 x 256 or 256 x 128 sums (which of
 //     the two: whatever reads less), and a second launch adds the ranges' tiles in order.
-//   * Sixteen warps bring 32 rows at a time from memory through registers into shared memory as 16-bit operands, row by row as they
-//     lie (MN-major, 128-byte swizzle: nothing is transposed), the next 32 rows on their way meanwhile; one warp issues
-//     tcgen05.mma.  A value of X is seven bits and a power of two, exact in bf16.  G in fp32 is three bf16 planes (24 bits, exact), in
+//   * Four teams of four warps each turn 16 rows at a time into 16-bit operands in shared memory, row by row as they lie (MN-major,
+//     128-byte swizzle: nothing is transposed), while further rows are on their way; one warp issues tcgen05.mma.  (All warps on the
+//     same 32 rows wait for one another in every step: 500 009 rows, 47 x 256 bf16: 127 us.)  A value of X is seven bits and a power of two, exact in bf16.  G in fp32 is three bf16 planes (24 bits, exact), in
 //     fp16 two (exact), in bf16 one.  So products lose nothing.
 //   * The tensor core cuts off what it adds to an accumulator, 2e-8 of the sum each time: after 128 rows (at most 24 additions)
 //     the accumulator, one of two, is read and added in registers, where sums round.
 // All waits are bounded: where one runs out the CTA's sums, and with them the result, become NaN.
 #include <algorithm>
 #include <string>
+#include <type_traits>
 
 #include "pack8.cuh"
 #include "pair_mma.cuh"
@@ -21,29 +22,31 @@ namespace tfk {
 
 namespace {
 
-constexpr int kWgWarps = 16, kWgThreads = 32 * (kWgWarps + 1);
-constexpr int kWgRows = 32;                    // of a slice: two K steps of 16
-constexpr int kWgChain = 4;                    // slices added up in tensor memory
+constexpr int kWgWarps = 16;
+__host__ __device__ constexpr int wg_threads(bool ring) { return 32 * (kWgWarps + (ring ? 2 : 1)); }
+constexpr int kWgTeams = 4, kWgTeam = 32 * kWgWarps / kWgTeams;  // teams of four warps, threads of one
+constexpr int kWgRows = 16;                    // of a slice: a K step
+constexpr int kWgChain = 8;                    // slices added up in tensor memory, a multiple of the teams
 constexpr int kWgBlock = kWgRows * 128;        // bytes of 64 columns of a slice
-constexpr int kWgMaxStages = 5;
+constexpr int kWgMaxRing = 16;
 constexpr int kWgSmem = 224 * 1024;
 constexpr int kWgWaitLimit = 1 << 22;
 
 __host__ __device__ constexpr int wg_stage_bytes(int planes, int mt) { return planes * mt * 2 * kWgBlock + (mt == 1 ? 4 : 2) * kWgBlock; }
-__host__ __device__ constexpr int wg_stages(int planes, int mt) {
-  return kWgSmem / wg_stage_bytes(planes, mt) < kWgMaxStages ? kWgSmem / wg_stage_bytes(planes, mt) : kWgMaxStages;
-}
+static_assert(kWgTeams * wg_stage_bytes(3, 2) <= kWgSmem, "a stage to each team");
 
 struct WgParams {
   const void *g; long long ld_g; int na;
   const signed char *codes; int ld_codes, nb; const unsigned char *exps;
   int m, rows;  // rows of a range
   bool whole_g;
+  int ring, g_bytes, ring_bytes;  // slices as they lie in memory that are on their way, bytes of G and of all of one
   float *part;  // [range][na][nb]
 };
 
 struct WgShared {
-  unsigned long long full[kWgMaxStages], empty[kWgMaxStages], acc_full[2], acc_empty[2];
+  unsigned long long raw_full[kWgMaxRing], raw_empty[kWgMaxRing];
+  unsigned long long full[kWgTeams], empty[kWgTeams], acc_full[2], acc_empty[2];
   unsigned tmem_base;
   int dead;
 };
@@ -59,31 +62,54 @@ __device__ __forceinline__ void wg_mma(unsigned d, unsigned long long da, unsign
       "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"(acc) : "memory");
 }
 
-// Eight neighbouring values of a gradient's row, zeros where there are none.
-template <class T> __device__ __forceinline__ void wg_load(const T *row, int col, int cols, bool whole, float (&v)[8]) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = 0.f;
+// Where rows are read from: global memory (a pointer), or places of the ring in shared memory (an address).  Nothing is written there
+// while they are read, but the compiler cannot know: these loads say nothing of memory, so that those of several rows are issued
+// together and not each behind the stores of the row before.  (A place of the ring is read between two barriers; ring_place orders
+// the address itself behind the first.)
+template <class V> __device__ __forceinline__ V wg_read(const char *p) { return __ldg(reinterpret_cast<const V *>(p)); }
+template <class V> __device__ __forceinline__ V wg_read(unsigned a) {
+  V v;
+  if constexpr (sizeof(V) == 16) asm("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  else if constexpr (sizeof(V) == 8) asm("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+  else if constexpr (sizeof(V) == 4) asm("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a));
+  else if constexpr (sizeof(V) == 2) asm("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(a));
+  else {
+    unsigned short u;
+    asm("ld.shared.u8 %0, [%1];" : "=h"(u) : "r"(a));
+    v = (V)u;
+  }
+  return v;
+}
+__device__ __forceinline__ unsigned ring_place(unsigned a) {
+  asm volatile("" : "+r"(a) :: "memory");
+  return a;
+}
+// 16 bytes of neighbouring values of a gradient, zeros where there are none: `n` of them exist.
+template <class T, class At> __device__ __forceinline__ void wg_load(At at, int n, bool whole, float (&v)[16 / sizeof(T)]) {
+  constexpr int W = 16 / sizeof(T);
+  using U = typename std::conditional<sizeof(T) == 4, unsigned, unsigned short>::type;
+  Pack<U, W> a = {};
   if (whole) {
-    if (col < cols) {
-      constexpr int W = 16 / sizeof(T);
-#pragma unroll
-      for (int i = 0; i < 8; i += W) {
-        const Pack<T, W> a = *reinterpret_cast<const Pack<T, W> *>(row + col + i);
-#pragma unroll
-        for (int k = 0; k < W; ++k) v[i + k] = to_float(a.v[k]);
-      }
+    if (n > 0) {
+      const uint4 q = wg_read<uint4>(at);
+      a = reinterpret_cast<const Pack<U, W> &>(q);
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (col + i < cols) v[i] = to_float(row[col + i]);
+    for (int i = 0; i < W; ++i)
+      if (i < n) a.v[i] = wg_read<U>(at + i * (int)sizeof(T));
   }
+#pragma unroll
+  for (int i = 0; i < W; ++i) v[i] = to_float(reinterpret_cast<const T &>(a.v[i]));
 }
 
-template <class T, int PLANES, int MT>
-__global__ void __launch_bounds__(kWgThreads, 1) weight_grad8_kernel(const WgParams P) {
-  constexpr int NT = MT == 1 ? 256 : 128, kPlane = MT * 2 * kWgBlock, kStage = wg_stage_bytes(PLANES, MT), kStages = wg_stages(PLANES, MT);
-  constexpr int QG = MT, QX = NT / 128;  // chunks of eight columns of a thread
+// RING: G and the codes have nothing between their rows and the tile holds all columns, so that 16 rows are one run of bytes each (a
+// multiple of 16, whatever the width): one warp keeps bulk copies of them running ahead through a ring, and what the copies brought
+// is read from shared memory.  Else (more columns than a tile, strided rows) the teams read rows from memory themselves.
+template <class T, int PLANES, int MT, bool RING>
+__global__ void __launch_bounds__(wg_threads(RING), 1) weight_grad8_kernel(const WgParams P) {
+  constexpr int NT = MT == 1 ? 256 : 128, kPlane = MT * 2 * kWgBlock, kStage = wg_stage_bytes(PLANES, MT);
+  constexpr int W = 16 / sizeof(T);  // values of G that a thread takes at a time; of X eight
   extern __shared__ char dyn[];
   __shared__ WgShared s;
   char *smem = reinterpret_cast<char *>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~(uintptr_t)1023);
@@ -94,8 +120,13 @@ __global__ void __launch_bounds__(kWgThreads, 1) weight_grad8_kernel(const WgPar
   const long long r1 = min((long long)P.m, r0 + P.rows);
   const int slices = (int)((r1 - r0 + kWgRows - 1) / kWgRows);
 
+  // columns beyond the operands' stay zero
+  for (int i = tid; i < kWgTeams * kStage / 16; i += wg_threads(RING)) reinterpret_cast<uint4 *>(smem)[i] = make_uint4(0, 0, 0, 0);
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   if (tid == 0) {
-    for (int i = 0; i < kStages; ++i) { mbar_init(&s.full[i], kWgWarps); mbar_init(&s.empty[i], 1); }
+    for (int i = 0; i < kWgTeams; ++i) { mbar_init(&s.full[i], kWgWarps / kWgTeams); mbar_init(&s.empty[i], 1); }
+    if (RING)
+      for (int i = 0; i < P.ring; ++i) { mbar_init(&s.raw_full[i], 1); mbar_init(&s.raw_empty[i], kWgWarps / kWgTeams); }
     for (int i = 0; i < 2; ++i) { mbar_init(&s.acc_full[i], 1); mbar_init(&s.acc_empty[i], kWgWarps); }
     s.dead = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -108,17 +139,45 @@ __global__ void __launch_bounds__(kWgThreads, 1) weight_grad8_kernel(const WgPar
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 
-  if (warp == kWgWarps) {
+  const int whole = RING ? (int)((r1 - r0) / kWgRows) : 0;  // slices of the ring: those with all their rows
+  char *raw = smem + kWgTeams * kStage;
+  if (RING && warp == kWgWarps + 1) {
+    // ---- copies ----
+    int rs = 0, issued = 0;
+    unsigned ph = 0;
+    bool ok = true;
+    for (int sl = 0; sl < whole; ++sl) {
+      if (sl >= P.ring && !(ok = __all_sync(kFull, pair_wait(&s.raw_empty[rs], ph ^ 1u, s.dead, kWgWaitLimit)))) break;
+      if (elect_one()) {
+        const long long row = r0 + (long long)sl * kWgRows;
+        const unsigned to = smem_u32(raw + rs * P.ring_bytes), bar = smem_u32(&s.raw_full[rs]);
+        mbar_expect_tx(&s.raw_full[rs], (unsigned)P.ring_bytes);
+        auto copy = [&](unsigned dst, const void *src, int bytes) {
+          asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
+                       : "memory");
+        };
+        copy(to, static_cast<const T *>(P.g) + row * P.na, P.g_bytes);
+        copy(to + P.g_bytes, P.codes + row * P.ld_codes, kWgRows * P.ld_codes);
+        copy(to + P.g_bytes + kWgRows * P.ld_codes, P.exps + row * (P.ld_codes / kPackGroup), kWgRows * P.ld_codes / kPackGroup);
+      }
+      __syncwarp();
+      if (issued < P.ring) ++issued;
+      if (++rs == P.ring) { rs = 0; ph ^= 1u; }
+    }
+    // a copy still in flight must not outlive the CTA (only after a wait ran out is one possible)
+    if (!ok || s.dead)
+      for (int i = 0; i < issued; ++i)
+        for (int k = 0; k < kWgWaitLimit && !mbar_wait(&s.raw_full[i], i < rs ? ph : ph ^ 1u, 1); ++k) {}
+  } else if (warp == kWgWarps) {
     // ---- products ----
     const unsigned idesc = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (1u << 16) | ((unsigned)(n_pad >> 3) << 17) | ((unsigned)(128 >> 4) << 24);
-    int st = 0;
-    unsigned ph = 0;
     bool ok = true;
     auto wait = [&](unsigned long long *bar, unsigned parity) { return ok = __all_sync(kFull, pair_wait(bar, parity, s.dead, kWgWaitLimit)); };
     for (int sl = 0; sl < slices; ++sl) {
+      const int st = sl % kWgTeams;
       const int chain = sl / kWgChain, buf = chain & 1, in = sl % kWgChain;
       if (in == 0 && chain >= 2 && !wait(&s.acc_empty[buf], (unsigned)(chain / 2 - 1) & 1u)) break;
-      if (!wait(&s.full[st], ph)) break;
+      if (!wait(&s.full[st], (unsigned)(sl / kWgTeams) & 1u)) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const unsigned base = smem_u32(smem + st * kStage);
       const unsigned long long a = wg_desc(base), b = wg_desc(base + PLANES * kPlane);
@@ -128,19 +187,16 @@ __global__ void __launch_bounds__(kWgThreads, 1) weight_grad8_kernel(const WgPar
 #pragma unroll
         for (int p = PLANES - 1; p >= 0; --p)  // the small products first
 #pragma unroll
-          for (int k = 0; k < kWgRows / 16; ++k)
-#pragma unroll
-            for (int t = 0; t < MT; ++t)
-              wg_mma(d + (unsigned)(t * NT), a + (unsigned)((p * kPlane + t * 2 * kWgBlock + k * 2048) >> 4), b + (unsigned)(k * 2048 >> 4), idesc,
-                     in || p != PLANES - 1 || k ? 1u : 0u);
+          for (int t = 0; t < MT; ++t)
+            wg_mma(d + (unsigned)(t * NT), a + (unsigned)((p * kPlane + t * 2 * kWgBlock) >> 4), b, idesc, in || p != PLANES - 1 ? 1u : 0u);
         umma_commit(&s.empty[st]);
         if (last) umma_commit(&s.acc_full[buf]);
       }
       __syncwarp();
-      if (++st == kStages) { st = 0; ph ^= 1u; }
     }
   } else {
-    // ---- rows into operands; and every fourth slice the sums of the four before out of tensor memory ----
+    // ---- rows into operands, every fourth slice to a team; and the sums of the chain before out of tensor memory ----
+    const int team = warp / (kWgWarps / kWgTeams), in_team = tid % kWgTeam;
     const int quadrant = warp & 3, cols0 = (warp >> 2) * 64;  // this thread's row and columns of the accumulator
     float acc[64];
 #pragma unroll
@@ -164,78 +220,99 @@ __global__ void __launch_bounds__(kWgThreads, 1) weight_grad8_kernel(const WgPar
       __syncwarp();
       if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&s.acc_empty[buf])) : "memory");
     };
-    float g[QG][8];
-    uint2 x[QX];
-    unsigned e[QX];
-    auto fetch = [&](int sl) {
-#pragma unroll
-      for (int i = 0; i < QG; ++i) {
-        const int q = tid + i * 512, c = q % (MT * 16) * 8;
-        const long long row = r0 + sl * kWgRows + q / (MT * 16);
-        if (row < r1) wg_load<T>(static_cast<const T *>(P.g) + row * P.ld_g, a0 + c, P.na, P.whole_g, g[i]);
-        else
-#pragma unroll
-          for (int k = 0; k < 8; ++k) g[i][k] = 0.f;
-      }
-#pragma unroll
-      for (int i = 0; i < QX; ++i) {
-        const int q = tid + i * 512, c = b0 + q % (NT / 8) * 8;
-        const long long row = r0 + sl * kWgRows + q / (NT / 8);
-        x[i] = make_uint2(0, 0);
-        e[i] = 127;
-        if (row < r1 && c < P.ld_codes) {
-          x[i] = __ldg(reinterpret_cast<const uint2 *>(P.codes + row * P.ld_codes + c));
-          e[i] = __ldg(P.exps + row * (P.ld_codes / kPackGroup) + c / kPackGroup);
-        }
-      }
-    };
-    int st = 0;
-    unsigned ph = 0;
-    if (slices > 0) fetch(0);
-    for (int sl = 0; sl < slices && ok; ++sl) {
-      if (sl >= kStages && !wait(&s.empty[st], ph ^ 1u)) break;
-      char *base = smem + st * kStage;
-#pragma unroll
-      for (int i = 0; i < QG; ++i) {
-        const int q = tid + i * 512, r = q / (MT * 16), chunk = q % (MT * 16);
-        char *to = base + chunk / 8 * kWgBlock + r * 128 + ((chunk & 7) ^ (r & 7)) * 16;
+    // A thread takes one column chunk of every few rows: a power of two of threads to a row, at least as many as it has chunks.
+    const int chunks_g = (min(MT * 128, P.na - a0) + W - 1) / W, chunks_x = (min(NT, P.ld_codes - b0) + 7) / 8;
+    const int lg = 32 - __clz(chunks_g - 1), lx = 32 - __clz(chunks_x - 1);
+    const int chunk_g = in_team & ((1 << lg) - 1), chunk_x = in_team & ((1 << lx) - 1);
+    const int first_g = chunk_g < chunks_g ? in_team >> lg : kWgRows, first_x = chunk_x < chunks_x ? in_team >> lx : kWgRows;
+    const int step_g = kWgTeam >> lg, step_x = kWgTeam >> lx;
+    const int at_g = chunk_g * W / 8;  // (half a chunk of 16 bytes where a value has four)
+    const int to_g = at_g / 8 * kWgBlock + (W == 4 ? (chunk_g & 1) * 8 : 0), to_x = PLANES * kPlane + chunk_x / 8 * kWgBlock;
+    const int n_g = min(W, P.na - a0 - chunk_g * W), from_x = b0 + chunk_x * 8, from_e = from_x / kPackGroup, ld_e = P.ld_codes / kPackGroup;
+    // `rows` rows of G, codes and exponents that start at the given places, `ld` bytes of G from one to the next, as operands at `base`
+    auto convert = [&](unsigned base, auto pg, auto ld, auto pc, auto pe, int rows) {
+      pg += first_g * ld + (a0 + chunk_g * W) * (int)sizeof(T);
+#pragma unroll 4
+      for (int r = first_g; r < kWgRows; r += step_g, pg += step_g * ld) {
+        float g[W];
+        wg_load<T>(pg, r < rows ? n_g : 0, P.whole_g, g);
+        const unsigned to = base + (unsigned)(to_g + r * 128 + ((at_g ^ r) & 7) * 16);
 #pragma unroll
         for (int p = 0; p < PLANES; ++p) {
-          unsigned u[4];
+          unsigned u[W / 2];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            u[k] = pack_pair(g[i][2 * k], g[i][2 * k + 1], false);
+          for (int k = 0; k < W / 2; ++k) {
+            u[k] = pack_pair(g[2 * k], g[2 * k + 1], false);
             if (p < PLANES - 1) {
-              g[i][2 * k] -= __uint_as_float(u[k] << 16);
-              g[i][2 * k + 1] -= __uint_as_float(u[k] & 0xffff0000u);
+              g[2 * k] -= __uint_as_float(u[k] << 16);
+              g[2 * k + 1] -= __uint_as_float(u[k] & 0xffff0000u);
             }
           }
-          *reinterpret_cast<uint4 *>(to + p * kPlane) = make_uint4(u[0], u[1], u[2], u[3]);
+          if constexpr (W == 8) asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + p * kPlane), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]));
+          else asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(to + p * kPlane), "r"(u[0]), "r"(u[1]));
         }
       }
-#pragma unroll
-      for (int i = 0; i < QX; ++i) {
-        const int q = tid + i * 512, r = q / (NT / 8), chunk = q % (NT / 8);
-        const float step = unpack8_step(e[i]);
+      pc += first_x * P.ld_codes + from_x;
+      pe += first_x * ld_e + from_e;
+#pragma unroll 4
+      for (int r = first_x; r < kWgRows; r += step_x, pc += step_x * P.ld_codes, pe += step_x * ld_e) {
+        uint2 x = make_uint2(0, 0);
+        unsigned e = 127;
+        if (r < rows) {
+          x = wg_read<uint2>(pc);
+          e = wg_read<unsigned char>(pe);
+        }
         float v[8];
-        unpack8_word(x[i].x, step, v);
-        unpack8_word(x[i].y, step, v + 4);
+        unpack8_values<8>(reinterpret_cast<const Pack<signed char, 8> &>(x), unpack8_step(e), v);
         unsigned u[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) u[k] = pack_pair(v[2 * k], v[2 * k + 1], false);
-        *reinterpret_cast<uint4 *>(base + PLANES * kPlane + chunk / 8 * kWgBlock + r * 128 + ((chunk & 7) ^ (r & 7)) * 16) =
-            make_uint4(u[0], u[1], u[2], u[3]);
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(base + (unsigned)(to_x + r * 128 + ((chunk_x ^ r) & 7) * 16)), "r"(u[0]), "r"(u[1]),
+                     "r"(u[2]), "r"(u[3]));
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // read next by the tensor core
+    };
+    auto arrive = [&](unsigned long long *bar) {
       __syncwarp();
-      if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&s.full[st])) : "memory");
-      if (sl + 1 < slices) fetch(sl + 1);
-      if (sl % kWgChain == kWgChain - 1 && sl / kWgChain >= 1) drain(sl / kWgChain - 1);
-      if (++st == kStages) { st = 0; ph ^= 1u; }
-    }
+      if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+    };
+    // (a team keeps to its stage and, the ring being a multiple of the teams, to its places in the ring: no other team's phase passes it by)
     const int chains = (slices + kWgChain - 1) / kWgChain;
-    if (ok && chains >= 2 && slices % kWgChain != 0) drain(chains - 2);
-    if (ok && chains >= 1) drain(chains - 1);
+    int drained = 0, turn = 0, rs = team;
+    unsigned raw_ph = 0;
+    const unsigned stage = smem_u32(smem + team * kStage);
+    for (int sl = team; sl < slices && ok; sl += kWgTeams, ++turn) {
+      if (turn && !wait(&s.empty[team], (unsigned)(turn - 1) & 1u)) break;
+      const long long row = r0 + (long long)sl * kWgRows;
+      if constexpr (RING) {
+        char *at = raw + rs * P.ring_bytes;
+        const bool all = sl < whole;
+        if (all && !wait(&s.raw_full[rs], raw_ph)) break;
+        int rows = kWgRows;
+        if (!all) {  // the last rows: the team copies them itself (what was there it has read, once its warps have met)
+          rows = (int)(r1 - row);
+          asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(kWgTeam) : "memory");
+          T *to = reinterpret_cast<T *>(at);
+          for (int i = in_team; i < rows * P.na; i += kWgTeam) to[i] = static_cast<const T *>(P.g)[row * P.na + i];
+          for (int i = in_team; i < rows * P.ld_codes; i += kWgTeam) at[P.g_bytes + i] = P.codes[row * P.ld_codes + i];
+          const int per = P.ld_codes / kPackGroup;
+          for (int i = in_team; i < rows * per; i += kWgTeam) at[P.g_bytes + kWgRows * P.ld_codes + i] = (char)P.exps[row * per + i];
+          asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(kWgTeam) : "memory");
+        }
+        const unsigned place = ring_place(smem_u32(at));
+        convert(stage, place, (unsigned)(P.na * sizeof(T)), place + P.g_bytes, place + P.g_bytes + kWgRows * P.ld_codes, rows);
+        arrive(&s.raw_empty[rs]);
+        if ((rs += kWgTeams) >= P.ring) { rs = team; raw_ph ^= 1u; }
+      } else
+        convert(stage, static_cast<const char *>(P.g) + row * P.ld_g * (long long)sizeof(T), P.ld_g * (long long)sizeof(T),
+                reinterpret_cast<const char *>(P.codes) + row * P.ld_codes, reinterpret_cast<const char *>(P.exps) + row * ld_e,
+                (int)min((long long)kWgRows, r1 - row));
+      arrive(&s.full[team]);
+      // this team's last slice of a chain: the chain before has been computed, or is about to be
+      const int chain = sl / kWgChain;
+      if (sl % kWgChain >= kWgChain - kWgTeams && chain >= 1) { drain(chain - 1); ++drained; }
+    }
+    while (ok && drained < chains) drain(drained++);
     const int t = MT == 2 ? cols0 / 128 : 0, col = b0 + (MT == 2 ? cols0 % 128 : cols0), row = a0 + t * 128 + quadrant * 32 + lane;
     const bool lost = !ok || *reinterpret_cast<volatile int *>(&s.dead);
     if (row < P.na) {
@@ -300,13 +377,24 @@ WgPlan wg_plan(int m, int na, int nb, int dtype) {
   return p;
 }
 
-template <class T, int PLANES, int MT> cudaError_t wg_launch(const WgPlan &p, const WgParams &P, cudaStream_t s) {
-  auto f = weight_grad8_kernel<T, PLANES, MT>;
-  const int smem = wg_stages(PLANES, MT) * wg_stage_bytes(PLANES, MT) + 1024;
-  const cudaError_t e = cudaFuncSetAttribute((const void *)f, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+template <class T, int PLANES, int MT, bool RING> cudaError_t wg_launch(const WgPlan &p, const WgParams &P, cudaStream_t s) {
+  auto f = weight_grad8_kernel<T, PLANES, MT, RING>;
+  const int smem = kWgTeams * wg_stage_bytes(PLANES, MT) + P.ring * P.ring_bytes + 1024;
+  const cudaError_t e = cudaFuncSetAttribute((const void *)f, cudaFuncAttributeMaxDynamicSharedMemorySize, kWgSmem + 2048);
   if (e != cudaSuccess) return e;
-  f<<<dim3(p.parts, p.tiles_a, p.tiles_b), kWgThreads, smem, s>>>(P);
+  f<<<dim3(p.parts, p.tiles_a, p.tiles_b), wg_threads(RING), smem, s>>>(P);
   return cudaGetLastError();
+}
+template <class T, int PLANES> cudaError_t wg_run(const WgPlan &p, WgParams P, cudaStream_t s) {
+  auto whole = [](const void *q) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0; };
+  P.ring = 0;
+  P.g_bytes = kWgRows * P.na * (int)sizeof(T);
+  P.ring_bytes = P.g_bytes + kWgRows * P.ld_codes + kWgRows * P.ld_codes / kPackGroup;
+  if (P.ld_g == P.na && p.tiles_a == 1 && p.tiles_b == 1 && P.ld_codes <= (p.mt == 1 ? 256 : 128) && whole(P.g) && whole(P.exps))
+    P.ring = std::min(kWgMaxRing, (kWgSmem - kWgTeams * wg_stage_bytes(PLANES, p.mt)) / P.ring_bytes) / kWgTeams * kWgTeams;
+  if (P.ring > 0) return p.mt == 1 ? wg_launch<T, PLANES, 1, true>(p, P, s) : wg_launch<T, PLANES, 2, true>(p, P, s);
+  P.ring = 0;
+  return p.mt == 1 ? wg_launch<T, PLANES, 1, false>(p, P, s) : wg_launch<T, PLANES, 2, false>(p, P, s);
 }
 
 }  // namespace
@@ -334,14 +422,12 @@ extern "C" int tf_weight_grad8(const void *g, long long ld_g, int dtype, int na,
   const WgPlan p = wg_plan(m, na, nb, dtype);
   WgParams P;
   P.g = g; P.ld_g = ld_g; P.na = na; P.codes = codes; P.ld_codes = ld_codes; P.nb = nb; P.exps = exponents; P.m = m; P.rows = p.rows;
-  P.whole_g = na % 8 == 0 && ld_g * value_bytes(dtype) % 16 == 0 && (reinterpret_cast<uintptr_t>(g) & 15) == 0;
+  P.whole_g = na % (16 / value_bytes(dtype)) == 0 && ld_g * value_bytes(dtype) % 16 == 0 && (reinterpret_cast<uintptr_t>(g) & 15) == 0;
   P.part = work;
   cudaStream_t s = (cudaStream_t)stream;
   cudaError_t e = cudaSuccess;
   if (m > 0) {
-    if (dtype == TF_F32) e = p.mt == 1 ? wg_launch<float, 3, 1>(p, P, s) : wg_launch<float, 3, 2>(p, P, s);
-    else if (dtype == TF_F16) e = p.mt == 1 ? wg_launch<__half, 2, 1>(p, P, s) : wg_launch<__half, 2, 2>(p, P, s);
-    else e = p.mt == 1 ? wg_launch<__nv_bfloat16, 1, 1>(p, P, s) : wg_launch<__nv_bfloat16, 1, 2>(p, P, s);
+    e = dtype == TF_F32 ? wg_run<float, 3>(p, P, s) : dtype == TF_F16 ? wg_run<__half, 2>(p, P, s) : wg_run<__nv_bfloat16, 1>(p, P, s);
   }
   if (e == cudaSuccess) {
     const int n = na * nb;
