@@ -42,8 +42,19 @@ _DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _l
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 
 
-def _on(t):
-    return torch.cuda.device(t.device), lambda: torch.cuda.current_stream(t.device).cuda_stream
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
+
+
+def _on_device_of_first(f):
+    """f with the device of its first tensor as the current one, on that device's current stream (given as the last argument)."""
+    def run(t, *args):
+        d = t.get_device()
+        if d == _current_device():
+            return f(t, *args, _raw_stream(d))
+        with torch.cuda.device(d):
+            return f(t, *args, _raw_stream(d))
+    return run
 
 
 def _check_values(name, what, t):
@@ -55,8 +66,11 @@ def _check_values(name, what, t):
 
 def _rows(t):
     """t as [rows, columns] whose rows do not overlap and have their values side by side."""
-    t = t.reshape(-1, t.shape[-1])
-    return t if (t.shape[1] == 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1]) else t.contiguous()
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
+    if t.is_contiguous():
+        return t
+    return t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] else t.contiguous()
 
 
 def _ld(t):
@@ -64,8 +78,14 @@ def _ld(t):
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
+def _records(*tensors):
+    """Whether autograd has to hear of a call with these inputs."""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
 def _same_device(name, *tensors):
-    if len({t.device for t in tensors if t is not None}) > 1:
+    first = tensors[0].device
+    if any(t is not None and t.device != first for t in tensors):
         raise ValueError(f"sw_gcn.{name}: the tensors must be on one device")
 
 
@@ -73,17 +93,41 @@ def _ptr(t):
     return t.data_ptr() if t is not None else None
 
 
-def _pack(x, relu):
+@_on_device_of_first
+def _pack(x, relu, stream):
     """Codes [rows, columns rounded up to 32] and exponents of a matrix."""
     n, d = x.shape
     ld = -(-d // 32) * 32
-    guard, stream = _on(x)
-    with guard:
-        codes = torch.empty((n, ld), device=x.device, dtype=torch.int8)
-        exponents = torch.empty((n, ld // 32), device=x.device, dtype=torch.uint8)
-        _lib.check(_lib.lib().tf_pack8(x.data_ptr(), _ld(x), _DTYPES[x.dtype], n, d, int(relu), codes.data_ptr(), ld, exponents.data_ptr(),
-                                       stream()))
+    codes = torch.empty((n, ld), device=x.device, dtype=torch.int8)
+    exponents = torch.empty((n, ld // 32), device=x.device, dtype=torch.uint8)
+    _lib.check(_lib.lib().tf_pack8(x.data_ptr(), _ld(x), _DTYPES[x.dtype], n, d, int(relu), codes.data_ptr(), ld, exponents.data_ptr(), stream))
     return codes, exponents
+
+
+@_on_device_of_first
+def _unpack(codes, ld, exponents, dtype, n, d, stream):
+    out = torch.empty((n, d), device=codes.device, dtype=dtype)
+    _lib.check(_lib.lib().tf_unpack8(codes.data_ptr(), ld, exponents.data_ptr(), _DTYPES[dtype], n, d, out.data_ptr(), d, stream))
+    return out
+
+
+@_on_device_of_first
+def _weight_grad(g, codes, ld, exponents, nb, stream):
+    L = _lib.lib()
+    m, na, code = g.shape[0], g.shape[1], _DTYPES[g.dtype]
+    out = torch.empty((na, nb), device=g.device, dtype=g.dtype)
+    work = torch.empty(L.tf_weight_grad8_work_floats(m, na, nb, code), device=g.device, dtype=torch.float32)
+    _lib.check(L.tf_weight_grad8(g.data_ptr(), _ld(g), code, na, codes.data_ptr(), ld, exponents.data_ptr(), nb, m, out.data_ptr(),
+                                 work.data_ptr(), work.numel(), stream))
+    return out
+
+
+@_on_device_of_first
+def relu_grad8_(grad, codes, stream):
+    """grad (a contiguous matrix, in place) where the packed value was positive, zero elsewhere."""
+    n, d = grad.shape
+    _lib.check(_lib.lib().tf_relu_grad8(codes.data_ptr(), codes.shape[1], _DTYPES[grad.dtype], n, d, grad.data_ptr(), d, stream))
+    return grad
 
 
 def _packed(name, codes, exponents):
@@ -92,11 +136,11 @@ def _packed(name, codes, exponents):
         raise ValueError(f"sw_gcn.{name}: codes must be a CUDA int8 matrix and exponents a uint8 one, as pack8 gives them")
     n, d = codes.shape
     ld = -(-d // 32) * 32
-    if d == 0 or tuple(exponents.shape) != (n, ld // 32):
+    if d == 0 or exponents.shape != (n, ld // 32):
         raise ValueError(f"sw_gcn.{name}: codes {tuple(codes.shape)} need exponents [{n}, {ld // 32}], not {list(exponents.shape)}")
     _same_device(name, codes, exponents)
-    room = codes.untyped_storage().nbytes() - codes.storage_offset()
-    if codes.stride(1) != 1 or _ld(codes) < (ld if n > 1 else 0) or (n > 1 and codes.stride(0) != ld) or codes.data_ptr() % 32 or room < n * ld:
+    at = codes.storage_offset()
+    if codes.stride(1) != 1 or (n > 1 and codes.stride(0) != ld) or codes.data_ptr() % 32 or codes.untyped_storage().nbytes() - at < n * ld:
         codes = torch.nn.functional.pad(codes, (0, ld - d)).contiguous()
     return codes, exponents.contiguous(), ld
 
@@ -105,8 +149,9 @@ def pack8(x, relu=False):
     _check_values("pack8", "x", x)
     if x.dim() != 2 or x.shape[1] == 0:
         raise ValueError(f"sw_gcn.pack8: x must be a matrix of at least one column, not {tuple(x.shape)}")
-    codes, exponents = _pack(_rows(x.detach()), relu)
-    return codes[:, :x.shape[1]], exponents
+    codes, exponents = _pack(_rows(x), relu)
+    d = x.shape[1]
+    return (codes if codes.shape[1] == d else codes[:, :d]), exponents
 
 
 def unpack8(codes, exponents, dtype=None):
@@ -115,11 +160,7 @@ def unpack8(codes, exponents, dtype=None):
         raise ValueError(f"sw_gcn.unpack8: dtype must be float32, bfloat16 or float16, not {dtype}")
     n, d = codes.shape[0], codes.shape[-1]
     codes, exponents, ld = _packed("unpack8", codes, exponents)
-    guard, stream = _on(codes)
-    with guard:
-        out = torch.empty((n, d), device=codes.device, dtype=dtype)
-        _lib.check(_lib.lib().tf_unpack8(codes.data_ptr(), ld, exponents.data_ptr(), _DTYPES[dtype], n, d, out.data_ptr(), d, stream()))
-    return out
+    return _unpack(codes, ld, exponents, dtype, n, d)
 
 
 def weight_grad8(grad, codes, exponents):
@@ -127,76 +168,62 @@ def weight_grad8(grad, codes, exponents):
     _check_values(name, "grad", grad)
     if grad.dim() != 2 or codes.dim() != 2 or grad.shape[0] != codes.shape[0] or grad.shape[1] == 0:
         raise ValueError(f"sw_gcn.{name}: grad {tuple(grad.shape)} and codes {tuple(codes.shape)} do not chain")
-    m, nb = codes.shape
+    nb = codes.shape[1]
     codes, exponents, ld = _packed(name, codes, exponents)
     _same_device(name, grad, codes)
+    return _weight_grad(_rows(grad), codes, ld, exponents, nb)
+
+
+@_on_device_of_first
+def _layer_norm_forward(xr, w, b, eps, stats, keep, stream):
+    """y, mean and rstd, codes and exponents (None where not asked for)."""
+    n, d = xr.shape
+    first = w if w is not None else b if b is not None else xr
+    y = torch.empty((n, d), device=xr.device, dtype=xr.dtype)
+    s = torch.empty((2, n), device=xr.device, dtype=torch.float32) if stats else None
+    at = s.data_ptr() if stats else None
+    ld = -(-d // 32) * 32
+    codes = torch.empty((n, ld), device=xr.device, dtype=torch.int8) if keep else None
+    exponents = torch.empty((n, ld // 32), device=xr.device, dtype=torch.uint8) if keep else None
+    _lib.check(_lib.lib().tf_layer_norm_fwd(xr.data_ptr(), _ld(xr), _DTYPES[xr.dtype], _ptr(w), _ptr(b), _DTYPES[first.dtype], n, d, eps,
+                                            y.data_ptr(), d, at, at + 4 * n if stats else None, _ptr(codes), ld, _ptr(exponents), stream))
+    return y, s, codes, exponents
+
+
+@_on_device_of_first
+def _layer_norm_backward(g, x, codes, exponents, w, s, dtype, w_dtype, want, stream):
     L = _lib.lib()
-    g = _rows(grad.detach())
-    na, code = g.shape[1], _DTYPES[g.dtype]
-    guard, stream = _on(g)
-    with guard:
-        out = torch.empty((na, nb), device=g.device, dtype=g.dtype)
-        work = torch.empty(L.tf_weight_grad8_work_floats(m, na, nb, code), device=g.device, dtype=torch.float32)
-        _lib.check(L.tf_weight_grad8(g.data_ptr(), _ld(g), code, na, codes.data_ptr(), ld, exponents.data_ptr(), nb, m, out.data_ptr(),
-                                     work.data_ptr(), work.numel(), stream()))
-    return out
-
-
-def relu_grad8_(grad, codes):
-    """grad (a contiguous matrix, in place) where the packed value was positive, zero elsewhere."""
-    n, d = grad.shape
-    guard, stream = _on(grad)
-    with guard:
-        _lib.check(_lib.lib().tf_relu_grad8(codes.data_ptr(), codes.shape[1], _DTYPES[grad.dtype], n, d, grad.data_ptr(), d, stream()))
-    return grad
+    n, d = g.shape
+    dx = torch.empty((n, d), device=g.device, dtype=dtype) if want[0] else None
+    dw = torch.empty(d, device=g.device, dtype=w_dtype) if want[1] else None
+    db = torch.empty(d, device=g.device, dtype=w_dtype) if want[2] else None
+    sums = want[1] or want[2]
+    work = torch.empty(L.tf_layer_norm_work_floats(n, d), device=g.device, dtype=torch.float32) if sums else None
+    at = s.data_ptr()
+    _lib.check(L.tf_layer_norm_bwd(_ptr(x), _ld(x) if x is not None else d, _ptr(codes), codes.shape[1] if codes is not None else 0,
+                                   _ptr(exponents), _DTYPES[dtype], _ptr(w), _DTYPES[w_dtype], n, d, at, at + 4 * n, g.data_ptr(), _ld(g),
+                                   _ptr(dx), d, _ptr(dw), _ptr(db), _ptr(work), work.numel() if sums else 0, stream))
+    return dx, dw, db
 
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, checkpoint):
-        L = _lib.lib()
+        need = ctx.needs_input_grad
         xr = _rows(x)
         w, b = (t.contiguous() if t is not None else None for t in (weight, bias))
-        n, d = xr.shape
-        w_code = _DTYPES[(w if w is not None else b if b is not None else x).dtype]
-        back = any(ctx.needs_input_grad[:3])
-        keep = checkpoint and (ctx.needs_input_grad[0] or ctx.needs_input_grad[1])
-        guard, stream = _on(x)
-        with guard:
-            y = torch.empty((n, d), device=x.device, dtype=x.dtype)
-            mean, rstd = torch.empty((2, n), device=x.device, dtype=torch.float32) if back else (None, None)
-            ld = -(-d // 32) * 32
-            codes = torch.empty((n, ld), device=x.device, dtype=torch.int8) if keep else None
-            exponents = torch.empty((n, ld // 32), device=x.device, dtype=torch.uint8) if keep else None
-            _lib.check(L.tf_layer_norm_fwd(xr.data_ptr(), _ld(xr), _DTYPES[x.dtype], _ptr(w), _ptr(b), w_code, n, d, eps, y.data_ptr(), d,
-                                           _ptr(mean), _ptr(rstd), _ptr(codes), ld, _ptr(exponents), stream()))
-        if back:
-            ctx.save_for_backward(None if keep else xr, codes, exponents, w, mean, rstd)
-        ctx.args = (x.shape, x.dtype, w_code, weight is not None, bias is not None)
-        return y.reshape(x.shape)
+        y, s, codes, exponents = _layer_norm_forward(xr, w, b, eps, True, checkpoint and (need[0] or need[1]))
+        ctx.save_for_backward(xr if codes is None else None, codes, exponents, w, s)
+        ctx.args = (x.shape, x.dtype, next(t for t in (w, b, x) if t is not None).dtype)
+        return y.view(x.shape)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        L = _lib.lib()
-        x, codes, exponents, w, mean, rstd = ctx.saved_tensors
-        shape, dtype, w_code, has_w, has_b = ctx.args
-        g = _rows(grad)
-        n, d = g.shape
-        want = ctx.needs_input_grad
-        guard, stream = _on(g)
-        with guard:
-            dx = torch.empty((n, d), device=g.device, dtype=dtype) if want[0] else None
-            w_dtype = next(t for t, c in _DTYPES.items() if c == w_code)
-            dw = torch.empty(d, device=g.device, dtype=w_dtype) if has_w and want[1] else None
-            db = torch.empty(d, device=g.device, dtype=w_dtype) if has_b and want[2] else None
-            sums = dw is not None or db is not None
-            work = torch.empty(L.tf_layer_norm_work_floats(n, d), device=g.device, dtype=torch.float32) if sums else None
-            _lib.check(L.tf_layer_norm_bwd(_ptr(x), _ld(x) if x is not None else d, _ptr(codes), codes.shape[1] if codes is not None else 0,
-                                           _ptr(exponents), _DTYPES[dtype], _ptr(w), w_code, n, d, mean.data_ptr(), rstd.data_ptr(),
-                                           g.data_ptr(), _ld(g), _ptr(dx), d, _ptr(dw), _ptr(db), _ptr(work),
-                                           work.numel() if sums else 0, stream()))
-        return dx.reshape(shape) if dx is not None else None, dw, db, None, None
+        x, codes, exponents, w, s = ctx.saved_tensors
+        shape, dtype, w_dtype = ctx.args
+        dx, dw, db = _layer_norm_backward(_rows(grad), x, codes, exponents, w, s, dtype, w_dtype, ctx.needs_input_grad[:3])
+        return dx.view(shape) if dx is not None else None, dw, db, None, None
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5, checkpoint=False):
@@ -207,50 +234,58 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, checkpoint=False):
     for what, t in (("weight", weight), ("bias", bias)):
         if t is not None:
             _check_values(name, what, t)
-            if tuple(t.shape) != (x.shape[-1],):
+            if t.shape != x.shape[-1:]:
                 raise ValueError(f"sw_gcn.{name}: {what} must have {x.shape[-1]} values, not {tuple(t.shape)}")
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise ValueError(f"sw_gcn.{name}: weight is {weight.dtype}, bias {bias.dtype}")
     _same_device(name, x, weight, bias)
-    return _LayerNorm.apply(x, weight, bias, float(eps), bool(checkpoint))
+    if _records(x, weight, bias):
+        return _LayerNorm.apply(x, weight, bias, float(eps), bool(checkpoint))
+    w, b = (t.contiguous() if t is not None else None for t in (weight, bias))
+    return _layer_norm_forward(_rows(x), w, b, float(eps), False, False)[0].view(x.shape)
+
+
+@_on_device_of_first
+def _loss_forward(xr, w, t, ignore_index, reduction, stream):
+    L = _lib.lib()
+    n, d, v, code = xr.shape[0], xr.shape[1], w.shape[0], _DTYPES[xr.dtype]
+    loss = torch.empty(n if reduction == 0 else (), device=xr.device, dtype=torch.float32)
+    lse = torch.empty(n, device=xr.device, dtype=torch.float32)
+    work = torch.empty(L.tf_linear_ce_work_bytes(n, d, v, code, 0), device=xr.device, dtype=torch.uint8)
+    _lib.check(L.tf_linear_ce_fwd(xr.data_ptr(), _ld(xr), w.data_ptr(), _ld(w), code, t.data_ptr(), n, d, v, ignore_index, reduction,
+                                  loss.data_ptr(), lse.data_ptr(), work.data_ptr(), work.numel(), stream))
+    return loss, lse
+
+
+@_on_device_of_first
+def _loss_backward(xr, w, t, lse, grad, ignore_index, reduction, want, stream):
+    L = _lib.lib()
+    n, d, v, code = xr.shape[0], xr.shape[1], w.shape[0], _DTYPES[xr.dtype]
+    dx = torch.empty((n, d), device=xr.device, dtype=xr.dtype) if want[0] else None
+    dw = torch.empty((v, d), device=xr.device, dtype=xr.dtype) if want[1] else None
+    work = torch.empty(L.tf_linear_ce_work_bytes(n, d, v, code, 1), device=xr.device, dtype=torch.uint8)
+    _lib.check(L.tf_linear_ce_bwd(xr.data_ptr(), _ld(xr), w.data_ptr(), _ld(w), code, t.data_ptr(), n, d, v, ignore_index, reduction,
+                                  lse.data_ptr(), grad.data_ptr(), _ptr(dx), _ptr(dw), work.data_ptr(), work.numel(), stream))
+    return dx, dw
 
 
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, target, ignore_index, reduction):
-        L = _lib.lib()
         xr, w, t = _rows(x), _rows(weight), target.reshape(-1).to(torch.int64).contiguous()
-        n, d, v = xr.shape[0], xr.shape[1], w.shape[0]
-        code = _DTYPES[x.dtype]
-        guard, stream = _on(x)
-        with guard:
-            loss = torch.empty(n if reduction == 0 else (), device=x.device, dtype=torch.float32)
-            lse = torch.empty(n, device=x.device, dtype=torch.float32)
-            work = torch.empty(L.tf_linear_ce_work_bytes(n, d, v, code, 0), device=x.device, dtype=torch.uint8)
-            _lib.check(L.tf_linear_ce_fwd(xr.data_ptr(), _ld(xr), w.data_ptr(), _ld(w), code, t.data_ptr(), n, d, v, ignore_index,
-                                          reduction, loss.data_ptr(), lse.data_ptr(), work.data_ptr(), work.numel(), stream()))
+        loss, lse = _loss_forward(xr, w, t, ignore_index, reduction)
         ctx.save_for_backward(xr, w, t, lse)
-        ctx.args = (ignore_index, reduction, x.shape, weight.shape)
-        return loss.reshape(target.shape) if reduction == 0 else loss
+        ctx.args = (ignore_index, reduction, x.shape)
+        return loss.view(target.shape) if reduction == 0 else loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        L = _lib.lib()
         xr, w, t, lse = ctx.saved_tensors
-        ignore_index, reduction, x_shape, w_shape = ctx.args
-        n, d, v = xr.shape[0], xr.shape[1], w.shape[0]
-        code = _DTYPES[xr.dtype]
-        guard, stream = _on(xr)
-        with guard:
-            g = grad.reshape(-1).to(torch.float32).contiguous()
-            dx = torch.empty((n, d), device=xr.device, dtype=xr.dtype) if ctx.needs_input_grad[0] else None
-            dw = torch.empty((v, d), device=xr.device, dtype=xr.dtype) if ctx.needs_input_grad[1] else None
-            work = torch.empty(L.tf_linear_ce_work_bytes(n, d, v, code, 1), device=xr.device, dtype=torch.uint8)
-            _lib.check(L.tf_linear_ce_bwd(xr.data_ptr(), _ld(xr), w.data_ptr(), _ld(w), code, t.data_ptr(), n, d, v, ignore_index,
-                                          reduction, lse.data_ptr(), g.data_ptr(), dx.data_ptr() if dx is not None else None,
-                                          dw.data_ptr() if dw is not None else None, work.data_ptr(), work.numel(), stream()))
-        return (dx.reshape(x_shape) if dx is not None else None, dw.reshape(w_shape) if dw is not None else None, None, None, None)
+        ignore_index, reduction, shape = ctx.args
+        g = grad.reshape(-1).to(torch.float32).contiguous()
+        dx, dw = _loss_backward(xr, w, t, lse, g, ignore_index, reduction, ctx.needs_input_grad[:2])
+        return dx.view(shape) if dx is not None else None, dw, None, None, None
 
 
 def linear_cross_entropy(x, weight, target, ignore_index=-100, reduction="mean"):
@@ -267,6 +302,8 @@ def linear_cross_entropy(x, weight, target, ignore_index=-100, reduction="mean")
         raise ValueError(f"sw_gcn.{name}: x is {x.dtype}, weight {weight.dtype}")
     if target.dtype not in (torch.int64, torch.int32) or target.shape != x.shape[:-1]:
         raise ValueError(f"sw_gcn.{name}: target must hold one int64 or int32 class for each row of x")
-    if x.device != weight.device or x.device != target.device:
-        raise ValueError(f"sw_gcn.{name}: x, weight and target must be on one device")
-    return _LinearCrossEntropy.apply(x, weight, target, int(ignore_index), _REDUCTIONS[reduction])
+    _same_device(name, x, weight, target)
+    if _records(x, weight):
+        return _LinearCrossEntropy.apply(x, weight, target, int(ignore_index), _REDUCTIONS[reduction])
+    loss, _ = _loss_forward(_rows(x), _rows(weight), target.reshape(-1).to(torch.int64).contiguous(), int(ignore_index), _REDUCTIONS[reduction])
+    return loss.view(target.shape) if reduction == "none" else loss
