@@ -1,0 +1,85 @@
+"""What the C entry points of the dense operators refuse, without a GPU: nothing is launched for a bad argument."""
+import ctypes as C
+
+import pytest
+
+from tile_fusion_b200 import _lib
+
+P = 4096  # an address that is never followed
+
+
+@pytest.fixture(scope="module")
+def L(built_lib):
+    return _lib.lib()
+
+
+def refused(rc, word=""):
+    assert rc in (_lib.TF_ERR_ARG, _lib.TF_ERR_UNSUPPORTED)
+    assert word in _lib.lib().tf_last_error().decode()
+
+
+def test_layer_norm(L):
+    fwd = lambda **k: L.tf_layer_norm_fwd(*{**dict(x=P, ld=8, t=0, w=None, b=None, wt=0, n=4, d=8, eps=1e-5, y=P, ldy=8, m=None, r=None, c=None, ldc=0, e=None, s=None), **k}.values())  # noqa: E731
+    refused(fwd(t=3), "type")
+    refused(fwd(wt=-1), "type")
+    refused(fwd(n=-1), "size")
+    refused(fwd(d=0), "size")
+    refused(fwd(d=16385, ld=20000, ldy=20000), "columns")
+    refused(fwd(x=None), "null")
+    refused(fwd(ld=7), "overlap")
+    refused(fwd(c=P, ldc=8, e=P), "codes")
+    refused(fwd(c=P + 1, ldc=32, e=P), "codes")
+    refused(fwd(c=P, ldc=32, e=None), "codes")
+    assert fwd(n=0, x=None, y=None) == 0
+    bwd = lambda **k: L.tf_layer_norm_bwd(*{**dict(x=P, ld=8, c=None, ldc=0, e=None, t=0, w=None, wt=0, n=4, d=8, m=P, r=P, dy=P, ldy=8, dx=P, ldx=8, dw=P, db=P, work=P, wn=1 << 20, s=None), **k}.values())  # noqa: E731
+    refused(bwd(m=None), "null")
+    refused(bwd(work=None), "null")
+    refused(bwd(wn=2 * 8 * 4 - 1), "work")
+    refused(bwd(ldx=4), "overlap")
+    refused(bwd(x=None), "null")
+    assert L.tf_layer_norm_work_floats(4, 8) == 64 and L.tf_layer_norm_work_floats(-1, 8) == 0
+
+
+def test_pack8(L):
+    pack = lambda **k: L.tf_pack8(*{**dict(x=P, ld=40, t=0, n=4, d=40, relu=0, c=P, ldc=64, e=P, s=None), **k}.values())  # noqa: E731
+    refused(pack(t=9), "type")
+    refused(pack(d=0), "size")
+    refused(pack(ld=39), "overlap")
+    refused(pack(ldc=40), "groups")
+    refused(pack(ldc=32), "overlap")
+    refused(pack(c=P + 16), "alignment")
+    refused(pack(e=None), "null")
+    assert pack(n=0) == 0
+    refused(L.tf_unpack8(P, 64, None, 0, 4, 40, P, 40, None), "null")
+    refused(L.tf_relu_grad8(P, 64, 0, 4, 40, None, 40, None), "null")
+    grad = lambda **k: L.tf_weight_grad8(*{**dict(g=P, ld=8, t=0, na=8, c=P, ldc=64, e=P, nb=40, m=4, out=P, work=P, wn=1 << 20, s=None), **k}.values())  # noqa: E731
+    refused(grad(g=None), "null")
+    refused(grad(ld=7), "overlap")
+    refused(grad(ldc=48), "groups")
+    refused(grad(wn=1), "work")
+    refused(grad(work=P + 4), "aligned")
+    refused(grad(na=1 << 14, ld=1 << 14, nb=1 << 13, ldc=1 << 13), "entries")
+    assert L.tf_weight_grad8_work_floats(0, 8, 40, 0) >= 8 * 40
+
+
+def test_linear_ce(L):
+    need = L.tf_linear_ce_work_bytes(4, 8, 5, 0, 0)
+    fwd = lambda **k: L.tf_linear_ce_fwd(*{**dict(x=P, ldx=8, w=P, ldw=8, t=0, y=P, n=4, d=8, v=5, ig=-100, red=1, loss=P, lse=P, work=P, wn=need, s=None), **k}.values())  # noqa: E731
+    refused(fwd(t=5), "type")
+    refused(fwd(v=0), "size")
+    refused(fwd(y=None), "null")
+    refused(fwd(ldw=7), "overlap")
+    refused(fwd(red=3), "reduction")
+    refused(fwd(work=P + 16), "aligned")
+    refused(fwd(wn=need - 1), "work")
+    refused(fwd(loss=None), "null")
+    need = L.tf_linear_ce_work_bytes(4, 8, 5, 0, 1)
+    bwd = lambda **k: L.tf_linear_ce_bwd(*{**dict(x=P, ldx=8, w=P, ldw=8, t=0, y=P, n=4, d=8, v=5, ig=-100, red=1, lse=P, g=P, dx=P, dw=P, work=P, wn=need, s=None), **k}.values())  # noqa: E731
+    refused(bwd(lse=None), "null")
+    refused(bwd(g=None), "null")
+    refused(bwd(wn=need - 1), "work")
+    assert bwd(dx=None, dw=None) == 0
+    refused(L.tf_linear_ce_status(None, None), "null")
+    # the slope of a large vocabulary is held in pieces: 8 192 rows of 128 000 classes in bf16 are 2 GB, a piece 256 MB
+    big = L.tf_linear_ce_work_bytes(8192, 4096, 128_000, 1, 1)
+    assert C.c_longlong(big).value < 8192 * 128_000 * 2 / 2 + 3 * 128_000 * 4096

@@ -54,7 +54,8 @@ def run(x, w, b, g, checkpoint=False, eps=1e-5):
 
 def check(x, w, b, g, checkpoint=False):
     import torch
-    u, uw = U[str(x.dtype)[6:]], U[str((w if w is not None else x).dtype)[6:]]
+    # (dw and db are rounded to the type of weight and bias, which is one)
+    u, uw = U[str(x.dtype)[6:]], U[str(next(t for t in (w, b, x) if t is not None).dtype)[6:]]
     kept = torch.ops.sw_gcn.unpack8(*torch.ops.sw_gcn.pack8(x.reshape(-1, x.shape[-1])), torch.float32).reshape(x.shape) if checkpoint else None
     got, want = run(x, w, b, g, checkpoint), reference(x, w, b, g, kept=kept)
     near(got[0], want[0], u + 3e-6)
@@ -82,3 +83,106 @@ def test_values_and_gradients(built_lib, dtype, rows, cols, checkpoint):
         assert got[1].abs().max().item() <= 1e-6 * g.abs().max().item() / 1e-5 ** 0.5
         return
     check(*data((rows, cols), dtype, seed=rows + cols), checkpoint=checkpoint)
+
+
+@pytest.mark.parametrize("dtype,w_dtype", [("float32", "float32"), ("bfloat16", "float32"), ("float16", "float32"), ("float32", "bfloat16"), ("bfloat16", "float16")])
+@pytest.mark.parametrize("cols", [96, 1000])
+def test_weights_of_other_types_and_none(built_lib, dtype, w_dtype, cols):
+    x, w, b, g = data((37, cols), dtype, w_dtype)
+    check(x, w, b, g)
+    check(x, w, None, g)
+    check(x, None, b, g)
+    check(x, None, None, g)
+    check(x, w, None, g, checkpoint=True)
+
+
+@pytest.mark.parametrize("dtype", list(U))
+def test_strides_dimensions_and_empty(built_lib, dtype):
+    import torch
+    from tile_fusion_b200 import sw_gcn  # noqa: F401
+    x, w, b, g = data((4, 6, 50), dtype)
+    check(x, w, b, g)
+    want = run(x.reshape(24, 50), w, b, g.reshape(24, 50))
+    wide = torch.zeros(24, 61, device="cuda", dtype=x.dtype)
+    wide[:, 5:55] = x.reshape(24, 50)
+    for xs, gs in ((wide[:, 5:55], g.reshape(24, 50)), (x.reshape(24, 50).t().contiguous().t(), g.reshape(24, 50).t().contiguous().t()), (x.reshape(24, 50), g.reshape(24, 50)[:, :])):
+        for p, q in zip(run(xs, w, b, gs), want):
+            assert torch.equal(p, q)
+    row = run(x[0, 0], w, b, g[0, 0])
+    assert row[0].shape == (50,) and torch.equal(row[0], want[0][0])
+    shared = run(x.reshape(24, 50), w, b, g[0, :1].expand(24, 50))  # one gradient for all rows
+    near(shared[3], 24 * g[0, 0].double(), U[dtype] + 5e-6)
+    y, dx, dw, db = run(x.reshape(24, 50)[:0], w, b, g.reshape(24, 50)[:0])
+    assert y.shape == (0, 50) and dx.shape == (0, 50) and (dw == 0).all() and (db == 0).all()
+
+
+def test_far_from_zero_and_bad_rows(built_lib):
+    """Rows whose mean is 2 000 times their spread keep their variance (centred values), constant rows give the bias, and a row that
+    is not finite leaves the others alone."""
+    import torch
+    x, w, b, g = data((64, 256), "float32")
+    far = x + 2000
+    # x is off by 2^-13 in units of 1 (its own rounding, which the reference has too); the mean by 2^-13 more at most
+    near(run(far, w, b, g)[0], reference(far, w, b, g)[0], 2.0 ** -13)
+    flat = torch.full_like(x, 3.25)
+    y, dx, _, _ = run(flat, w, b, g)
+    assert torch.equal(y, b.expand_as(y)) and dx.isfinite().all()
+    bad = x.clone()
+    bad[5] = float("nan")
+    bad[9, 3] = float("inf")
+    keep = [i for i in range(64) if i not in (5, 9)]
+    got, want = run(bad, w, b, g), run(x, w, b, g)
+    assert torch.equal(got[0][keep], want[0][keep]) and torch.equal(got[1][keep], want[1][keep])
+    assert got[0][[5, 9]].isnan().all()
+
+
+def test_against_differences(built_lib):
+    import torch
+    x, w, b, g = data((10, 40), "float32")
+    _, dx, dw, db = run(x, w, b, g)
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    f = lambda x, w, b: (run(x, w, b, g)[0].double() * g.double()).sum().item()  # noqa: E731
+    for i, grad in enumerate((dx, dw, db)):
+        u = torch.randn(grad.shape, generator=gen, device="cuda")
+        u /= u.norm()
+        h, at = 2.0 ** -6, [x, w, b]
+        up, down = list(at), list(at)
+        up[i], down[i] = at[i] + h * u, at[i] - h * u
+        # y carries 2^-22 in 400 terms of about one: 1e-5 over 2 h; the third-order term is h^2 of a derivative of order one
+        assert abs((f(*up) - f(*down)) / (2 * h) - (grad.double() * u).sum().item()) <= 2e-3 * grad.norm().item() + 1e-3
+
+
+def test_streams_and_graphs(built_lib):
+    import torch
+    from tile_fusion_b200 import sw_gcn  # noqa: F401
+    x, w, b, g = data((200, 640), "bfloat16")
+    want = run(x, w, b, g, True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = run(x, w, b, g, True)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+    xs, ws, bs = (t.clone().requires_grad_() for t in (x, w, b))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = torch.ops.sw_gcn.layer_norm(xs, ws, bs, 1e-5, True)
+        grads = torch.autograd.grad(y, (xs, ws, bs), g)
+    x2 = data((200, 640), "bfloat16", seed=7)[0]
+    for a, want_ in ((x2, run(x2, w, b, g, True)), (x, want)):
+        with torch.no_grad():
+            xs.copy_(a)
+        graph.replay()
+        assert all(torch.equal(p, q) for p, q in zip((y.detach(), *grads), want_))
+
+
+def test_refusals(built_lib):
+    import torch
+    from tile_fusion_b200 import _lib, sw_gcn  # noqa: F401
+    call = torch.ops.sw_gcn.layer_norm
+    x, w, b, g = data((4, 16), "float32")
+    for args in ((x.cpu(),), (x.double(),), (x, w[:8]), (x, w, b[:8]), (x, w.cpu()), (x, w, b.bfloat16()), (x[:, :0],), (x, w.long())):
+        with pytest.raises(ValueError):
+            call(*args)
+    with pytest.raises(_lib.TileFusionError, match="columns"):
+        call(torch.zeros(2, 16_385, device="cuda"))

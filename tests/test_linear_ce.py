@@ -78,3 +78,144 @@ def test_loss_and_gradients(built_lib, dtype, n, d, v):
     near(dw, ww, U[dtype])
     again = run(x, w, t, grad=torch.tensor(scale, device="cuda"))
     assert torch.equal(again[0], loss) and torch.equal(again[1], dx) and torch.equal(again[2], dw)
+
+
+# several pieces of the vocabulary, sums cut in parts, and the reductions
+@pytest.mark.parametrize("n,d,v,dtype", [(4096, 64, 70_001, "bfloat16"), (3000, 40, 50_000, "float32"), (9000, 72, 33, "float16")])
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_pieces_and_reductions(built_lib, n, d, v, dtype, reduction):
+    import torch
+    x, w, t = make(n, d, v, dtype)
+    g = torch.linspace(-1, 2, n, device="cuda") if reduction == "none" else torch.tensor(64.0 if reduction == "mean" else 0.25, device="cuda")
+    loss, dx, dw = run(x, w, t, reduction, g)
+    want, wx, ww = reference(x, w, t, reduction, g)
+    assert loss.shape == want.shape
+    assert (loss.double() - want).abs().max().item() <= 2e-5 * (n if reduction == "sum" else 1)
+    near(dx, wx, U[dtype])
+    near(dw, ww, U[dtype])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rows_that_do_not_count_reach_nothing(built_lib, dtype):
+    import torch
+    x, w, t = make(300, 64, 130, dtype)
+    clean = run(x, w, t)
+    bad = t == -100
+    assert bad.any()
+    x2 = x.clone()
+    x2[bad] = float("nan")
+    x2[bad.nonzero()[0]] = float("inf")
+    for a, b in zip(run(x2, w, t), clean):
+        assert torch.equal(a, b)
+    assert (clean[1][bad] == 0).all()
+    none = torch.full_like(t, -100)
+    loss, dx, dw = run(x2, w, none)
+    assert loss.item() == 0 and (dx == 0).all() and (dw == 0).all()
+    loss, dx, dw = run(x2, w, none, "none", torch.ones(300, device="cuda"))
+    assert (loss == 0).all() and (dx == 0).all() and (dw == 0).all()
+
+
+def test_classes_outside_are_seen(built_lib):
+    import torch
+    x, w, t = make(50, 32, 10, "float32", ignored=0)
+    t[7], t[9] = 10, -3
+    loss, dx, _ = run(x, w, t, "none", torch.ones(50, device="cuda"))
+    assert loss.isnan().nonzero().flatten().tolist() == [7, 9]
+    assert dx.isnan().any(1).nonzero().flatten().tolist() == [7, 9]
+
+
+@pytest.mark.parametrize("big", [1e-25, 1e-6, 1e12])
+def test_magnitudes(built_lib, big):
+    """fp32 operands of any magnitude: the planes' powers of two follow the largest value."""
+    x, w, t = make(200, 96, 300, "float32")
+    loss, dx, dw = run(x * big, w / big, t)
+    want, wx, ww = reference(x * big, w / big, t)
+    assert abs(loss.double() - want).item() <= 2e-5
+    near(dx, wx, U["float32"])
+    near(dw, ww, U["float32"])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_strides_dimensions_and_index_types(built_lib, dtype):
+    import torch
+    x, w, t = make(60, 48, 70, dtype)
+    want = run(x, w, t)
+    wide = torch.zeros(60, 57, device="cuda", dtype=x.dtype)
+    wide[:, 3:51] = x
+    from tile_fusion_b200 import sw_gcn  # noqa: F401
+    call = torch.ops.sw_gcn.linear_cross_entropy
+    for xs, ws, ts in ((wide[:, 3:51], w, t), (x, w.t().contiguous().t(), t.int()), (x.reshape(3, 20, 48), w, t.reshape(3, 20)), (x.flip(0).flip(0), w, t)):
+        xs, ws = xs.detach().requires_grad_(), ws.detach().requires_grad_()
+        loss = call(xs, ws, ts)
+        gx, gw = torch.autograd.grad(loss, (xs, ws))
+        assert torch.equal(loss, want[0]) and torch.equal(gx.reshape(60, 48), want[1]) and torch.equal(gw, want[2])
+    one = x[:1].expand(60, 48).detach().requires_grad_()  # rows that are one row in memory
+    loss = call(one, w, t)
+    assert abs(loss.double() - reference(x[:1].expand(60, 48), w, t)[0]).item() <= 2e-5
+    with torch.no_grad():
+        assert torch.equal(call(x, w, t), want[0])
+    only = w.detach().requires_grad_()
+    assert torch.equal(torch.autograd.grad(call(x, only, t), only)[0], want[2])
+    only = x.detach().requires_grad_()
+    assert torch.equal(torch.autograd.grad(call(only, w, t), only)[0], want[1])
+    empty = call(x[:0], w, t[:0])
+    assert empty.item() == 0
+    none = torch.full((60,), 7, device="cuda")
+    assert call(x, w, none, 7).item() == 0 and call(x, w, none, 7, "none").shape == (60,)
+
+
+def test_against_differences(built_lib):
+    """The gradient along a direction, and the loss to both sides of it: in fp32 losses carry 1e-6, a step of 1/32 leaves 4e-4 of a
+    third-order term."""
+    import torch
+    x, w, t = make(100, 32, 50, "float32")
+    _, dx, dw = run(x, w, t)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    for a, grad in (("x", dx), ("w", dw)):
+        u = torch.randn(grad.shape, generator=g, device="cuda")
+        u /= u.norm()
+        h = 1 / 32
+        f = lambda s: run(x + s * u if a == "x" else x, w + s * u if a == "w" else w, t, "sum")[0].double()  # noqa: E731
+        number = int((t != -100).sum())
+        assert abs(((f(h) - f(-h)) / (2 * h) / number).item() - (grad * u).sum().item()) <= 2e-3 * grad.norm().item() + 1e-4 / number
+
+
+def test_streams_and_graphs(built_lib):
+    import torch
+    from tile_fusion_b200 import sw_gcn  # noqa: F401
+    x, w, t = make(300, 64, 500, "float32")
+    want = run(x, w, t)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = run(x, w, t)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    xs, ws = x.clone().requires_grad_(), w.clone().requires_grad_()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss = torch.ops.sw_gcn.linear_cross_entropy(xs, ws, t)
+        grads = torch.autograd.grad(loss, (xs, ws))
+    x2, w2, _ = make(300, 64, 500, "float32", seed=3)
+    want2 = run(x2, w2, t)
+    for a, b, want_ in ((x2, w2, want2), (x, w, want)):
+        with torch.no_grad():
+            xs.copy_(a)
+            ws.copy_(b)
+        graph.replay()
+        assert torch.equal(loss.detach(), want_[0]) and torch.equal(grads[0], want_[1]) and torch.equal(grads[1], want_[2])
+
+
+def test_refusals(built_lib):
+    import torch
+    from tile_fusion_b200 import sw_gcn  # noqa: F401
+    call = torch.ops.sw_gcn.linear_cross_entropy
+    x, w, t = make(8, 16, 5, "float32")
+    for args in ((x.cpu(), w, t), (x, w.cpu(), t), (x, w, t.cpu()), (x.double(), w.double(), t), (x, w.bfloat16(), t), (x[:, :8], w, t), (x, w, t[:4]),
+                 (x, w, t.float()), (x, w[0], t), (x, w[:0], t), (x, w, t, -100, "average")):
+        with pytest.raises(ValueError):
+            call(*args)
+    loss = call(x.requires_grad_(), w, t)
+    (g,) = torch.autograd.grad(loss, x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()

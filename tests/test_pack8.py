@@ -100,3 +100,75 @@ def test_weight_grad(built_lib, dtype, m, na, nb):
         assert off <= (U[dtype] + 5e-6) * want[inside].norm().item(), off / want[inside].norm().item()
         assert first is None or torch.equal(got, first)
         first = got
+
+
+def test_strides_and_foreign_codes(built_lib):
+    import torch
+    from tile_fusion_b200 import sw_gcn  # noqa: F401
+    ops = torch.ops.sw_gcn
+    x = data(40, 75, "float32")
+    codes, exps = ops.pack8(x)
+    wide = torch.zeros(40, 90, device="cuda")
+    wide[:, 7:82] = x
+    for other in (wide[:, 7:82], x.t().contiguous().t(), x.requires_grad_()):
+        c, e = ops.pack8(other)
+        assert torch.equal(c, codes) and torch.equal(e, exps) and not c.requires_grad
+    value = ops.unpack8(codes, exps)
+    g = data(40, 9, "float32", 1)
+    grad = ops.weight_grad8(g, codes, exps)
+    for c in (codes.contiguous(), codes.clone(), codes.t().contiguous().t()):  # rows of 75 bytes, and columns in turn
+        assert torch.equal(ops.unpack8(c, exps), value) and torch.equal(ops.weight_grad8(g, c, exps), grad)
+    some = ops.unpack8(codes[8:24], exps[8:24])
+    assert torch.equal(some, value[8:24])
+    assert torch.equal(ops.weight_grad8(g[8:24], codes[8:24], exps[8:24]), ops.weight_grad8(g[8:24].clone(), codes[8:24].clone(), exps[8:24].clone()))
+    gs = torch.zeros(40, 20, device="cuda")
+    gs[:, 4:13] = g
+    assert torch.equal(ops.weight_grad8(gs[:, 4:13], codes, exps), grad)
+    none = ops.weight_grad8(g[:0], codes[:0], exps[:0])
+    assert none.shape == (9, 75) and (none == 0).all()
+    c, e = ops.pack8(x[:0])
+    assert c.shape == (0, 75) and ops.unpack8(c, e).shape == (0, 75)
+
+
+# ranges of 16 rows off the CTAs' ranges, operands that need several tiles, and G in all the ways that rows are read
+@pytest.mark.parametrize("dtype", list(U))
+@pytest.mark.parametrize("m,na,nb", [(100_003, 40, 60), (20_011, 256, 128), (20_011, 128, 256), (9_999, 257, 260), (30_001, 33, 300)])
+def test_weight_grad_of_many_rows(built_lib, dtype, m, na, nb):
+    import torch
+    from tile_fusion_b200 import sw_gcn  # noqa: F401
+    gen = torch.Generator(device="cuda").manual_seed(m)
+    x = torch.randn(m, nb, generator=gen, device="cuda")
+    g = (torch.randn(m, na, generator=gen, device="cuda") / m ** 0.5).to(getattr(torch, dtype))
+    codes, exps = torch.ops.sw_gcn.pack8(x, False)
+    want = g.double().t() @ torch.ops.sw_gcn.unpack8(codes, exps).double()
+    got = torch.ops.sw_gcn.weight_grad8(g, codes, exps)
+    off = (got.double() - want).norm().item()
+    assert off <= (U[dtype] + 5e-6) * want.norm().item(), off / want.norm().item()
+
+
+def test_rows_that_are_not_finite_and_large_steps(built_lib):
+    import torch
+    from tile_fusion_b200 import sw_gcn  # noqa: F401
+    x, g = data(100, 64, "float32"), data(100, 20, "float32", 1)
+    x[3, 40] = float("inf")
+    codes, exps = torch.ops.sw_gcn.pack8(x)
+    dw = torch.ops.sw_gcn.weight_grad8(g, codes, exps)
+    assert dw[:, 32:].isnan().all() and dw[:, :32].isfinite().all()
+    x = data(64, 32, "float32").sign() * 2.0 ** 120
+    g = data(64, 20, "float32", 2) * 2.0 ** -100
+    codes, exps = torch.ops.sw_gcn.pack8(x)
+    want = g.double().t() @ x.double()
+    assert (torch.ops.sw_gcn.weight_grad8(g, codes, exps).double() - want).norm().item() <= 5e-6 * want.norm().item()
+
+
+def test_refusals(built_lib):
+    import torch
+    from tile_fusion_b200 import sw_gcn  # noqa: F401
+    ops = torch.ops.sw_gcn
+    x = data(8, 40, "float32")
+    codes, exps = ops.pack8(x)
+    for f, args in ((ops.pack8, (x.cpu(),)), (ops.pack8, (x.double(),)), (ops.pack8, (x[0],)), (ops.pack8, (x[:, :0],)), (ops.unpack8, (codes.int(), exps)),
+                    (ops.unpack8, (codes, exps[:, :1])), (ops.unpack8, (codes, exps, torch.float64)), (ops.unpack8, (codes.cpu(), exps.cpu())),
+                    (ops.weight_grad8, (x[:4], codes, exps)), (ops.weight_grad8, (x.double(), codes, exps)), (ops.weight_grad8, (x, codes, exps.int()))):
+        with pytest.raises(ValueError):
+            f(*args)

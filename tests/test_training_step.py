@@ -1,0 +1,111 @@
+"""The dense operators together, as a deep GCN trains with them: a layer that keeps its input in 8 bits, a norm that keeps its input in 8
+bits, the next layer behind its ReLU, and the loss; values and gradients against the same formulas in fp64, at the kept values.
+
+The adjacency is symmetric, as the layers assume.  Hidden values next to zero fall on one side of the ReLU or on the other by
+rounding; the reference takes the side from the fp32 values.  Tolerance: products of at most 64 terms by split TF32 (2e-6),
+norms and sums of fp32 terms (5e-6, see their tests), through two layers and their gradients: 1e-4 of the 2-norm.
+"""
+import math
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+def near(got, want, tol=1e-4):
+    off = (got.double() - want).norm().item()
+    assert off <= tol * want.norm().item(), off / want.norm().item()
+
+
+def graph(n, seed=0):
+    import numpy as np
+    import torch
+    from tile_fusion_b200 import synth
+    ap, ai, ax = synth.rmat_gcn(seed, n, 8)
+    a = torch.sparse_csr_tensor(torch.from_numpy(np.asarray(ap)), torch.from_numpy(np.asarray(ai)), torch.from_numpy(np.asarray(ax)), size=(len(ap) - 1,) * 2).cuda()
+    return a, a.to_dense().double()
+
+
+@pytest.mark.parametrize("relu", [False, True])
+def test_layer_that_keeps_8_bits(built_lib, relu):
+    import torch
+    from tile_fusion_b200 import sw_gcn  # noqa: F401
+    ops = torch.ops.sw_gcn
+    adj, dense = graph(1000)
+    n = dense.shape[0]
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(n, 40, generator=gen, device="cuda").requires_grad_()
+    w = (torch.randn(24, 40, generator=gen, device="cuda") / 6).requires_grad_()
+    g = torch.randn(n, 24, generator=gen, device="cuda")
+    sched = ops.inspect(adj, 64)
+    y = ops.fusedGeMMSpMM_ck8(adj, x, w, sched, 4, relu)
+    assert torch.equal(y, ops.fusedGeMMSpMM(adj, torch.relu(x) if relu else x, w, sched, 4))
+    dx, dw = torch.autograd.grad(y, (x, w), g)
+    kept = ops.unpack8(*ops.pack8(x.detach(), relu)).double()
+    ag = dense @ g.double()
+    near(dw, ag.t() @ kept)
+    near(dx, (ag @ w.double()) * (x > 0 if relu else 1))
+    # the plain layer's gradients, whose weight gradient the 8 bits are 1 % off at most: half a step is 2^-7 of a group's largest value
+    px, pw = x.detach().requires_grad_(), w.detach().requires_grad_()
+    want = torch.autograd.grad(ops.fusedGeMMSpMM(adj, torch.relu(px) if relu else px, pw, sched, 4), (px, pw), g)
+    assert torch.equal(dx, want[0])
+    near(dw, want[1].double(), 1e-2)
+    with torch.no_grad():
+        assert torch.equal(ops.fusedGeMMSpMM_ck8(adj, x, w, sched, 4, relu), y)
+    with pytest.raises(ValueError):
+        ops.fusedGeMMSpMM_ck8(adj, x[:, :8], w, sched, 4, relu)
+
+
+def test_training_step(built_lib):
+    import torch
+    from tile_fusion_b200 import sw_gcn  # noqa: F401
+    ops = torch.ops.sw_gcn
+    adj, dense = graph(1500, seed=2)
+    n, f, h, classes = dense.shape[0], 48, 64, 37
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    r = lambda *s: torch.randn(*s, generator=gen, device="cuda")  # noqa: E731
+    x = r(n, f)
+    w1, w2, head = (r(h, f) / math.sqrt(f)).requires_grad_(), (r(h, h) / math.sqrt(h)).requires_grad_(), (r(classes, h) / math.sqrt(h)).requires_grad_()
+    gain, shift = (1 + 0.1 * r(h)).requires_grad_(), (0.1 * r(h)).requires_grad_()
+    target = torch.randint(0, classes, (n,), generator=gen, device="cuda")
+    target[::3] = -100
+    params = (w1, gain, shift, w2, head)
+
+    def step():
+        a = ops.fusedGeMMSpMM_ck8(adj, x, w1, [], 4, False)
+        b = ops.layer_norm(a, gain, shift, 1e-5, True)
+        c = ops.fusedGeMMSpMM_ck8(adj, b, w2, [], 4, True)
+        loss = ops.linear_cross_entropy(c, head, target)
+        return loss, a, b, c, torch.autograd.grad(loss, params)
+
+    loss, a, b, c, grads = step()
+    kept = lambda t, relu: ops.unpack8(*ops.pack8(t.detach(), relu)).double()  # noqa: E731
+    d1, d2, dh, dg, ds = (p.detach().double() for p in (w1, w2, head, gain, shift))
+    ra = dense @ (x.double() @ d1.t())
+    mean, var = ra.mean(1, keepdim=True), ra.var(1, unbiased=False, keepdim=True)
+    rstd = (var + 1e-5).rsqrt()
+    rb = (ra - mean) * rstd * dg + ds
+    on = b.detach() > 0
+    rc = dense @ (torch.where(on, rb, 0) @ d2.t())
+    logp = torch.log_softmax(rc @ dh.t(), 1)
+    ok = target >= 0
+    rows = ok.nonzero()[:, 0]
+    near(a.detach(), ra, 2e-5)
+    near(b.detach(), rb, 5e-5)
+    near(c.detach(), rc, 5e-5)
+    want = -logp[rows, target[rows]].mean()
+    assert abs(loss.item() - want.item()) <= 1e-4
+    p = logp.exp()
+    p[rows, target[rows]] -= 1
+    p = p * (ok / len(rows))[:, None]
+    gc = p @ dh
+    ag = dense @ gc
+    gb = (ag @ d2) * on
+    xh = (kept(a, False) - mean) * rstd
+    hh = gb * dg
+    ga = rstd * (hh - hh.mean(1, keepdim=True) - xh * (hh * xh).mean(1, keepdim=True))
+    ag1 = dense @ ga
+    for got, ref in zip(grads, (ag1.t() @ kept(x, False), (gb * xh).sum(0), gb.sum(0), ag.t() @ kept(b, True), p.t() @ rc)):
+        near(got, ref)
+    again = step()
+    assert torch.equal(again[0], loss) and all(torch.equal(s, t) for s, t in zip(again[4], grads))

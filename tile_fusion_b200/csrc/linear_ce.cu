@@ -393,7 +393,7 @@ extern "C" int tf_linear_ce_fwd(const void *x, long long ld_x, const void *w, lo
   c.b = {sp.copy_w ? sp.w_hi : w, sp.w_lo, sp.copy_w ? sp.ldp : ld_w, false};
   c.m = rows; c.n = vocab; c.k = cols;
   c.f16 = dtype != TF_BF16;
-  c.chain = f32 ? 2 : 4;
+  c.chain = f32 ? 2 : 8;  // (16 bits, 4 096 x 2 048 x 50 021: loss off by 6e-8 with 4, 4e-7 with 16; 562 and 529 us)
   c.epilogue = kPlaneSoftmaxSums;
   if (f32) { c.scale_a = &sp.h->unscale_x; c.scale_b = &sp.h->unscale_w; }
   c.target = target;
@@ -443,7 +443,7 @@ extern "C" int tf_linear_ce_bwd(const void *x, long long ld_x, const void *w, lo
     c.b = {wp_hi, wp_lo, ld_w16, false};
     c.m = rows; c.n = nv; c.k = cols;
     c.f16 = dtype != TF_BF16;
-    c.chain = f32 ? 2 : 4;
+    c.chain = f32 ? 2 : 16;
     c.epilogue = kPlaneSoftmaxSlope;
     if (f32) { c.scale_a = &sp.h->unscale_x; c.scale_b = &sp.h->unscale_w; }
     c.target = target; c.col0 = v0;
