@@ -84,23 +84,40 @@ __device__ __forceinline__ unsigned ring_place(unsigned a) {
   asm volatile("" : "+r"(a) :: "memory");
   return a;
 }
-// 16 bytes of neighbouring values of a gradient, zeros where there are none: `n` of them exist.
-template <class T, class At> __device__ __forceinline__ void wg_load(At at, int n, bool whole, float (&v)[16 / sizeof(T)]) {
+// 16 bytes of neighbouring values of a gradient; WHOLE: all exist, and start on 16 bytes; else zeros from the n-th on.
+template <class T, bool WHOLE, class At> __device__ __forceinline__ void wg_load(At at, int n, float (&v)[16 / sizeof(T)]) {
   constexpr int W = 16 / sizeof(T);
   using U = typename std::conditional<sizeof(T) == 4, unsigned, unsigned short>::type;
-  Pack<U, W> a = {};
-  if (whole) {
-    if (n > 0) {
-      const uint4 q = wg_read<uint4>(at);
-      a = reinterpret_cast<const Pack<U, W> &>(q);
-    }
+  Pack<U, W> a;
+  if constexpr (WHOLE) {
+    const uint4 q = wg_read<uint4>(at);
+    a = reinterpret_cast<const Pack<U, W> &>(q);
   } else {
 #pragma unroll
-    for (int i = 0; i < W; ++i)
-      if (i < n) a.v[i] = wg_read<U>(at + i * (int)sizeof(T));
+    for (int i = 0; i < W; ++i) {  // (what does not exist is read again from the start: no branches)
+      const U u = wg_read<U>(at + (i < n ? i : 0) * (int)sizeof(T));
+      a.v[i] = i < n ? u : (U)0;
+    }
   }
 #pragma unroll
   for (int i = 0; i < W; ++i) v[i] = to_float(reinterpret_cast<const T &>(a.v[i]));
+}
+// They as bf16 operands, one plane after the other (each what the planes before leave).
+template <int PLANES, int W> __device__ __forceinline__ void wg_planes(float (&g)[W], unsigned to, int plane) {
+#pragma unroll
+  for (int p = 0; p < PLANES; ++p) {
+    unsigned u[W / 2];
+#pragma unroll
+    for (int k = 0; k < W / 2; ++k) {
+      u[k] = pack_pair(g[2 * k], g[2 * k + 1], false);
+      if (p < PLANES - 1) {
+        g[2 * k] -= __uint_as_float(u[k] << 16);
+        g[2 * k + 1] -= __uint_as_float(u[k] & 0xffff0000u);
+      }
+    }
+    if constexpr (W == 8) asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + p * plane), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]));
+    else asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(to + p * plane), "r"(u[0]), "r"(u[1]));
+  }
 }
 
 // RING: G and the codes have nothing between their rows and the tile holds all columns, so that 16 rows are one run of bytes each (a
@@ -229,41 +246,34 @@ __global__ void __launch_bounds__(wg_threads(RING), 1) weight_grad8_kernel(const
     const int at_g = chunk_g * W / 8;  // (half a chunk of 16 bytes where a value has four)
     const int to_g = at_g / 8 * kWgBlock + (W == 4 ? (chunk_g & 1) * 8 : 0), to_x = PLANES * kPlane + chunk_x / 8 * kWgBlock;
     const int n_g = min(W, P.na - a0 - chunk_g * W), from_x = b0 + chunk_x * 8, from_e = from_x / kPackGroup, ld_e = P.ld_codes / kPackGroup;
-    // `rows` rows of G, codes and exponents that start at the given places, `ld` bytes of G from one to the next, as operands at `base`
+    // Rows of G, codes and exponents that start at the given places, `ld` bytes of G from one to the next, as operands at `base`.  From
+    // memory only `rows` of them are there; the others are read as the first and count as zero.
     auto convert = [&](unsigned base, auto pg, auto ld, auto pc, auto pe, int rows) {
-      pg += first_g * ld + (a0 + chunk_g * W) * (int)sizeof(T);
+      pg += (a0 + chunk_g * W) * (int)sizeof(T);
+      auto gradient = [&](auto whole) {
 #pragma unroll 4
-      for (int r = first_g; r < kWgRows; r += step_g, pg += step_g * ld) {
-        float g[W];
-        wg_load<T>(pg, r < rows ? n_g : 0, P.whole_g, g);
-        const unsigned to = base + (unsigned)(to_g + r * 128 + ((at_g ^ r) & 7) * 16);
+        for (int r = first_g; r < kWgRows; r += step_g) {
+          float g[W];
+          const bool here = RING || r < rows;
+          wg_load<T, decltype(whole)::value>(pg + (here ? r : 0) * ld, n_g, g);
+          if (!here)
 #pragma unroll
-        for (int p = 0; p < PLANES; ++p) {
-          unsigned u[W / 2];
-#pragma unroll
-          for (int k = 0; k < W / 2; ++k) {
-            u[k] = pack_pair(g[2 * k], g[2 * k + 1], false);
-            if (p < PLANES - 1) {
-              g[2 * k] -= __uint_as_float(u[k] << 16);
-              g[2 * k + 1] -= __uint_as_float(u[k] & 0xffff0000u);
-            }
-          }
-          if constexpr (W == 8) asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + p * kPlane), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]));
-          else asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(to + p * kPlane), "r"(u[0]), "r"(u[1]));
+            for (int k = 0; k < W; ++k) g[k] = 0.f;
+          wg_planes<PLANES, W>(g, base + (unsigned)(to_g + r * 128 + ((at_g ^ r) & 7) * 16), kPlane);
         }
-      }
-      pc += first_x * P.ld_codes + from_x;
-      pe += first_x * ld_e + from_e;
+      };
+      if (P.whole_g) gradient(std::true_type());
+      else gradient(std::false_type());
+      pc += from_x;
+      pe += from_e;
 #pragma unroll 4
-      for (int r = first_x; r < kWgRows; r += step_x, pc += step_x * P.ld_codes, pe += step_x * ld_e) {
-        uint2 x = make_uint2(0, 0);
-        unsigned e = 127;
-        if (r < rows) {
-          x = wg_read<uint2>(pc);
-          e = wg_read<unsigned char>(pe);
-        }
+      for (int r = first_x; r < kWgRows; r += step_x) {
+        const bool here = RING || r < rows;
+        uint2 x = wg_read<uint2>(pc + (here ? r : 0) * P.ld_codes);
+        const unsigned e = wg_read<unsigned char>(pe + (here ? r : 0) * ld_e);
+        if (!here) x = make_uint2(0, 0);
         float v[8];
-        unpack8_values<8>(reinterpret_cast<const Pack<signed char, 8> &>(x), unpack8_step(e), v);
+        unpack8_values<8>(reinterpret_cast<const Pack<signed char, 8> &>(x), here ? unpack8_step(e) : 0.f, v);
         unsigned u[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) u[k] = pack_pair(v[2 * k], v[2 * k + 1], false);
@@ -288,19 +298,18 @@ __global__ void __launch_bounds__(wg_threads(RING), 1) weight_grad8_kernel(const
         char *at = raw + rs * P.ring_bytes;
         const bool all = sl < whole;
         if (all && !wait(&s.raw_full[rs], raw_ph)) break;
-        int rows = kWgRows;
-        if (!all) {  // the last rows: the team copies them itself (what was there it has read, once its warps have met)
-          rows = (int)(r1 - row);
+        if (!all) {  // the last rows: the team copies them itself, and zeros behind them (what was there it has read, once its warps have met)
+          const int rows = (int)(r1 - row), per = P.ld_codes / kPackGroup;
           asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(kWgTeam) : "memory");
           T *to = reinterpret_cast<T *>(at);
-          for (int i = in_team; i < rows * P.na; i += kWgTeam) to[i] = static_cast<const T *>(P.g)[row * P.na + i];
-          for (int i = in_team; i < rows * P.ld_codes; i += kWgTeam) at[P.g_bytes + i] = P.codes[row * P.ld_codes + i];
-          const int per = P.ld_codes / kPackGroup;
-          for (int i = in_team; i < rows * per; i += kWgTeam) at[P.g_bytes + kWgRows * P.ld_codes + i] = (char)P.exps[row * per + i];
+          for (int i = in_team; i < kWgRows * P.na; i += kWgTeam) to[i] = i < rows * P.na ? static_cast<const T *>(P.g)[row * P.na + i] : from_float<T>(0.f);
+          for (int i = in_team; i < kWgRows * P.ld_codes; i += kWgTeam) at[P.g_bytes + i] = i < rows * P.ld_codes ? P.codes[row * P.ld_codes + i] : 0;
+          for (int i = in_team; i < kWgRows * per; i += kWgTeam)
+            at[P.g_bytes + kWgRows * P.ld_codes + i] = (char)(i < rows * per ? P.exps[row * per + i] : 127);
           asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(kWgTeam) : "memory");
         }
         const unsigned place = ring_place(smem_u32(at));
-        convert(stage, place, (unsigned)(P.na * sizeof(T)), place + P.g_bytes, place + P.g_bytes + kWgRows * P.ld_codes, rows);
+        convert(stage, place, (unsigned)(P.na * sizeof(T)), place + P.g_bytes, place + P.g_bytes + kWgRows * P.ld_codes, kWgRows);
         arrive(&s.raw_empty[rs]);
         if ((rs += kWgTeams) >= P.ring) { rs = team; raw_ph ^= 1u; }
       } else
