@@ -9,9 +9,9 @@ ROOT = os.path.dirname(HERE)
 LIB = os.path.join(HERE, "libtilefusion_b200.so")
 SOURCES = ["kernels.cu", "api.cu", "inspector.cpp", "planner.cpp", "tiling.cpp", "noalloc.cu", "gemm_tc.cu", "tile_pipeline.cu", "lattice.cpp", "lattice_march.cu", "multi.cu", "io.cpp", "reorder.cpp",
            "gather.cu", "gather_plan.cpp", "row_gemm.cu", "sddmm_gather.cu", "line_march.cu", "line_plan.cpp", "band_march.cu", "band_plan.cpp", "atb.cu", "spmm_gemm.cu", "spmm_gemm_plan.cpp",
-           "plane_gemm.cu", "linear_ce.cu", "layer_norm.cu", "layer_norm_grad.cu", "pack8.cu", "weight_grad8.cu"]
+           "plane_gemm.cu", "linear_ce.cu", "ce_few.cu", "layer_norm.cu", "layer_norm_grad.cu", "pack8.cu", "weight_grad8.cu"]
 HEADERS = ["kernels.cuh", "launch.h", "tf_internal.h", "gemm_tc.cuh", "gemm_tc_host.h", "lattice_march.h", "host_stage.h", "gather.h", "row_gemm.h", "line_march.h", "band_march.h", "segments.h", "spmm_gemm.h", "pair_mma.cuh",
-           "values.cuh", "plane_gemm.h", "pack8.cuh", "layer_norm.cuh"]
+           "values.cuh", "plane_gemm.h", "ce_few.h", "pack8.cuh", "layer_norm.cuh"]
 
 
 def _stale() -> bool:

@@ -1,0 +1,31 @@
+// Softmax cross entropy of a linear layer over few classes (ce_few.cu): both passes in one launch each.
+#pragma once
+#include <cuda_runtime.h>
+
+namespace tfk {
+
+constexpr int kFewClasses = 64, kFewCols = 256;
+
+struct CeFewCall {
+  const void *x = nullptr, *w = nullptr;
+  long long ld_x = 0, ld_w = 0;
+  int dtype = 0, rows = 0, cols = 0, vocab = 0;
+  const long long *target = nullptr;
+  long long ignore = 0;
+  int *error = nullptr;
+  // forward
+  float *lse2 = nullptr, *row_loss = nullptr;    // row_loss or, for each CTA, the sum of its rows' losses and their number
+  double *cta_loss = nullptr;
+  int *cta_count = nullptr;
+  // backward
+  const float *row_scale = nullptr, *unscale = nullptr;
+  void *dx = nullptr;                            // null: not asked for
+  float *dw_parts = nullptr;                     // [CTA][vocab][cols], times 1 / *unscale; null: not asked for
+};
+
+bool ce_few_supported(int cols, int vocab);
+int ce_few_ctas(int rows);
+cudaError_t ce_few_forward(const CeFewCall &c, cudaStream_t s);
+cudaError_t ce_few_backward(const CeFewCall &c, cudaStream_t s);
+
+}  // namespace tfk

@@ -6,6 +6,8 @@
 //              planes (at most kCeSlopeBytes of them, however large the vocabulary), then dx += P W_piece and
 //              dW_piece = P^T x.  Four products of 2 n d V operations in all where kept logits would need three.
 //
+//   Up to 64 classes and 256 columns have kernels of their own (ce_few.cu), which read x once a pass.
+//
 // Types.  bf16 and fp16 operands are multiplied as they are.  The slope is rounded to their type before its products, one
 // rounding of relative size 2^-9 (bf16) or 2^-12 (fp16) of each summand; the sums are fp32.  fp32 operands are split into two fp16
 // planes behind a power of two that brings the largest finite value to [2^14, 2^15): 22 bits of every value within 2^-27 of the
@@ -18,6 +20,7 @@
 #include <algorithm>
 #include <string>
 
+#include "ce_few.h"
 #include "plane_gemm.h"
 #include "tf_internal.h"
 #include "values.cuh"
@@ -252,6 +255,22 @@ __global__ void __launch_bounds__(256) ce_parts_kernel(const float *__restrict__
   }
 }
 
+// out[i] = (part[0][i] + part[1][i] + ...) * *scale, in order; eight threads share an element's parts.
+__global__ void __launch_bounds__(256) ce_few_sum_kernel(const float *__restrict__ part, int parts, int n, const float *scale, void *__restrict__ out, int dtype) {
+  __shared__ float s[8][32];
+  const int lane = threadIdx.x & 31, l = threadIdx.x >> 5, i = blockIdx.x * 32 + lane;
+  float v = 0.f;
+  if (i < n)
+#pragma unroll 4
+    for (int k = l; k < parts; k += 8) v += __ldg(part + (size_t)k * n + i);
+  s[l][lane] = v;
+  __syncthreads();
+  if (l || i >= n) return;
+#pragma unroll
+  for (int k = 1; k < 8; ++k) v += s[k][lane];
+  store_value(out, dtype, i, v * *scale);
+}
+
 long long up(long long v, long long to) { return (v + to - 1) / to * to; }
 
 // What the workspace holds, for the sizes of a call; `base` null: sizes only.
@@ -262,7 +281,7 @@ struct CeSpace {
   float *row_scale = nullptr; unsigned short *slope_hi = nullptr, *slope_lo = nullptr; float *parts_x = nullptr, *parts_w = nullptr;
   int ldp, ld_slope = 0, piece = 0, cut_x = 0, cut_w = 0;  // cut_: slices of a cut of the sum, 0: not cut
   long long bytes;
-  bool copy_x, copy_w;
+  bool few, copy_x, copy_w;
 };
 
 // Slices of a cut of the long sum of a gradient product (0: not cut), so that few tiles still fill the pairs of the device.  A
@@ -290,6 +309,18 @@ CeSpace ce_space(char *base, int rows, int cols, int vocab, int dtype, bool back
   };
   const bool f32 = dtype == TF_F32;
   s.h = (CeHeader *)take(sizeof(CeHeader));
+  s.few = ce_few_supported(cols, vocab);
+  if (s.few) {
+    const int ctas = ce_few_ctas(rows);
+    s.block_loss = (double *)take(8ll * ctas);
+    s.block_count = (int *)take(4ll * ctas);
+    if (backward) {
+      s.row_scale = (float *)take(4ll * rows);
+      s.parts_w = (float *)take(4ll * ctas * vocab * cols);
+    }
+    s.bytes = at;
+    return s;
+  }
   s.ldp = (int)up(cols, 8);
   s.copy_x = f32 || backward || !whole_x;
   s.copy_w = f32 || !whole_w;
@@ -345,6 +376,15 @@ int sm_count() {
   return sms;
 }
 
+CeFewCall few_call(const CeSpace &sp, const void *x, long long ld_x, const void *w, long long ld_w, int dtype, const long long *target, int rows, int cols,
+                   int vocab, long long ignore) {
+  CeFewCall c;
+  c.x = x; c.w = w; c.ld_x = ld_x; c.ld_w = ld_w; c.dtype = dtype; c.rows = rows; c.cols = cols; c.vocab = vocab;
+  c.target = target; c.ignore = ignore;
+  c.error = &sp.h->error;
+  return c;
+}
+
 // Planes of both operands, where they are not multiplied as they lie.
 cudaError_t ce_planes(const CeSpace &sp, const void *x, long long ld_x, const void *w, long long ld_w, int dtype, int rows, int cols, int vocab,
                       const long long *target, long long ignore, cudaStream_t s) {
@@ -385,6 +425,18 @@ extern "C" int tf_linear_ce_fwd(const void *x, long long ld_x, const void *w, lo
   }
   const CeSpace sp = ce_space((char *)work, rows, cols, vocab, dtype, false, ce_whole(x, ld_x, dtype), ce_whole(w, ld_w, dtype));
   cudaError_t e = cudaMemsetAsync(sp.h, 0, sizeof(CeHeader), s);
+  if (sp.few) {
+    CeFewCall c = few_call(sp, x, ld_x, w, ld_w, dtype, target, rows, cols, vocab, ignore_index);
+    c.lse2 = lse2;
+    c.row_loss = reduction ? nullptr : loss;
+    if (reduction) { c.cta_loss = sp.block_loss; c.cta_count = sp.block_count; }
+    if (e == cudaSuccess) e = ce_few_forward(c, s);
+    if (e == cudaSuccess && reduction) {
+      ce_total_kernel<<<1, 1024, 0, s>>>(sp.block_loss, sp.block_count, ce_few_ctas(rows), reduction == 1, loss);
+      e = cudaGetLastError();
+    }
+    return e == cudaSuccess ? TF_OK : ce_fail(who, e);
+  }
   if (e == cudaSuccess) e = ce_planes(sp, x, ld_x, w, ld_w, dtype, rows, cols, vocab, target, ignore_index, s);
   if (e != cudaSuccess) return ce_fail(who, e);
   const bool f32 = dtype == TF_F32;
@@ -430,6 +482,18 @@ extern "C" int tf_linear_ce_bwd(const void *x, long long ld_x, const void *w, lo
     ce_count_kernel<<<std::min((rows + 255) / 256, 148 * 4), 256, 0, s>>>(target, reduction ? nullptr : grad, rows, ignore_index, sp.h);
   ce_scale_kernel<<<(rows + 255) / 256, 256, 0, s>>>(target, grad, rows, ignore_index, vocab, reduction, dtype == TF_BF16 ? 1.f : kSlopeUnit,
                                                      sp.row_scale, sp.h);
+  if (sp.few) {
+    CeFewCall c = few_call(sp, x, ld_x, w, ld_w, dtype, target, rows, cols, vocab, ignore_index);
+    c.lse2 = const_cast<float *>(lse2);
+    c.row_scale = sp.row_scale; c.unscale = &sp.h->unscale_slope;
+    c.dx = dx; c.dw_parts = dw ? sp.parts_w : nullptr;
+    e = ce_few_backward(c, s);
+    if (e == cudaSuccess && dw) {
+      ce_few_sum_kernel<<<(vocab * cols + 31) / 32, 256, 0, s>>>(sp.parts_w, ce_few_ctas(rows), vocab * cols, &sp.h->unscale_slope, dw, dtype);
+      e = cudaGetLastError();
+    }
+    return e == cudaSuccess ? TF_OK : ce_fail(who, e);
+  }
   e = ce_planes(sp, x, ld_x, w, ld_w, dtype, rows, cols, vocab, target, ignore_index, s);
   if (e != cudaSuccess) return ce_fail(who, e);
   const int sms = sm_count();
