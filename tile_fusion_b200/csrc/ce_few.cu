@@ -1,13 +1,13 @@
 // Softmax cross entropy of a linear layer over at most 64 classes and 256 columns: node classification, many rows and little work
 // to each.  Bound by x, which the forward pass reads once, and by x and dx, which the backward pass reads and writes once.
 //
-//   * A CTA walks tiles of 64 rows.  Seven warps bring the next tile from memory, all of it in flight at once, and leave it in shared
+//   * A CTA walks tiles of 64 rows.  Seven warps (forward thirteen) bring the next tile from memory, all of it in flight at once, and leave it in shared
 //     memory as 16-bit operands (two buffers); the weight is there from the start, in the same form.  fp32 values become two fp16
 //     planes behind a power of two, x = 2^-e (hi + lo), of which a tile has one of its own: products hi hi + hi lo + lo hi.
 //   * One warp issues the products of a tile (tcgen05.mma, M = 128 of which 64 rows count): logits L = X W^T, one tile ahead;
 //     then, 128 columns at a time through three accumulators, dX = P W and dW += P^T X.  X, W and P lie in shared memory once and
 //     are read along either index (K-major or MN-major, both with the 128-byte swizzle).
-//   * Four warps turn logits into losses, or into the slope P = (exp(l - lse) - (class == target)) * row_scale as operand planes,
+//   * Eight warps (forward two) turn logits into losses, or into the slope P = (exp(l - lse) - (class == target)) * row_scale as operand planes,
 //     write dX, and add up dW in registers: 24 additions in tensor memory, which cuts off, then one that rounds.
 //   * The CTAs' dW are added by a second launch, in order.
 // All waits are bounded: the one that runs out sets the error flag, and every role leaves.
@@ -23,16 +23,20 @@ namespace tfk {
 
 namespace {
 
-constexpr int kFewRows = 64, kFewThreads = 384;
+constexpr int kFewRows = 64, kFewThreads = 512;
 constexpr int kFewBlock = kFewRows * 128;  // bytes of 64 columns of a tile
-constexpr int kFewLoaders = 7, kFewMmaWarp = 11;
+// Warps of the backward pass: those that may read the accumulators' lanes of 64 rows (of four two), one that issues the products, and
+// seven for the tiles; forward two of the former are enough, and thirteen bring tiles.
+constexpr int kFewMmaWarp = 15;
+__host__ __device__ constexpr int few_drains(bool back) { return back ? 8 : 2; }
+__host__ __device__ constexpr int few_loaders(bool back) { return 15 - few_drains(back); }
 constexpr int kFewWaitLimit = 1 << 22;
 constexpr int kFewRegions = 3;             // accumulators of 128 columns behind two of 64 for the logits
 constexpr float kFewLog2e = 1.4426950408889634f, kFewLn2 = 0.69314718055994531f;
 
 struct FewShared {
-  unsigned long long x_full[2], x_empty[2], w_full, log_full[2], log_empty[2], p_full, job_full[kFewRegions], job_empty[kFewRegions];
-  unsigned top[2][kFewLoaders];
+  unsigned long long x_full[2], x_empty[2], w_full, log_full[2], log_empty[2], p_full[2], job_full[kFewRegions], job_empty[kFewRegions];
+  unsigned top[2][few_loaders(false)];
   float unscale_x[2], unscale_w;
   double loss[2];
   int count[2];
@@ -63,30 +67,43 @@ __device__ __forceinline__ void few_arrive(unsigned long long *bar) {
   if ((threadIdx.x & 31) == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
+// Whether a phase has completed, without waiting for it (a try_wait may be put to sleep).
+__device__ __forceinline__ bool few_done(unsigned long long *bar, unsigned parity) {
+  unsigned done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+  return __all_sync(kFull, done != 0);
+}
+
 // DT: tf_dtype of x, w and dx.  BLOCKS: blocks of 64 columns; known, so that the issuing warp's descriptors are one register and
 // constants.
 template <int DT, int BLOCKS, bool BACK>
 __global__ void __launch_bounds__(kFewThreads, 1) ce_few_kernel(const CeFewCall P) {
   constexpr int PLANES = DT == TF_F32 ? 2 : 1;
   constexpr bool F16 = DT != TF_BF16;
+  constexpr int kFewLoaders = few_loaders(BACK), kDrains = few_drains(BACK);
   extern __shared__ char dyn[];
   __shared__ FewShared s;
   char *smem = reinterpret_cast<char *>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~(uintptr_t)1023);
   const int tid = threadIdx.x, warp = __shfl_sync(kFull, tid >> 5, 0), lane = tid & 31;
   constexpr int plane = BLOCKS * kFewBlock, tile_bytes = PLANES * plane;
-  const unsigned at_x = smem_u32(smem), at_w = at_x + 2 * tile_bytes, at_p = at_w + tile_bytes;
+  // two slopes, two tiles of x, the weight: an operand of 128 rows of which 64 count reads into what lies behind it
+  constexpr int slope_bytes = PLANES * kFewBlock;
+  const unsigned at_p = smem_u32(smem), at_x = at_p + 2 * slope_bytes, at_w = at_x + 2 * tile_bytes;
   const int tiles_all = (P.rows + kFewRows - 1) / kFewRows;
   const int tiles = tiles_all > (int)blockIdx.x ? (tiles_all - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x : 0;
   constexpr int halves = (BLOCKS + 1) / 2;  // of 128 columns
 
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&s.x_full[i], kFewLoaders); mbar_init(&s.x_empty[i], BACK ? 1 : 5);
-      mbar_init(&s.log_full[i], 1); mbar_init(&s.log_empty[i], 4);
+      mbar_init(&s.x_full[i], kFewLoaders); mbar_init(&s.x_empty[i], BACK ? 1 : 1 + kDrains);
+      mbar_init(&s.log_full[i], 1); mbar_init(&s.log_empty[i], kDrains);
+      mbar_init(&s.p_full[i], kDrains);
     }
     mbar_init(&s.w_full, kFewLoaders);
-    mbar_init(&s.p_full, 4);
-    for (int i = 0; i < kFewRegions; ++i) { mbar_init(&s.job_full[i], 1); mbar_init(&s.job_empty[i], 4); }
+    for (int i = 0; i < kFewRegions; ++i) { mbar_init(&s.job_full[i], 1); mbar_init(&s.job_empty[i], kDrains); }
     s.dead = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -103,7 +120,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) ce_few_kernel(const CeFewCall 
   if (warp == kFewMmaWarp) {
     // ---- products ----
     const unsigned tmem = s.tmem_base;
-    int job = 0;
+    int job = 0;  // accumulators of 128 columns handed out so far
     // D = sum of BL products of planes, the small ones (lo hi, hi lo) before all hi hi; of four steps of 16 terms each
     auto product = [&](auto bl, unsigned d, unsigned a, unsigned b, auto plane_a, auto plane_b, auto step_a, auto step_b, unsigned idesc) {
       const unsigned long long da = few_desc(a), db = few_desc(b);
@@ -125,8 +142,6 @@ __global__ void __launch_bounds__(kFewThreads, 1) ce_few_kernel(const CeFewCall 
     static_assert(kFewRows / 16 == 4 && kFewClasses / 16 == 4, "steps of a product");
     auto logits = [&](int t) {
       const int b = t & 1;
-      if (!wait(&s.x_full[b], (unsigned)(t / 2) & 1u)) return;
-      if (t >= 2 && !wait(&s.log_empty[b], (unsigned)(t / 2 - 1) & 1u)) return;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       if (elect_one()) {  // (a block of 64 columns is a K-major tile of its own)
         product(std::integral_constant<int, BLOCKS>(), tmem + b * 64, at_x + b * tile_bytes, at_w, Plane(), Plane(), Along(), Along(), few_idesc(F16, 0, 0, 64));
@@ -135,60 +150,76 @@ __global__ void __launch_bounds__(kFewThreads, 1) ce_few_kernel(const CeFewCall 
       }
       __syncwarp();
     };
-    if (tiles > 0 && wait(&s.w_full, 0)) logits(0);
-    for (int t = 0; t < tiles && ok; ++t) {
-      if (t + 1 < tiles) logits(t + 1);
-      if (!BACK || !ok) continue;
-      if (!wait(&s.p_full, (unsigned)t & 1u)) break;
+    // One of the products of a tile's gradients: 128 columns of dW, which the tile's place is free after, or of dX.
+    const int jobs_w = P.dw_parts ? halves : 0, jobs = jobs_w + (P.dx ? halves : 0);
+    auto gradient = [&](int t, int j) {
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const unsigned x = at_x + (t & 1) * tile_bytes;
-      for (int j = 0; j < 2 * halves && ok; ++j) {
-        const bool to_w = j >= halves;
-        if (to_w ? !P.dw_parts : !P.dx) continue;
-        const int h = to_w ? j - halves : j, n = min(128, BLOCKS * 64 - h * 128), r = job % kFewRegions;
-        if (job >= kFewRegions && !wait(&s.job_empty[r], (unsigned)(job / kFewRegions - 1) & 1u)) break;
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        if (elect_one()) {
-          const unsigned d = tmem + 128 + r * 128;
-          if (to_w) product(One(), d, at_p, x + h * 2 * kFewBlock, Slope(), Plane(), Across(), Across(), few_idesc(F16, 1, 1, n));
-          else product(One(), d, at_p, at_w + h * 2 * kFewBlock, Slope(), Plane(), Along(), Across(), few_idesc(F16, 0, 1, n));
-          umma_commit(&s.job_full[r]);
-        }
-        __syncwarp();
-        ++job;
+      const unsigned x = at_x + (t & 1) * tile_bytes, slope = at_p + (t & 1) * slope_bytes;
+      const bool to_w = j < jobs_w;
+      const int h = to_w ? j : j - jobs_w, n = min(128, BLOCKS * 64 - h * 128), r = job % kFewRegions;
+      if (elect_one()) {
+        const unsigned d = tmem + 128 + r * 128;
+        if (to_w) product(One(), d, slope, x + h * 2 * kFewBlock, Slope(), Plane(), Across(), Across(), few_idesc(F16, 1, 1, n));
+        else product(One(), d, slope, at_w + h * 2 * kFewBlock, Slope(), Plane(), Along(), Across(), few_idesc(F16, 0, 1, n));
+        umma_commit(&s.job_full[r]);
+        if (j == max(jobs_w, 1) - 1) umma_commit(&s.x_empty[t & 1]);
       }
-      if (elect_one()) umma_commit(&s.x_empty[t & 1]);
       __syncwarp();
+    };
+    // Whatever can run: logits of the next tile whose rows and accumulator are ready, else a product of the gradients of the next whose
+    // slope is, into the next accumulator that has been read.  Nothing is waited for: the warps that read accumulators wait for the
+    // logits of the next tile before they read this one's gradients.
+    if (tiles > 0) wait(&s.w_full, 0);
+    int next = 0, done = BACK ? 0 : tiles, step = 0;
+    for (long long idle = 0; ok && (next < tiles || done < tiles);) {
+      if (next < tiles && few_done(&s.x_full[next & 1], (unsigned)(next / 2) & 1u) &&
+          (next < 2 || few_done(&s.log_empty[next & 1], (unsigned)(next / 2 - 1) & 1u))) {
+        logits(next++);
+        idle = 0;
+      } else if (BACK && done < next && (step > 0 || few_done(&s.p_full[done & 1], (unsigned)(done / 2) & 1u)) &&
+                 (job < kFewRegions || few_done(&s.job_empty[job % kFewRegions], (unsigned)(job / kFewRegions - 1) & 1u))) {
+        gradient(done, step);
+        ++job;
+        if (++step == jobs) { step = 0; ++done; }
+        idle = 0;
+      } else {
+        __nanosleep(20);  // (the loop would take the issue slots of the warps that bring tiles)
+        if (++idle <= 64ll * kFewWaitLimit && !*reinterpret_cast<volatile int *>(&s.dead)) continue;
+        s.dead = 1;
+        ok = false;
+      }
     }
     // the last arrivals on barriers that nobody waits for must be in before the CTA ends
     if (ok)
       for (int t = max(0, tiles - 2); t < tiles; ++t) wait(&s.x_empty[t & 1], (unsigned)(t / 2) & 1u);
-  } else if (warp < 8 && (warp & 3) < 2) {
-    // ---- rows 32 (warp & 3) .. + 31 of a tile, and half of the columns ----
+  } else if (BACK ? (warp & 3) < 2 : warp < 2) {
+    // ---- rows 32 (warp & 3) .. + 31 of a tile, and (backward) a quarter of the columns ----
     const int quadrant = warp & 3, side = warp >> 2, in_tile = quadrant * 32 + lane;
     const unsigned lanes = s.tmem_base + ((unsigned)(quadrant * 32) << 16);
-    float dw[BACK ? 128 : 1];
+    float dw[BACK ? 64 : 1];
     if (BACK)
 #pragma unroll
-      for (int i = 0; i < 128; ++i) dw[BACK ? i : 0] = 0.f;
+      for (int i = 0; i < 64; ++i) dw[BACK ? i : 0] = 0.f;
     double loss = 0.;
     int count = 0, job = 0;
     float unscale_w = 1.f, unscale_p = 1.f;
     if (tiles > 0 && wait(&s.w_full, 0)) unscale_w = s.unscale_w;
     if (BACK) unscale_p = __ldg(P.unscale);
-    for (int t = 0; t < tiles && ok; ++t) {
+    float scale_of[2];
+    // logits of a tile into losses, or into its slope
+    auto softmax = [&](int t) {
       const int b = t & 1;
       const long long row = ((long long)blockIdx.x + (long long)t * gridDim.x) * kFewRows + in_tile;
       const bool in = row < P.rows;
       const long long target = in ? __ldg(P.target + row) : -1;
       float lse2 = 0.f, by = 0.f;
       if (BACK && in) { lse2 = __ldg(P.lse2 + row); by = __ldg(P.row_scale + row); }
-      if (!wait(&s.x_full[b], (unsigned)(t / 2) & 1u) || !wait(&s.log_full[b], (unsigned)(t / 2) & 1u)) break;
-      const float unscale_x = s.unscale_x[b];  // (backward: before P, after which the tile may be replaced)
+      if (!wait(&s.x_full[b], (unsigned)(t / 2) & 1u) || !wait(&s.log_full[b], (unsigned)(t / 2) & 1u)) return;
+      const float unscale_x = scale_of[b] = s.unscale_x[b];  // (backward: before P, after which the tile may be replaced)
       if (!BACK) few_arrive(&s.x_empty[b]);
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       if (!BACK) {
-        if (side == 0) {  // all classes of a row are one thread's
+        {  // all classes of a row are one thread's
           float top = -INFINITY, own = 0.f, sum = 0.f, l[64];
 #pragma unroll
           for (int c = 0; c < 64; c += 16) {
@@ -218,90 +249,97 @@ __global__ void __launch_bounds__(kFewThreads, 1) ce_few_kernel(const CeFewCall 
         }
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         few_arrive(&s.log_empty[b]);
-        continue;
+        return;
       }
       {
-        float v[32];
-        tmem_load32(v, lanes + b * 64 + side * 32);
-        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-        tmem_loaded(v);
+        float v[16];
+        tmem_load16(v, lanes + b * 64 + side * 16);
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         few_arrive(&s.log_empty[b]);
-        const float in2 = unscale_x * kFewLog2e;
-        const unsigned to = at_p + in_tile * 128;
+        const float in2 = unscale_x * unscale_w * kFewLog2e;  // (powers of two: their product may leave the range only where all logits do)
+        const int mine = in && target >= side * 16 && target < side * 16 + 16 ? (int)target - side * 16 : -1;
+        const unsigned to = at_p + b * slope_bytes + in_tile * 128;
 #pragma unroll
-        for (int c = 0; c < 32; c += 8) {
+        for (int c = 0; c < 16; ++c) {
+          const float e = few_ex2(fmaf(v[c], in2, -lse2)) - (c == mine ? 1.f : 0.f);
+          v[c] = by == 0.f || side * 16 + c >= P.vocab ? 0.f : e * by;  // (a row that does not count stays zero whatever it holds)
+        }
+#pragma unroll
+        for (int c = 0; c < 16; c += 8) {
           unsigned hi[4], lo[4];
 #pragma unroll
-          for (int q = 0; q < 8; q += 2) {
-            float p[2];
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const int cls = side * 32 + c + q + k;
-              const float e = few_ex2(fmaf(v[c + q + k] * unscale_w, in2, -lse2)) - (cls == target ? 1.f : 0.f);
-              p[k] = by == 0.f || cls >= P.vocab ? 0.f : e * by;  // (a row that does not count stays zero whatever it holds)
-            }
-            hi[q / 2] = pack_pair(p[0], p[1], F16);
+          for (int q = 0; q < 4; ++q) {
+            hi[q] = pack_pair(v[c + 2 * q], v[c + 2 * q + 1], F16);
             if (PLANES == 2) {
-              const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi[q / 2]));
-              lo[q / 2] = pack_pair(p[0] - f.x, p[1] - f.y, true);
+              const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi[q]));
+              lo[q] = pack_pair(v[c + 2 * q] - f.x, v[c + 2 * q + 1] - f.y, true);
             }
           }
-          const unsigned a = to + (unsigned)(((side * 4 + c / 8) ^ (in_tile & 7)) * 16);
+          const unsigned a = to + (unsigned)(((side * 2 + c / 8) ^ (in_tile & 7)) * 16);
           asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(hi[0]), "r"(hi[1]), "r"(hi[2]), "r"(hi[3]) : "memory");
           if (PLANES == 2)
             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a + kFewBlock), "r"(lo[0]), "r"(lo[1]), "r"(lo[2]), "r"(lo[3]) : "memory");
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        few_arrive(&s.p_full);
+        few_arrive(&s.p_full[b]);
       }
+    };
+    // a tile's gradients out of tensor memory
+    auto drain = [&](int t) {
+      const long long row = ((long long)blockIdx.x + (long long)t * gridDim.x) * kFewRows + in_tile;
+      const bool in = row < P.rows;
+      const float unscale_x = t & 1 ? scale_of[1] : scale_of[0];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const bool to_w = j >= 2;
+        const bool to_w = j < 2;
         const int h = j & 1;
         if (h >= halves || (to_w ? !P.dw_parts : !P.dx)) continue;
         const int r = job % kFewRegions;
-        if (!wait(&s.job_full[r], (unsigned)(job / kFewRegions) & 1u)) break;
+        if (!wait(&s.job_full[r], (unsigned)(job / kFewRegions) & 1u)) return;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const unsigned from = lanes + 128 + r * 128 + side * 64;
-        const int col = h * 128 + side * 64;
-        if (col < BLOCKS * 64) {
+        const int col = h * 128 + side * 32;
+        float v[32];
+        tmem_load32(v, lanes + 128 + r * 128 + side * 32);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        tmem_loaded(v);
+        if (to_w) {
+          if (col < BLOCKS * 64) {
 #pragma unroll
-          for (int c = 0; c < 64; c += 16) {
-            float v[16];
-            tmem_load16(v, from + c);
-            if (to_w) {
+            for (int c = 0; c < 32; ++c) dw[BACK ? h * 32 + c : 0] = fmaf(v[c], unscale_x, dw[BACK ? h * 32 + c : 0]);
+          }
+        } else if (in) {
 #pragma unroll
-              for (int q = 0; q < 16; ++q) dw[BACK ? h * 64 + c + q : 0] = fmaf(v[q], unscale_x, dw[BACK ? h * 64 + c + q : 0]);
-            } else if (in) {
+          for (int c = 0; c < 32; ++c) v[c] = v[c] * unscale_p * unscale_w;
+          const long long at = row * P.cols + col;
+          if (P.cols % 8 == 0) {  // whole sectors at a time
 #pragma unroll
-              for (int q = 0; q < 16; ++q) v[q] = v[q] * unscale_p * unscale_w;
-              const long long at = row * P.cols + col + c;
+            for (int c = 0; c < 32; c += 8) {
+              if (col + c >= P.cols) break;
+              if constexpr (DT == TF_F32) {
+                Pack<float, 8> a;
 #pragma unroll
-              for (int q = 0; q < 16; q += 8) {
-                if (P.cols % 8 == 0) {  // whole sectors at a time
-                  if (col + c + q >= P.cols) break;
-                  if constexpr (DT == TF_F32) {
-                    Pack<float, 8> a;
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) a.v[k] = v[q + k];
-                    store_raw<float, 8>(static_cast<float *>(P.dx) + at + q, a);
-                  } else
-                    *reinterpret_cast<uint4 *>(static_cast<unsigned short *>(P.dx) + at + q) =
-                        make_uint4(pack_pair(v[q], v[q + 1], F16), pack_pair(v[q + 2], v[q + 3], F16), pack_pair(v[q + 4], v[q + 5], F16), pack_pair(v[q + 6], v[q + 7], F16));
-                } else {
-#pragma unroll
-                  for (int k = 0; k < 8; ++k)
-                    if (col + c + q + k < P.cols) store_value(P.dx, DT, at + q + k, v[q + k]);
-                }
-              }
+                for (int k = 0; k < 8; ++k) a.v[k] = v[c + k];
+                store_raw<float, 8>(static_cast<float *>(P.dx) + at + c, a);
+              } else
+                *reinterpret_cast<uint4 *>(static_cast<unsigned short *>(P.dx) + at + c) =
+                    make_uint4(pack_pair(v[c], v[c + 1], F16), pack_pair(v[c + 2], v[c + 3], F16), pack_pair(v[c + 4], v[c + 5], F16), pack_pair(v[c + 6], v[c + 7], F16));
             }
+          } else {
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+              if (col + c < P.cols) store_value(P.dx, DT, at + c, v[c]);
           }
         }
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         few_arrive(&s.job_empty[r]);
         ++job;
       }
+    };
+    // The slope of the next tile first, so that its products follow this one's.
+    if (tiles > 0) softmax(0);
+    for (int t = 0; t < tiles && ok; ++t) {
+      if (t + 1 < tiles) softmax(t + 1);
+      if (BACK && ok) drain(t);
     }
     const bool lost = !ok || *reinterpret_cast<volatile int *>(&s.dead);
     if (BACK && P.dw_parts && in_tile < P.vocab) {
@@ -309,12 +347,12 @@ __global__ void __launch_bounds__(kFewThreads, 1) ce_few_kernel(const CeFewCall 
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int c = 0; c < 64; ++c) {
-          const int col = h * 128 + side * 64 + c;
-          if (col < P.cols) to[col] = lost ? __int_as_float(0x7fc00000) : dw[BACK ? h * 64 + c : 0];
+        for (int c = 0; c < 32; ++c) {
+          const int col = h * 128 + side * 32 + c;
+          if (col < P.cols) to[col] = lost ? __int_as_float(0x7fc00000) : dw[BACK ? h * 32 + c : 0];
         }
     }
-    if (!BACK && side == 0) {
+    if (!BACK) {
       if (lost) loss = __longlong_as_double(0x7ff8000000000000ll);
       for (int k = 16; k; k >>= 1) {
         loss += __shfl_xor_sync(kFull, loss, k);
@@ -323,12 +361,12 @@ __global__ void __launch_bounds__(kFewThreads, 1) ce_few_kernel(const CeFewCall 
       if (lane == 0) { s.loss[quadrant] = loss; s.count[quadrant] = count; }
     }
   } else if (warp < kFewMmaWarp) {
-    // ---- tiles of 64 rows into operands: warps 2, 3, 6, 7, 8, 9, 10 ----
-    const int loader = warp < 4 ? warp - 2 : warp < 8 ? warp - 4 : warp - 4;
+    // ---- tiles of 64 rows into operands ----
+    const int loader = BACK ? (warp >> 2) * 2 + (warp & 3) - 2 : warp - 2;
     constexpr int kMine = (kFewRows + kFewLoaders - 1) / kFewLoaders;  // rows of a warp: eight columns a lane
     const int col = lane * 8;
-    unsigned raw[kMine][PLANES * 4];  // as they lie in memory
-    auto fetch = [&](const void *src, long long ld, long long row0, long long rows, const long long *target) {
+    using Raw = unsigned[kMine][PLANES * 4];  // rows as they lie in memory
+    auto fetch = [&](Raw &raw, const void *src, long long ld, long long row0, long long rows, const long long *target) {
       constexpr int BYTES = DT == TF_F32 ? 4 : 2;
       const bool whole = P.cols % 8 == 0 && ld * BYTES % 16 == 0 && (reinterpret_cast<uintptr_t>(src) & 15) == 0;
       // which of this warp's rows exist and count: lane i asks for the i-th
@@ -362,14 +400,14 @@ __global__ void __launch_bounds__(kFewThreads, 1) ce_few_kernel(const CeFewCall 
       }
     };
     int turn = 0;
-    auto put = [&](unsigned to, float *unscale) {
+    auto put = [&](const Raw &raw, unsigned to, float *unscale) {
       float by = 1.f;
       if (DT == TF_F32) {  // the power of two that brings the tile's largest finite value to [2^14, 2^15)
         float m = 0.f;
 #pragma unroll
         for (int i = 0; i < kMine; ++i)
 #pragma unroll
-          for (int k = 0; k < PLANES * 4; ++k) m = fmaxf(m, fabsf(__uint_as_float(raw[i][k])));  // (a NaN does not count)
+          for (int k = 0; k < PLANES * 4; k += 2) m = max3_abs_numbers(m, __uint_as_float(raw[i][k]), __uint_as_float(raw[i][k + 1]));
         if (m == INFINITY) {
           m = 0.f;
 #pragma unroll
@@ -414,17 +452,36 @@ __global__ void __launch_bounds__(kFewThreads, 1) ce_few_kernel(const CeFewCall 
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // read next by the tensor core
     };
-    if (tiles > 0) {
-      fetch(P.w, P.ld_w, 0, P.vocab, nullptr);
-      put(at_w, &s.unscale_w);
-      few_arrive(&s.w_full);
-    }
-    for (int t = 0; t < tiles; ++t) {
-      fetch(P.x, P.ld_x, ((long long)blockIdx.x + (long long)t * gridDim.x) * kFewRows, P.rows, P.target);
+    auto fetch_tile = [&](Raw &raw, int t) {
+      fetch(raw, P.x, P.ld_x, ((long long)blockIdx.x + (long long)t * gridDim.x) * kFewRows, P.rows, P.target);
+    };
+    auto put_tile = [&](const Raw &raw, int t) {
       // (where a wait has run out the waits end at once; no warp leaves, for the others would stay at the barrier in put())
       if (t >= 2) wait(&s.x_empty[t & 1], (unsigned)(t / 2 - 1) & 1u);
-      put(at_x + (t & 1) * tile_bytes, &s.unscale_x[t & 1]);
+      put(raw, at_x + (t & 1) * tile_bytes, &s.unscale_x[t & 1]);
       few_arrive(&s.x_full[t & 1]);
+    };
+    Raw raw;
+    if (tiles > 0) {
+      fetch(raw, P.w, P.ld_w, 0, P.vocab, nullptr);
+      put(raw, at_w, &s.unscale_w);
+      few_arrive(&s.w_full);
+      fetch_tile(raw, 0);
+    }
+    if constexpr (BACK) {
+      for (int t = 0; t < tiles; ++t) {
+        put_tile(raw, t);
+        if (t + 1 < tiles) fetch_tile(raw, t + 1);
+      }
+    } else {  // (five rows of a warp leave registers for the next tile's)
+      Raw more;
+      for (int t = 0; t < tiles; t += 2) {
+        if (t + 1 < tiles) fetch_tile(more, t + 1);
+        put_tile(raw, t);
+        if (t + 1 >= tiles) break;
+        if (t + 2 < tiles) fetch_tile(raw, t + 2);
+        put_tile(more, t + 1);
+      }
     }
   }
   __syncwarp();
@@ -445,8 +502,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) ce_few_kernel(const CeFewCall 
 
 template <int DT, int BLOCKS, bool BACK> cudaError_t few_launch(const CeFewCall &c, cudaStream_t s) {
   auto f = ce_few_kernel<DT, BLOCKS, BACK>;
-  // two tiles of x, the weight, the slope, and what an operand of 128 rows reads behind its 64
-  constexpr int smem = (DT == TF_F32 ? 2 : 1) * (3 * BLOCKS + 1) * kFewBlock + kFewBlock + 1024;
+  constexpr int smem = (DT == TF_F32 ? 2 : 1) * (3 * BLOCKS + 2) * kFewBlock + 1024;
   const cudaError_t e = cudaFuncSetAttribute((const void *)f, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
   f<<<ce_few_ctas(c.rows), kFewThreads, smem, s>>>(c);
