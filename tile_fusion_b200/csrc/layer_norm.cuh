@@ -156,10 +156,23 @@ inline LnShape ln_shape(int al, int cols, int bytes) {
   while ((vecs + nv - 1) / nv > (nv == 1 ? 256 : kLnRowThreads)) nv *= 2;
   return {al, nv, 0, ((vecs + nv - 1) / nv + 31) / 32 * 32};
 }
+// What the runtime says of a kernel's resident CTAs, asked once (it takes 2 us to say so).
+inline cudaError_t ln_occupancy(const void *f, int threads, size_t smem, int &each) {
+  struct Entry { const void *f; int threads; size_t smem; int each; };
+  thread_local Entry last[16] = {};
+  Entry &e = last[(reinterpret_cast<uintptr_t>(f) >> 4 ^ (uintptr_t)threads) & 15];
+  if (e.f != f || e.threads != threads || e.smem != smem) {
+    const cudaError_t rc = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&each, f, threads, smem);
+    if (rc != cudaSuccess) return rc;
+    e = {f, threads, smem, each};
+  }
+  each = e.each;
+  return cudaSuccess;
+}
 // CTAs of a launch: as many as fit the device at one time, or as have rows.
 template <class F> cudaError_t ln_ctas(F f, int threads, size_t smem, int rows, int rows_cta, int &ctas) {
   int each = 1;
-  const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&each, (const void *)f, threads, smem);
+  const cudaError_t e = ln_occupancy((const void *)f, threads, smem, each);
   ctas = std::max(1, std::min((rows + rows_cta - 1) / rows_cta, std::min(kLnMaxCtas, 148 * std::max(1, each))));
   return e;
 }

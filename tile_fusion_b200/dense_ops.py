@@ -78,9 +78,9 @@ def _ld(t):
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _records(*tensors):
-    """Whether autograd has to hear of a call with these inputs."""
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+def _fine(t, d):
+    """Whether t holds values that the library takes, on device d."""
+    return t.is_cuda and t.dtype in _DTYPES and t.get_device() == d
 
 
 def _same_device(name, *tensors):
@@ -138,7 +138,8 @@ def _packed(name, codes, exponents):
     ld = -(-d // 32) * 32
     if d == 0 or exponents.shape != (n, ld // 32):
         raise ValueError(f"sw_gcn.{name}: codes {tuple(codes.shape)} need exponents [{n}, {ld // 32}], not {list(exponents.shape)}")
-    _same_device(name, codes, exponents)
+    if exponents.get_device() != codes.get_device():
+        _same_device(name, codes, exponents)
     at = codes.storage_offset()
     if codes.stride(1) != 1 or (n > 1 and codes.stride(0) != ld) or codes.data_ptr() % 32 or codes.untyped_storage().nbytes() - at < n * ld:
         codes = torch.nn.functional.pad(codes, (0, ld - d)).contiguous()
@@ -146,7 +147,8 @@ def _packed(name, codes, exponents):
 
 
 def pack8(x, relu=False):
-    _check_values("pack8", "x", x)
+    if not _fine(x, x.get_device()):
+        _check_values("pack8", "x", x)
     if x.dim() != 2 or x.shape[1] == 0:
         raise ValueError(f"sw_gcn.pack8: x must be a matrix of at least one column, not {tuple(x.shape)}")
     codes, exponents = _pack(_rows(x), relu)
@@ -209,24 +211,26 @@ def _layer_norm_backward(g, x, codes, exponents, w, s, dtype, w_dtype, want, str
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, checkpoint):
-        need = ctx.needs_input_grad
+        need, shape = ctx.needs_input_grad, x.shape
         xr = _rows(x)
-        w, b = (t.contiguous() if t is not None else None for t in (weight, bias))
+        w = weight.contiguous() if weight is not None else None
+        b = bias.contiguous() if bias is not None else None
         y, s, codes, exponents = _layer_norm_forward(xr, w, b, eps, True, checkpoint and (need[0] or need[1]))
         ctx.save_for_backward(xr if codes is None else None, codes, exponents, w, s)
-        ctx.args = (x.shape, x.dtype, next(t for t in (w, b, x) if t is not None).dtype)
-        return y.view(x.shape)
+        ctx.args = (shape, x.dtype, (w if w is not None else b if b is not None else x).dtype)
+        return y if len(shape) == 2 else y.view(shape)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
         x, codes, exponents, w, s = ctx.saved_tensors
         shape, dtype, w_dtype = ctx.args
-        dx, dw, db = _layer_norm_backward(_rows(grad), x, codes, exponents, w, s, dtype, w_dtype, ctx.needs_input_grad[:3])
-        return dx.view(shape) if dx is not None else None, dw, db, None, None
+        dx, dw, db = _layer_norm_backward(_rows(grad), x, codes, exponents, w, s, dtype, w_dtype, ctx.needs_input_grad)
+        return dx if dx is None or len(shape) == 2 else dx.view(shape), dw, db, None, None
 
 
-def layer_norm(x, weight=None, bias=None, eps=1e-5, checkpoint=False):
+def _refuse_layer_norm(x, weight, bias):
+    """Says what is wrong with the arguments of layer_norm, if anything is."""
     name = "layer_norm"
     _check_values(name, "x", x)
     if x.dim() < 1 or x.shape[-1] == 0:
@@ -239,10 +243,21 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, checkpoint=False):
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise ValueError(f"sw_gcn.{name}: weight is {weight.dtype}, bias {bias.dtype}")
     _same_device(name, x, weight, bias)
-    if _records(x, weight, bias):
-        return _LayerNorm.apply(x, weight, bias, float(eps), bool(checkpoint))
-    w, b = (t.contiguous() if t is not None else None for t in (weight, bias))
-    return _layer_norm_forward(_rows(x), w, b, float(eps), False, False)[0].view(x.shape)
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, checkpoint=False):
+    shape = x.shape
+    d, last = x.get_device(), shape[-1:]
+    # (one expression where all is well: the checks one by one cost a small call a tenth of its time)
+    if not (_fine(x, d) and last and last[0] > 0 and (weight is None or (_fine(weight, d) and weight.shape == last))
+            and (bias is None or (_fine(bias, d) and bias.shape == last and (weight is None or weight.dtype == bias.dtype)))):
+        _refuse_layer_norm(x, weight, bias)
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
+        return _LayerNorm.apply(x, weight, bias, eps, checkpoint)
+    w = weight.contiguous() if weight is not None else None
+    b = bias.contiguous() if bias is not None else None
+    y = _layer_norm_forward(_rows(x), w, b, eps, False, False)[0]
+    return y if len(shape) == 2 else y.view(shape)
 
 
 @_on_device_of_first
@@ -269,26 +284,31 @@ def _loss_backward(xr, w, t, lse, grad, ignore_index, reduction, want, stream):
     return dx, dw
 
 
+def _classes(target):
+    return target if target.dim() == 1 and target.dtype == torch.int64 and target.is_contiguous() else target.reshape(-1).to(torch.int64).contiguous()
+
+
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, target, ignore_index, reduction):
-        xr, w, t = _rows(x), _rows(weight), target.reshape(-1).to(torch.int64).contiguous()
+        xr, w, t = _rows(x), _rows(weight), _classes(target)
         loss, lse = _loss_forward(xr, w, t, ignore_index, reduction)
         ctx.save_for_backward(xr, w, t, lse)
         ctx.args = (ignore_index, reduction, x.shape)
-        return loss.view(target.shape) if reduction == 0 else loss
+        return loss if reduction or target.dim() == 1 else loss.view(target.shape)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
         xr, w, t, lse = ctx.saved_tensors
         ignore_index, reduction, shape = ctx.args
-        g = grad.reshape(-1).to(torch.float32).contiguous()
-        dx, dw = _loss_backward(xr, w, t, lse, g, ignore_index, reduction, ctx.needs_input_grad[:2])
-        return dx.view(shape) if dx is not None else None, dw, None, None, None
+        g = grad if grad.dtype == torch.float32 and grad.is_contiguous() else grad.to(torch.float32).contiguous()
+        dx, dw = _loss_backward(xr, w, t, lse, g, ignore_index, reduction, ctx.needs_input_grad)
+        return dx if dx is None or len(shape) == 2 else dx.view(shape), dw, None, None, None
 
 
-def linear_cross_entropy(x, weight, target, ignore_index=-100, reduction="mean"):
+def _refuse_linear_cross_entropy(x, weight, target, reduction):
+    """Says what is wrong with the arguments of linear_cross_entropy, if anything is."""
     name = "linear_cross_entropy"
     _check_values(name, "x", x)
     _check_values(name, "weight", weight)
@@ -303,7 +323,15 @@ def linear_cross_entropy(x, weight, target, ignore_index=-100, reduction="mean")
     if target.dtype not in (torch.int64, torch.int32) or target.shape != x.shape[:-1]:
         raise ValueError(f"sw_gcn.{name}: target must hold one int64 or int32 class for each row of x")
     _same_device(name, x, weight, target)
-    if _records(x, weight):
-        return _LinearCrossEntropy.apply(x, weight, target, int(ignore_index), _REDUCTIONS[reduction])
-    loss, _ = _loss_forward(_rows(x), _rows(weight), target.reshape(-1).to(torch.int64).contiguous(), int(ignore_index), _REDUCTIONS[reduction])
-    return loss.view(target.shape) if reduction == "none" else loss
+
+
+def linear_cross_entropy(x, weight, target, ignore_index=-100, reduction="mean"):
+    d, code = x.get_device(), _REDUCTIONS.get(reduction)
+    if not (_fine(x, d) and _fine(weight, d) and target.is_cuda and target.get_device() == d and x.dtype == weight.dtype and code is not None
+            and weight.dim() == 2 and x.dim() > 0 and x.shape[-1] == weight.shape[1] and weight.numel() > 0
+            and target.dtype in (torch.int64, torch.int32) and target.shape == x.shape[:-1]):
+        _refuse_linear_cross_entropy(x, weight, target, reduction)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+        return _LinearCrossEntropy.apply(x, weight, target, ignore_index, code)
+    loss, _ = _loss_forward(_rows(x), _rows(weight), _classes(target), ignore_index, code)
+    return loss if code or target.dim() == 1 else loss.view(target.shape)
