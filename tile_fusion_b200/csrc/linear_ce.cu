@@ -284,12 +284,13 @@ struct CeSpace {
   bool few, copy_x, copy_w;
 };
 
-// Slices of a cut of the long sum of a gradient product (0: not cut), so that few tiles still fill the pairs of the device.  A
-// cut has at least 32 slices (2 048 terms), so that reading the parts back stays small beside the products.
+// Slices of a cut of the long sum of a gradient product (0: not cut), so that few tiles still fill the pairs of the device.  Where tiles
+// nearly do, a cut has at least 32 slices (2 048 terms), so that reading the parts back stays small beside the products; where
+// they leave most pairs idle, at least four.
 int ce_cut(int m, int n, int k, bool along_rows) {
-  const int bn = plane_gemm_width(n, along_rows), pairs = 74;
+  const int bn = plane_gemm_width(m, n, along_rows), pairs = 74;
   const long long tiles = (long long)((m + 255) / 256) * ((n + bn - 1) / bn);
-  const int slices = (k + 63) / 64, most = std::max(1, slices / 32);
+  const int slices = (k + 63) / 64, most = std::max(1, slices / (4 * tiles <= pairs ? 4 : 32));
   int best = 1;
   double cost = 1e30;
   for (int s = 1; s <= std::min(most, pairs); ++s) {
@@ -329,7 +330,7 @@ CeSpace ce_space(char *base, int rows, int cols, int vocab, int dtype, bool back
   if (s.copy_w) s.w_hi = (unsigned short *)take(2ll * vocab * s.ldp);
   if (f32) s.w_lo = (unsigned short *)take(2ll * vocab * s.ldp);
   if (!backward) {
-    s.sums = (float2 *)take(8ll * rows * plane_gemm_parts(vocab));
+    s.sums = (float2 *)take(8ll * rows * plane_gemm_parts(rows, vocab));
     s.target_logit = (float *)take(4ll * rows);
     s.block_loss = (double *)take(8ll * ((rows + 31) / 32));
     s.block_count = (int *)take(4ll * ((rows + 31) / 32));
@@ -453,7 +454,7 @@ extern "C" int tf_linear_ce_fwd(const void *x, long long ld_x, const void *w, lo
   rc = plane_gemm(c, &sp.h->error, kCeWaitLimit, sm_count(), s);
   if (rc != TF_OK) return rc;
   const int blocks = (rows + 31) / 32;
-  ce_join_kernel<<<blocks, 256, 0, s>>>(sp.sums, plane_gemm_parts(vocab), rows, sp.target_logit, target, ignore_index, vocab, lse2,
+  ce_join_kernel<<<blocks, 256, 0, s>>>(sp.sums, plane_gemm_parts(rows, vocab), rows, sp.target_logit, target, ignore_index, vocab, lse2,
                                         reduction ? nullptr : loss, reduction ? sp.block_loss : nullptr, sp.block_count, sp.h);
   if (reduction) ce_total_kernel<<<1, 1024, 0, s>>>(sp.block_loss, sp.block_count, blocks, reduction == 1, loss);
   e = cudaGetLastError();

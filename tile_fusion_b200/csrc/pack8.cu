@@ -31,9 +31,9 @@ template <bool FLAT> struct Walk {
   }
 };
 
-// N values a thread; codes [rows][ld_codes], exponents [rows][ld_codes / 32]; columns from `cols` on become zero.
+// N values a thread, in pieces of AL; codes [rows][ld_codes], exponents [rows][ld_codes / 32]; columns from `cols` on become zero.
 // FLAT: rows of whole groups with nothing between them, one row of rows * cols values.
-template <class T, int N, bool RELU, bool FLAT>
+template <class T, int N, int AL, bool RELU, bool FLAT>
 __global__ void __launch_bounds__(kPackThreads)
 pack8_kernel(const T *__restrict__ x, long long ld, int rows, long long cols, signed char *__restrict__ codes, long long ld_codes,
              unsigned char *__restrict__ exps) {
@@ -49,7 +49,18 @@ pack8_kernel(const T *__restrict__ x, long long ld, int rows, long long cols, si
       to[u] = in ? (FLAT ? col : w.row * ld_codes + col) : -1;
 #pragma unroll
       for (int i = 0; i < N; ++i) v[u].v[i] = from_float<T>(0.f);
-      if (in && (FLAT || col < cols)) v[u] = load_raw<T, N>(x + (FLAT ? col : w.row * ld + col));
+      if constexpr (AL == N) {
+        if (in && (FLAT || col < cols)) v[u] = load_raw<T, N>(x + (FLAT ? col : w.row * ld + col));
+      } else if (in) {
+        const T *p = x + w.row * ld + col;
+#pragma unroll
+        for (int i = 0; i < N; i += AL) {
+          if (col + i >= cols) continue;
+          const Pack<T, AL> a = *reinterpret_cast<const Pack<T, AL> *>(p + i);
+#pragma unroll
+          for (int k = 0; k < AL; ++k) v[u].v[i + k] = a.v[k];
+        }
+      }
     }
 #pragma unroll
     for (int u = 0; u < kPackUnroll; ++u) {
@@ -91,6 +102,41 @@ unpack8_kernel(const signed char *__restrict__ codes, long long ld_codes, const 
       for (int i = 0; i < N; ++i) a.v[i] = from_float<T>(v[i]);
       store_raw<T, N>(out + to[u], a);
     }
+  }
+}
+
+// Rows that start anywhere, but one behind the other: 16 bytes of values a thread as the whole array has them, across the ends of
+// rows, so that what is written are whole sectors; the codes come byte by byte, from L1.
+template <class T>
+__global__ void __launch_bounds__(kPackThreads)
+unpack8_flat_kernel(const signed char *__restrict__ codes, int ld_codes, const unsigned char *__restrict__ exps, long long all, int cols, T *__restrict__ out) {
+  constexpr int N = 16 / (int)sizeof(T);
+  const long long step = (long long)gridDim.x * blockDim.x * N, d_row = step / cols;
+  const int d_col = (int)(step - d_row * cols), ld_e = ld_codes / kPackGroup;
+  long long at = (blockIdx.x * (long long)blockDim.x + threadIdx.x) * N, row = at / cols;
+  int col = (int)(at - row * cols);
+  for (; at < all; at += step, row += d_row, col += d_col) {
+    if (col >= cols) { col -= cols; ++row; }
+    const signed char *c = codes + row * ld_codes;
+    const unsigned char *e = exps + row * ld_e;
+    int q = col;
+    float v[N];
+    int code[N];
+    unsigned exp[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const bool in = at + i < all;
+      code[i] = in ? __ldg(c + q) : 0;
+      exp[i] = in ? __ldg(e + q / kPackGroup) : 127;
+      if (++q == cols) { q = 0; c += ld_codes; e += ld_e; }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = unpack8_value(code[i], unpack8_step(exp[i]));
+    if (at + N <= all) store_pack<T, N>(out + at, v);
+    else
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (at + i < all) out[at + i] = from_float<T>(v[i]);
   }
 }
 
@@ -143,21 +189,33 @@ int check(const char *who, const void *values, long long ld, int dtype, int rows
   return TF_OK;
 }
 
+template <class T, int N, int AL> void launch_pack_as(const void *x, long long ld, int rows, int cols, signed char *codes, int ld_codes, unsigned char *exps,
+                                                     bool relu, cudaStream_t s) {
+  const unsigned grid = pack_grid((long long)rows * (ld_codes / N));
+  if constexpr (AL == N)
+    if (ld == cols && cols == ld_codes) {
+      const long long all = (long long)rows * cols;
+      if (relu) pack8_kernel<T, N, N, true, true><<<grid, kPackThreads, 0, s>>>((const T *)x, all, 1, all, codes, all, exps);
+      else pack8_kernel<T, N, N, false, true><<<grid, kPackThreads, 0, s>>>((const T *)x, all, 1, all, codes, all, exps);
+      return;
+    }
+  if (relu) pack8_kernel<T, N, AL, true, false><<<grid, kPackThreads, 0, s>>>((const T *)x, ld, rows, cols, codes, ld_codes, exps);
+  else pack8_kernel<T, N, AL, false, false><<<grid, kPackThreads, 0, s>>>((const T *)x, ld, rows, cols, codes, ld_codes, exps);
+}
+// n: values that one access takes; 16 bytes of them to a thread where it takes fewer
 template <class T, int N> void launch_pack(const void *x, long long ld, int rows, int cols, signed char *codes, int ld_codes, unsigned char *exps, bool relu,
                                            cudaStream_t s) {
-  const unsigned grid = pack_grid((long long)rows * (ld_codes / N));
-  if (N >= 4 && ld == cols && cols == ld_codes) {
-    const long long all = (long long)rows * cols;
-    if (relu) pack8_kernel<T, N, true, true><<<grid, kPackThreads, 0, s>>>((const T *)x, all, 1, all, codes, all, exps);
-    else pack8_kernel<T, N, false, true><<<grid, kPackThreads, 0, s>>>((const T *)x, all, 1, all, codes, all, exps);
-  } else if (relu) pack8_kernel<T, N, true, false><<<grid, kPackThreads, 0, s>>>((const T *)x, ld, rows, cols, codes, ld_codes, exps);
-  else pack8_kernel<T, N, false, false><<<grid, kPackThreads, 0, s>>>((const T *)x, ld, rows, cols, codes, ld_codes, exps);
+  constexpr int M = 16 / (int)sizeof(T);
+  launch_pack_as<T, (N < M ? M : N), N>(x, ld, rows, cols, codes, ld_codes, exps, relu, s);
 }
 template <class T, int N> void launch_unpack(const signed char *codes, int ld_codes, const unsigned char *exps, int rows, int cols, void *out, long long ld,
                                              cudaStream_t s) {
   const unsigned grid = pack_grid((long long)rows * (cols / N));
   const long long all = (long long)rows * cols;
-  if (N >= 4 && ld == cols && cols == ld_codes) unpack8_kernel<T, N, true><<<grid, kPackThreads, 0, s>>>(codes, all, exps, 1, all, (T *)out, all);
+  constexpr int M = 16 / (int)sizeof(T);
+  if (N >= M && ld == cols && cols == ld_codes) unpack8_kernel<T, N, true><<<grid, kPackThreads, 0, s>>>(codes, all, exps, 1, all, (T *)out, all);
+  else if (N < M && ld == cols && (reinterpret_cast<uintptr_t>(out) & 15) == 0)
+    unpack8_flat_kernel<T><<<pack_grid(4 * (all / M + 1)), kPackThreads, 0, s>>>(codes, ld_codes, exps, all, cols, (T *)out);
   else unpack8_kernel<T, N, false><<<grid, kPackThreads, 0, s>>>(codes, ld_codes, exps, rows, cols, (T *)out, ld);
 }
 template <class T, int N> void launch_mask(const signed char *codes, int ld_codes, int rows, int cols, void *grad, long long ld, cudaStream_t s) {

@@ -402,11 +402,14 @@ cudaError_t pg_launch(const CUtensorMap *maps, const PlaneGemmParams &P, int pai
 
 }  // namespace
 
-int plane_gemm_width(int n, bool b_along_rows) {
-  if (n <= 64 && !b_along_rows) return 64;
-  return n <= 128 ? 128 : 256;
+// As narrow as keeps every pair of SMs at a tile at most: few rows leave few tiles, whose sums then take as long as their width.
+int plane_gemm_width(int m, int n, bool b_along_rows) {
+  const long long tiles_m = (m + 255) / 256;
+  for (int bn = b_along_rows ? 128 : 64; bn < 256; bn *= 2)
+    if (n <= bn || tiles_m * ((n + bn - 1) / bn) <= 74) return bn;
+  return 256;
 }
-int plane_gemm_parts(int n) { const int bn = plane_gemm_width(n, false); return 2 * ((n + bn - 1) / bn); }
+int plane_gemm_parts(int m, int n) { const int bn = plane_gemm_width(m, n, false); return 2 * ((n + bn - 1) / bn); }
 
 int plane_gemm_splits(int k, int split_slices) {
   const int slices = (k + kPgSlice - 1) / kPgSlice;
@@ -414,7 +417,7 @@ int plane_gemm_splits(int k, int split_slices) {
 }
 
 int plane_gemm(const PlaneGemmCall &c, int *error, int wait_limit, int sm_count, cudaStream_t s) {
-  const int bn = plane_gemm_width(c.n, c.b.along_rows);
+  const int bn = plane_gemm_width(c.m, c.n, c.b.along_rows);
   PlaneGemmParams P = {};
   P.m = c.m; P.n = c.n;
   P.slices = (c.k + kPgSlice - 1) / kPgSlice;

@@ -45,8 +45,8 @@ struct PlaneGemmCall {
   long long ld_slope = 0;
 };
 
-int plane_gemm_width(int n, bool b_along_rows);  // columns of a tile
-int plane_gemm_parts(int n);                     // parts that kPlaneSoftmaxSums writes for a row
+int plane_gemm_width(int m, int n, bool b_along_rows);  // columns of a tile
+int plane_gemm_parts(int m, int n);                     // parts that kPlaneSoftmaxSums writes for a row
 int plane_gemm_splits(int k, int split_slices);  // cuts of a sum of k terms
 int plane_gemm(const PlaneGemmCall &c, int *error, int wait_limit, int sm_count, cudaStream_t s);
 
