@@ -18,8 +18,8 @@ namespace tfk {
 namespace {
 
 // One row whose statistics are known.
-template <class T, int AL, int NV, bool KEEP8, class Col, class Value>
-__device__ __forceinline__ void ln_write(const LnParams &P, Value x, long long row, bool in, float mean, float rstd, Col col, const float (&w)[NV][kLnN<T>],
+template <class T, int AL, int PIECE, int NV, bool KEEP8, class Value>
+__device__ __forceinline__ void ln_write(const LnParams &P, Value x, long long row, bool in, float mean, float rstd, LnCols<T, PIECE> col, const float (&w)[NV][kLnN<T>],
                                          const float (&b)[NV][kLnN<T>]) {
   constexpr int N = kLnN<T>;
 #pragma unroll
@@ -30,16 +30,16 @@ __device__ __forceinline__ void ln_write(const LnParams &P, Value x, long long r
     for (int k = 0; k < N; ++k) v[k] = to_float(raw.v[k]);
     if (KEEP8) {
       unsigned code[N];
-      const int e = pack8_lanes<N, false>(v, code);
-      if (in && col(i) < P.ld_codes) {
-        store_codes<N>(P.codes + row * P.ld_codes + col(i), code);
-        if (col(i) % kPackGroup == 0) P.exps[row * (P.ld_codes / kPackGroup) + col(i) / kPackGroup] = (unsigned char)(e + 127);
+      const int e = pack8_lanes<N, false>(v, code), c = col(i, 0);
+      if (in && c < P.ld_codes) {
+        store_codes<N>(P.codes + row * P.ld_codes + c, code);
+        if (c % kPackGroup == 0) P.exps[row * (P.ld_codes / kPackGroup) + c / kPackGroup] = (unsigned char)(e + 127);
       }
     }
-    if (!in || col(i) >= P.cols) continue;
+    if (!in || col(i, 0) >= P.cols) continue;
 #pragma unroll
     for (int k = 0; k < N; ++k) v[k] = fmaf((v[k] - mean) * rstd, w[i][k], b[i][k]);
-    ln_store<T, AL>(static_cast<T *>(P.y) + row * P.ld_y, col(i), P.cols, v);
+    ln_store<T, AL, PIECE>(static_cast<T *>(P.y) + row * P.ld_y, col, i, P.cols, v);
   }
 }
 
@@ -53,12 +53,12 @@ template <class T, int NV, class Value> __device__ __forceinline__ float ln_tota
   }
   return s;
 }
-template <class T, int NV, class Value, class Col> __device__ __forceinline__ float ln_spread(Value x, float mean, int cols, Col col) {
+template <class T, int NV, int PIECE, class Value> __device__ __forceinline__ float ln_spread(Value x, float mean, int cols, LnCols<T, PIECE> col) {
   float s = 0.f;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const Pack<T, kLnN<T>> v = x(i);
-    if (col(i) + kLnN<T> <= cols) {
+    if (col(i, kLnN<T> - 1) < cols) {
 #pragma unroll
       for (int k = 0; k < kLnN<T>; ++k) {
         const float c = to_float(v.v[k]) - mean;
@@ -67,7 +67,7 @@ template <class T, int NV, class Value, class Col> __device__ __forceinline__ fl
     } else {
 #pragma unroll
       for (int k = 0; k < kLnN<T>; ++k) {
-        const float c = col(i) + k < cols ? to_float(v.v[k]) - mean : 0.f;
+        const float c = col(i, k) < cols ? to_float(v.v[k]) - mean : 0.f;
         s = fmaf(c, c, s);
       }
     }
@@ -76,24 +76,24 @@ template <class T, int NV, class Value, class Col> __device__ __forceinline__ fl
 }
 
 // Eight lanes or a warp to a row.
-template <class T, int AL, int NV, int LANES, bool KEEP8>
+template <class T, int AL, int PIECE, int NV, int LANES, bool KEEP8>
 __global__ void __launch_bounds__(kLnWarpThreads) ln_forward_kernel(const LnParams P) {
   constexpr int N = kLnN<T>;
   LnPlace<T, LANES> at;
   const int t = at.t;
-  auto col = [&](int i) { return (i * LANES + t) * N; };
+  const LnCols<T, PIECE> col = {t, LANES};
   int slot = 0;
   float w[NV][N], b[NV][N];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    ln_weight<T>(P.w, P, col(i), 1.f, w[i]);
-    ln_weight<T>(P.b, P, col(i), 0.f, b[i]);
+    ln_weight<T, PIECE>(P.w, P, col, i, 1.f, w[i]);
+    ln_weight<T, PIECE>(P.b, P, col, i, 0.f, b[i]);
   }
   const float over = 1.f / (float)P.cols;
   Pack<T, N> next[NV];
   auto fetch = [&](long long row) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) next[i] = ln_load<T, AL>(static_cast<const T *>(P.x) + row * P.ld_x, col(i), P.cols, row < P.rows);
+    for (int i = 0; i < NV; ++i) next[i] = ln_load<T, AL, PIECE>(static_cast<const T *>(P.x) + row * P.ld_x, col, i, P.cols, row < P.rows);
   };
   fetch(at.row);
   for (; at.more(P.rows); at.row += at.step) {
@@ -106,10 +106,10 @@ __global__ void __launch_bounds__(kLnWarpThreads) ln_forward_kernel(const LnPara
     float sum[1] = {ln_total<T, NV>(x)};
     ln_sum<LANES, 1>(sum, nullptr, slot);
     const float mean = sum[0] * over;
-    float var[1] = {ln_spread<T, NV>(x, mean, P.cols, col)};
+    float var[1] = {ln_spread<T, NV, PIECE>(x, mean, P.cols, col)};
     ln_sum<LANES, 1>(var, nullptr, slot);
     const float rstd = 1.f / sqrtf(var[0] * over + P.eps);
-    ln_write<T, AL, NV, KEEP8>(P, x, at.row, in, mean, rstd, col, w, b);
+    ln_write<T, AL, PIECE, NV, KEEP8>(P, x, at.row, in, mean, rstd, col, w, b);
     if (in && t == 0) {
       if (P.mean) P.mean[at.row] = mean;
       if (P.rstd) P.rstd[at.row] = rstd;
@@ -119,21 +119,21 @@ __global__ void __launch_bounds__(kLnWarpThreads) ln_forward_kernel(const LnPara
 
 // A CTA to a row, R rows a turn.  Shared memory: [turn][row][NV][thread].
 template <class T, int NV> __host__ __device__ constexpr int ln_turn_bytes(int threads) { return ln_rows_at_once<NV>() * NV * threads * 16; }
-template <class T, int AL, int NV, bool KEEP8>
+template <class T, int AL, int PIECE, int NV, bool KEEP8>
 __global__ void __launch_bounds__(kLnRowThreads, 1) ln_forward_rows_kernel(const LnParams P) {
   constexpr int N = kLnN<T>, R = ln_rows_at_once<NV>(), AHEAD = ln_ahead<NV>();
   extern __shared__ float4 rows_smem[];
   __shared__ float scratch[2][kLnRowThreads / 32][R];
   const int t = threadIdx.x, lanes = blockDim.x;
   Pack<T, N> *sx = reinterpret_cast<Pack<T, N> *>(rows_smem);
-  auto col = [&](int i) { return (i * lanes + t) * N; };
+  const LnCols<T, PIECE> col = {t, lanes};
   auto at = [&](int turn, int r, int i) { return ((turn * R + r) * NV + i) * lanes + t; };
   int slot = 0;
   float w[NV][N], b[NV][N];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    ln_weight<T>(P.w, P, col(i), 1.f, w[i]);
-    ln_weight<T>(P.b, P, col(i), 0.f, b[i]);
+    ln_weight<T, PIECE>(P.w, P, col, i, 1.f, w[i]);
+    ln_weight<T, PIECE>(P.b, P, col, i, 0.f, b[i]);
   }
   const float over = 1.f / (float)P.cols;
   const long long step = gridDim.x * (long long)R;
@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(kLnRowThreads, 1) ln_forward_rows_kernel(const
     for (int r = 0; r < R; ++r) {
       const bool in = row + r < P.rows;
 #pragma unroll
-      for (int i = 0; i < NV; ++i) ln_copy<T, AL>(sx + at(turn, r, i), static_cast<const T *>(P.x) + (in ? row + r : 0) * P.ld_x, col(i), P.cols, in);
+      for (int i = 0; i < NV; ++i) ln_copy<T, AL, PIECE>(sx + at(turn, r, i), static_cast<const T *>(P.x) + (in ? row + r : 0) * P.ld_x, col, i, P.cols, in);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -160,14 +160,14 @@ __global__ void __launch_bounds__(kLnRowThreads, 1) ln_forward_rows_kernel(const
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       sum[r] *= over;  // the mean
-      var[r] = ln_spread<T, NV>([&](int i) { return sx[at(turn, r, i)]; }, sum[r], P.cols, col);
+      var[r] = ln_spread<T, NV, PIECE>([&](int i) { return sx[at(turn, r, i)]; }, sum[r], P.cols, col);
     }
     ln_sum<0, R>(var, scratch, slot);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const bool in = row + r < P.rows;
       const float rstd = 1.f / sqrtf(var[r] * over + P.eps);
-      ln_write<T, AL, NV, KEEP8>(P, [&](int i) { return sx[at(turn, r, i)]; }, row + r, in, sum[r], rstd, col, w, b);
+      ln_write<T, AL, PIECE, NV, KEEP8>(P, [&](int i) { return sx[at(turn, r, i)]; }, row + r, in, sum[r], rstd, col, w, b);
       if (in && t == 0) {
         if (P.mean) P.mean[row + r] = sum[r];
         if (P.rstd) P.rstd[row + r] = rstd;
@@ -178,15 +178,15 @@ __global__ void __launch_bounds__(kLnRowThreads, 1) ln_forward_rows_kernel(const
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-template <class T, int AL, bool KEEP8> cudaError_t ln_by_nv(const LnShape &s, const LnParams &P, cudaStream_t st) {
+template <class T, int AL, int PIECE, bool KEEP8> cudaError_t ln_by_nv(const LnShape &s, const LnParams &P, cudaStream_t st) {
   int ctas;
 #define TF_LN(NV)                                                                                                                              \
   if (s.nv == NV) {                                                                                                                            \
     if (s.lanes == 0)                                                                                                                          \
-      return ln_go(ln_forward_rows_kernel<T, AL, NV, KEEP8>, s, P, ln_rows_at_once<NV>(), (ln_ahead<NV>() + 1) * ln_turn_bytes<T, NV>(s.threads), ctas, st); \
+      return ln_go(ln_forward_rows_kernel<T, AL, PIECE, NV, KEEP8>, s, P, ln_rows_at_once<NV>(), (ln_ahead<NV>() + 1) * ln_turn_bytes<T, NV>(s.threads), ctas, st); \
     if constexpr (NV <= 16 / kLnN<T>) {                                                                                                        \
-      if (s.lanes == 32) return ln_go(ln_forward_kernel<T, AL, NV, 32, KEEP8>, s, P, kLnWarpThreads / 32, 0, ctas, st);                         \
-      return ln_go(ln_forward_kernel<T, AL, NV, 8, KEEP8>, s, P, kLnWarpThreads / 8, 0, ctas, st);                                             \
+      if (s.lanes == 32) return ln_go(ln_forward_kernel<T, AL, PIECE, NV, 32, KEEP8>, s, P, kLnWarpThreads / 32, 0, ctas, st);                         \
+      return ln_go(ln_forward_kernel<T, AL, PIECE, NV, 8, KEEP8>, s, P, kLnWarpThreads / 8, 0, ctas, st);                                             \
     }                                                                                                                                          \
   }
   TF_LN(1) TF_LN(2) TF_LN(4)
@@ -196,8 +196,10 @@ template <class T, int AL, bool KEEP8> cudaError_t ln_by_nv(const LnShape &s, co
 }
 template <class T> cudaError_t ln_by_align(const LnShape &s, const LnParams &P, cudaStream_t st) {
   constexpr int N = kLnN<T>;
-  if (P.codes) return s.al == N ? ln_by_nv<T, N, true>(s, P, st) : s.al == 2 ? ln_by_nv<T, 2, true>(s, P, st) : ln_by_nv<T, 1, true>(s, P, st);
-  return s.al == N ? ln_by_nv<T, N, false>(s, P, st) : s.al == 2 ? ln_by_nv<T, 2, false>(s, P, st) : ln_by_nv<T, 1, false>(s, P, st);
+  if (P.codes) return s.al == N ? ln_by_nv<T, N, N, true>(s, P, st) : s.al == 2 ? ln_by_nv<T, 2, N, true>(s, P, st) : ln_by_nv<T, 1, N, true>(s, P, st);
+  if (s.piece == N) return s.al == N ? ln_by_nv<T, N, N, false>(s, P, st) : ln_by_nv<T, 1, N, false>(s, P, st);
+  if (s.piece == 2) return s.al == 2 ? ln_by_nv<T, 2, 2, false>(s, P, st) : ln_by_nv<T, 1, 2, false>(s, P, st);
+  return ln_by_nv<T, 1, 1, false>(s, P, st);
 }
 
 }  // namespace
@@ -230,7 +232,7 @@ extern "C" int tf_layer_norm_fwd(const void *x, long long ld_x, int dtype, const
   P.rows = rows; P.cols = cols; P.eps = eps; P.y = y; P.ld_y = ld_y; P.mean = mean; P.rstd = rstd;
   P.codes = codes; P.ld_codes = ld_codes; P.exps = exponents;
   // (codes reach to the end of the columns' group)
-  const LnShape s = ln_shape(ln_align(cols, bytes, {{x, ld_x}, {y, ld_y}}), codes ? ld_codes : cols, bytes);
+  const LnShape s = ln_shape(ln_pieces(cols, bytes, codes != nullptr, {{x, ld_x}, {y, ld_y}}), codes ? ld_codes : cols, bytes);
   cudaStream_t st = (cudaStream_t)stream;
   const cudaError_t e = dtype == TF_F32 ? ln_by_align<float>(s, P, st) : dtype == TF_BF16 ? ln_by_align<__nv_bfloat16>(s, P, st) : ln_by_align<__half>(s, P, st);
   return e == cudaSuccess ? TF_OK : tf::fail(TF_ERR_CUDA, std::string("tf_layer_norm_fwd: ") + cudaGetErrorString(e));

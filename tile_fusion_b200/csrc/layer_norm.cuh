@@ -1,7 +1,9 @@
 // What the two passes of the layer norm share (layer_norm.cu, layer_norm_grad.cu): how a row lies over threads.
 //
-// A thread holds N neighbouring columns (16 bytes of values) NV times, whatever the rows' alignment: they come and go in pieces of
-// AL values, all N where every row starts on 16 bytes, else two, else one.
+// A thread holds N columns (16 bytes of values) NV times, in pieces of PIECE neighbours: all N, two or one, whichever divides the
+// width, so that rows one behind the other start on whole pieces.  A warp's pieces lie side by side, and its accesses are whole
+// sectors.  (With the 8 bits always N: a group of 32 belongs to few lanes.)  Accesses are of AL values, a piece or, where operands
+// are aligned otherwise, less.  Which columns a thread adds up depends on the width alone, so results do not depend on alignment.
 #pragma once
 #include "pack8.cuh"
 #include "tf_internal.h"
@@ -27,7 +29,13 @@ struct LnParams {
 
 template <class T> constexpr int kLnN = 16 / (int)sizeof(T);
 
-template <class T, int AL> __device__ __forceinline__ Pack<T, kLnN<T>> ln_load(const T *row, int col, int cols, bool in) {
+// The column of value k of a thread's i-th access; PIECE neighbouring columns of a thread.
+template <class T, int PIECE> struct LnCols {
+  int t, lanes;
+  __device__ int operator()(int i, int k) const { return ((i * (kLnN<T> / PIECE) + k / PIECE) * lanes + t) * PIECE + k % PIECE; }
+};
+
+template <class T, int AL, int PIECE> __device__ __forceinline__ Pack<T, kLnN<T>> ln_load(const T *row, LnCols<T, PIECE> col, int i, int cols, bool in) {
   constexpr int N = kLnN<T>;
   Pack<T, N> v;
 #pragma unroll
@@ -35,27 +43,28 @@ template <class T, int AL> __device__ __forceinline__ Pack<T, kLnN<T>> ln_load(c
     Pack<T, AL> a;
 #pragma unroll
     for (int k = 0; k < AL; ++k) a.v[k] = from_float<T>(0.f);
-    if (in && col + p < cols) a = *reinterpret_cast<const Pack<T, AL> *>(row + col + p);
+    if (in && col(i, p) < cols) a = *reinterpret_cast<const Pack<T, AL> *>(row + col(i, p));
 #pragma unroll
     for (int k = 0; k < AL; ++k) v.v[p + k] = a.v[k];
   }
   return v;
 }
-template <class T, int AL> __device__ __forceinline__ void ln_store(T *row, int col, int cols, const float (&v)[kLnN<T>]) {
+template <class T, int AL, int PIECE> __device__ __forceinline__ void ln_store(T *row, LnCols<T, PIECE> col, int i, int cols, const float (&v)[kLnN<T>]) {
   constexpr int N = kLnN<T>;
 #pragma unroll
   for (int p = 0; p < N; p += AL) {
-    if (col + p >= cols) break;
+    if (col(i, p) >= cols) break;
     float a[AL];
 #pragma unroll
     for (int k = 0; k < AL; ++k) a[k] = v[p + k];
-    store_pack<T, AL>(row + col + p, a);
+    store_pack<T, AL>(row + col(i, p), a);
   }
 }
-// N weights from `col` on, `none` where there are none.
-template <class T> __device__ __forceinline__ void ln_weight(const void *w, const LnParams &P, int col, float none, float (&v)[kLnN<T>]) {
+// A thread's weights of its i-th access, `none` where there are none.
+template <class T, int PIECE> __device__ __forceinline__ void ln_weight(const void *w, const LnParams &P, LnCols<T, PIECE> cols_, int i, float none, float (&v)[kLnN<T>]) {
   constexpr int N = kLnN<T>;
-  if (w && P.w_whole && col + N <= P.cols) {
+  const int col = cols_(i, 0);
+  if (PIECE == N && w && P.w_whole && col + N <= P.cols) {
     if (P.w_dtype == TF_F32) {
 #pragma unroll
       for (int k = 0; k < N; k += 4) {
@@ -74,7 +83,7 @@ template <class T> __device__ __forceinline__ void ln_weight(const void *w, cons
     return;
   }
 #pragma unroll
-  for (int k = 0; k < N; ++k) v[k] = w && col + k < P.cols ? load_value(w, P.w_dtype, col + k) : none;
+  for (int k = 0; k < N; ++k) v[k] = w && cols_(i, k) < P.cols ? load_value(w, P.w_dtype, cols_(i, k)) : none;
 }
 
 // K sums over LANES lanes, or (LANES == 0) over the CTA; `slot` alternates between two scratch arrays.
@@ -105,15 +114,15 @@ template <int NV> __host__ __device__ constexpr int ln_rows_at_once() { return N
 template <int NV> __host__ __device__ constexpr int ln_ahead() { return NV >= 8 ? 0 : 2; }
 
 // Copies of AL values of a thread into its own shared memory, zeros where there are none.  Below four bytes there is no asynchronous copy.
-template <class T, int AL> __device__ __forceinline__ void ln_copy(Pack<T, kLnN<T>> *to, const T *row, int col, int cols, bool in) {
+template <class T, int AL, int PIECE> __device__ __forceinline__ void ln_copy(Pack<T, kLnN<T>> *to, const T *row, LnCols<T, PIECE> col, int i, int cols, bool in) {
   constexpr int N = kLnN<T>, BYTES = AL * (int)sizeof(T);
-  if constexpr (BYTES < 4) *to = ln_load<T, AL>(row, col, cols, in);
+  if constexpr (BYTES < 4) *to = ln_load<T, AL, PIECE>(row, col, i, cols, in);
   else {
     const unsigned dst = (unsigned)__cvta_generic_to_shared(to);
 #pragma unroll
     for (int p = 0; p < N; p += AL) {
-      const bool here = in && col + p < cols;
-      const T *src = here ? row + col + p : row;  // (nothing is read for a size of zero)
+      const bool here = in && col(i, p) < cols;
+      const T *src = here ? row + col(i, p) : row;  // (nothing is read for a size of zero)
       if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(here ? 16 : 0) : "memory");
       else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst + p * (int)sizeof(T)), "l"(src), "n"(BYTES), "r"(here ? BYTES : 0) : "memory");
     }
@@ -129,32 +138,34 @@ template <class T, int LANES> struct LnPlace {
     row = blockIdx.x * (long long)(blockDim.x / LANES) + threadIdx.x / LANES;
     step = (long long)gridDim.x * (blockDim.x / LANES);
   }
-  __device__ int col(int i) const { return (i * LANES + t) * kLnN<T>; }
   // rows of a warp's lanes end at different times: it goes on as one
   __device__ bool more(int rows) const { return LANES < 32 ? __any_sync(0xffffffffu, row < rows) : row < rows; }
 };
 
-struct LnShape { int al, nv, lanes, threads; };  // lanes 0: a CTA to a row
+struct LnShape { int al, piece, nv, lanes, threads; };  // lanes 0: a CTA to a row
 
-inline int ln_align(int cols, int bytes, std::initializer_list<std::pair<const void *, long long>> operands) {
-  for (int al : {16 / bytes, 2}) {
-    bool whole = cols % al == 0;
-    for (const auto &o : operands) whole = whole && (!o.first || (o.second % al == 0 && reinterpret_cast<uintptr_t>(o.first) % (al * bytes) == 0));
-    if (whole) return al;
+// al and piece of a shape
+inline LnShape ln_pieces(int cols, int bytes, bool keep8, std::initializer_list<std::pair<const void *, long long>> operands) {
+  const int n = 16 / bytes, piece = keep8 || cols % n == 0 ? n : cols % 2 == 0 ? 2 : 1;
+  int al = 1;
+  for (int k : {2, n}) {
+    bool whole = cols % k == 0 && k <= piece && (keep8 || k == piece);
+    for (const auto &o : operands) whole = whole && (!o.first || (o.second % k == 0 && reinterpret_cast<uintptr_t>(o.first) % (k * bytes) == 0));
+    if (whole) al = k;
   }
-  return 1;
+  return {al, piece, 1, 0, 0};
 }
 // Eight lanes to a row where they hold it with 16 values each, a warp where it does (512 columns), a CTA beyond: of as many threads as
 // hold it with one access each up to 256, with two, four or (fp32) eight up to 512 (16 384 x 4 096 bf16, forward and backward: 256
 // threads with two 67 and 98 us, 512 with one 74 and 108).
-inline LnShape ln_shape(int al, int cols, int bytes) {
+inline LnShape ln_shape(LnShape s, int cols, int bytes) {
   const int n = 16 / bytes, vecs = (cols + n - 1) / n, most = 16 / n;
   auto least = [&](int lanes) { int nv = 1; while (lanes * nv < vecs) nv *= 2; return nv; };
-  if (vecs <= 8 * most) return {al, least(8), 8, kLnWarpThreads};
-  if (vecs <= 32 * most) return {al, least(32), 32, kLnWarpThreads};
+  if (vecs <= 8 * most) return {s.al, s.piece, least(8), 8, kLnWarpThreads};
+  if (vecs <= 32 * most) return {s.al, s.piece, least(32), 32, kLnWarpThreads};
   int nv = 1;
   while ((vecs + nv - 1) / nv > (nv == 1 ? 256 : kLnRowThreads)) nv *= 2;
-  return {al, nv, 0, ((vecs + nv - 1) / nv + 31) / 32 * 32};
+  return {s.al, s.piece, nv, 0, ((vecs + nv - 1) / nv + 31) / 32 * 32};
 }
 // What the runtime says of a kernel's resident CTAs, asked once (it takes 2 us to say so).
 inline cudaError_t ln_occupancy(const void *f, int threads, size_t smem, int &each) {

@@ -21,16 +21,17 @@ namespace tfk {
 namespace {
 
 // Eight lanes or a warp to a row.
-template <class T, int AL, int NV, int LANES, bool KEEP8>
+template <class T, int AL, int PIECE, int NV, int LANES, bool KEEP8>
 __global__ void __launch_bounds__(kLnWarpThreads) ln_backward_kernel(const LnParams P) {
   constexpr int N = kLnN<T>;
   extern __shared__ float joined[];  // [warps][2][cols]
   LnPlace<T, LANES> at;
+  const LnCols<T, PIECE> col = {at.t, LANES};
   int slot = 0;
   float w[NV][N], dw[NV][N], db[NV][N];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    ln_weight<T>(P.w, P, at.col(i), 1.f, w[i]);
+    ln_weight<T, PIECE>(P.w, P, col, i, 1.f, w[i]);
 #pragma unroll
     for (int k = 0; k < N; ++k) dw[i][k] = db[i][k] = 0.f;
   }
@@ -44,13 +45,13 @@ __global__ void __launch_bounds__(kLnWarpThreads) ln_backward_kernel(const LnPar
     if (in) { next_mean = __ldg(P.mean + row); next_rstd = __ldg(P.rstd + row); }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = at.col(i);
-      if (!KEEP8) next_x[i] = ln_load<T, AL>(static_cast<const T *>(P.x) + row * P.ld_x, c, P.cols, in);
+      const int c = col(i, 0);
+      if (!KEEP8) next_x[i] = ln_load<T, AL, PIECE>(static_cast<const T *>(P.x) + row * P.ld_x, col, i, P.cols, in);
       else if (in && c < P.cols) {
         next_c[i] = *reinterpret_cast<const Pack<signed char, N> *>(P.codes + row * P.ld_codes + c);
         next_e[i] = __ldg(P.exps + row * (P.ld_codes / kPackGroup) + c / kPackGroup);
       }
-      next_g[i] = ln_load<T, AL>(static_cast<const T *>(P.dy) + row * P.ld_dy, c, P.cols, in);
+      next_g[i] = ln_load<T, AL, PIECE>(static_cast<const T *>(P.dy) + row * P.ld_dy, col, i, P.cols, in);
     }
   };
   fetch(at.row);
@@ -64,7 +65,7 @@ __global__ void __launch_bounds__(kLnWarpThreads) ln_backward_kernel(const LnPar
       if (KEEP8) unpack8_values<N>(next_c[i], unpack8_step(next_e[i]), x);
 #pragma unroll
       for (int k = 0; k < N; ++k) {
-        const bool here = in && at.col(i) + k < P.cols;
+        const bool here = in && col(i, k) < P.cols;
         const float g = here ? to_float(next_g[i].v[k]) : 0.f;
         xh[i][k] = here ? ((KEEP8 ? x[k] : to_float(next_x[i].v[k])) - mean) * rstd : 0.f;
         dw[i][k] = fmaf(g, xh[i][k], dw[i][k]);
@@ -79,11 +80,11 @@ __global__ void __launch_bounds__(kLnWarpThreads) ln_backward_kernel(const LnPar
     const float m0 = sum[0] * over, m1 = sum[1] * over;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      if (!P.dx || !in || at.col(i) >= P.cols) continue;
+      if (!P.dx || !in || col(i, 0) >= P.cols) continue;
       float d[N];
 #pragma unroll
       for (int k = 0; k < N; ++k) d[k] = rstd * (h[i][k] - m0 - xh[i][k] * m1);
-      ln_store<T, AL>(static_cast<T *>(P.dx) + at.row * P.ld_dx, at.col(i), P.cols, d);
+      ln_store<T, AL, PIECE>(static_cast<T *>(P.dx) + at.row * P.ld_dx, col, i, P.cols, d);
     }
   }
   if (!P.part) return;
@@ -99,7 +100,7 @@ __global__ void __launch_bounds__(kLnWarpThreads) ln_backward_kernel(const LnPar
         dw[i][k] += __shfl_xor_sync(0xffffffffu, dw[i][k], o);
         db[i][k] += __shfl_xor_sync(0xffffffffu, db[i][k], o);
       }
-      const int c = at.col(i) + k;
+      const int c = col(i, k);
       if (lane < LANES && c < P.cols) {
         joined[(warp * 2) * P.cols + c] = dw[i][k];
         joined[(warp * 2 + 1) * P.cols + c] = db[i][k];
@@ -118,7 +119,7 @@ template <int NV> __host__ __device__ constexpr int ln_grad_rows() { return NV >
 template <class T, int NV, bool KEEP8> __host__ __device__ constexpr int ln_turn_bytes(int threads) {
   return ln_grad_rows<NV>() * NV * threads * (16 + (KEEP8 ? kLnN<T> : 16));
 }
-template <class T, int AL, int NV, bool KEEP8>
+template <class T, int AL, int PIECE, int NV, bool KEEP8>
 __global__ void __launch_bounds__(kLnRowThreads, 1) ln_backward_rows_kernel(const LnParams P) {
   constexpr int N = kLnN<T>, R = ln_grad_rows<NV>(), AHEAD = ln_ahead<NV>(), TURNS = AHEAD + 1;
   extern __shared__ float4 rows_smem[];
@@ -128,13 +129,13 @@ __global__ void __launch_bounds__(kLnRowThreads, 1) ln_backward_rows_kernel(cons
   Pack<T, N> *sg = reinterpret_cast<Pack<T, N> *>(rows_smem);
   Pack<T, N> *sx = sg + (KEEP8 ? 0 : TURNS * R * NV * lanes);
   Kept *sc = reinterpret_cast<Kept *>(sg + TURNS * R * NV * lanes);
-  auto col = [&](int i) { return (i * lanes + t) * N; };
+  const LnCols<T, PIECE> col = {t, lanes};
   auto at = [&](int turn, int r, int i) { return ((turn * R + r) * NV + i) * lanes + t; };
   int slot = 0;
   float w[NV][N], dw[NV][N], db[NV][N];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    ln_weight<T>(P.w, P, col(i), 1.f, w[i]);
+    ln_weight<T, PIECE>(P.w, P, col, i, 1.f, w[i]);
 #pragma unroll
     for (int k = 0; k < N; ++k) dw[i][k] = db[i][k] = 0.f;
   }
@@ -149,11 +150,11 @@ __global__ void __launch_bounds__(kLnRowThreads, 1) ln_backward_rows_kernel(cons
       for (int i = 0; i < NV; ++i) {
         if (KEEP8) {
           const unsigned dst = (unsigned)__cvta_generic_to_shared(sc + at(turn, r, i));
-          const bool here = in && col(i) < P.cols;
-          asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(P.codes + q * P.ld_codes + (here ? col(i) : 0)), "n"(N),
+          const bool here = in && col(i, 0) < P.cols;
+          asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(P.codes + q * P.ld_codes + (here ? col(i, 0) : 0)), "n"(N),
                        "r"(here ? N : 0) : "memory");
-        } else ln_copy<T, AL>(sx + at(turn, r, i), static_cast<const T *>(P.x) + q * P.ld_x, col(i), P.cols, in);
-        ln_copy<T, AL>(sg + at(turn, r, i), static_cast<const T *>(P.dy) + q * P.ld_dy, col(i), P.cols, in);
+        } else ln_copy<T, AL, PIECE>(sx + at(turn, r, i), static_cast<const T *>(P.x) + q * P.ld_x, col, i, P.cols, in);
+        ln_copy<T, AL, PIECE>(sg + at(turn, r, i), static_cast<const T *>(P.dy) + q * P.ld_dy, col, i, P.cols, in);
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -174,7 +175,7 @@ __global__ void __launch_bounds__(kLnRowThreads, 1) ln_backward_rows_kernel(cons
       if (KEEP8)
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-          next_e[r][i] = in && col(i) < P.cols ? __ldg(P.exps + (row + r) * (P.ld_codes / kPackGroup) + col(i) / kPackGroup) : 127;
+          next_e[r][i] = in && col(i, 0) < P.cols ? __ldg(P.exps + (row + r) * (P.ld_codes / kPackGroup) + col(i, 0) / kPackGroup) : 127;
     }
   };
   fetch_stats(row);
@@ -227,13 +228,13 @@ __global__ void __launch_bounds__(kLnRowThreads, 1) ln_backward_rows_kernel(cons
         const float m0 = sum[2 * r] * over, m1 = sum[2 * r + 1] * over;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-          if (row + r >= P.rows || col(i) >= P.cols) continue;
+          if (row + r >= P.rows || col(i, 0) >= P.cols) continue;
           float xh[N], d[N];
           hats(r, i, xh);
           const Pack<T, N> g = sg[at(turn, r, i)];
 #pragma unroll
           for (int k = 0; k < N; ++k) d[k] = rstd[r] * (to_float(g.v[k]) * w[i][k] - m0 - xh[k] * m1);
-          ln_store<T, AL>(static_cast<T *>(P.dx) + (row + r) * P.ld_dx, col(i), P.cols, d);
+          ln_store<T, AL, PIECE>(static_cast<T *>(P.dx) + (row + r) * P.ld_dx, col, i, P.cols, d);
         }
       }
     }
@@ -246,7 +247,7 @@ __global__ void __launch_bounds__(kLnRowThreads, 1) ln_backward_rows_kernel(cons
   for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-      const int c = col(i) + k;
+      const int c = col(i, k);
       if (c < P.cols) { part[c] = dw[i][k]; part[P.cols + c] = db[i][k]; }
     }
 }
@@ -269,15 +270,15 @@ __global__ void __launch_bounds__(1024) ln_join_kernel(const float *__restrict__
   } else if (c < 2 * cols && db) store_value(db, dtype, c - cols, v);
 }
 
-template <class T, int AL, bool KEEP8> cudaError_t ln_by_nv(const LnShape &s, const LnParams &P, int &ctas, cudaStream_t st) {
+template <class T, int AL, int PIECE, bool KEEP8> cudaError_t ln_by_nv(const LnShape &s, const LnParams &P, int &ctas, cudaStream_t st) {
   const size_t joined = (size_t)kLnWarpThreads / 32 * 2 * P.cols * 4;
 #define TF_LN(NV)                                                                                                                                  \
   if (s.nv == NV) {                                                                                                                                \
     if (s.lanes == 0)                                                                                                                              \
-      return ln_go(ln_backward_rows_kernel<T, AL, NV, KEEP8>, s, P, ln_grad_rows<NV>(), (ln_ahead<NV>() + 1) * ln_turn_bytes<T, NV, KEEP8>(s.threads), ctas, st); \
+      return ln_go(ln_backward_rows_kernel<T, AL, PIECE, NV, KEEP8>, s, P, ln_grad_rows<NV>(), (ln_ahead<NV>() + 1) * ln_turn_bytes<T, NV, KEEP8>(s.threads), ctas, st); \
     if constexpr (NV <= 16 / kLnN<T>) {                                                                                                            \
-      if (s.lanes == 32) return ln_go(ln_backward_kernel<T, AL, NV, 32, KEEP8>, s, P, kLnWarpThreads / 32, joined, ctas, st);                       \
-      return ln_go(ln_backward_kernel<T, AL, NV, 8, KEEP8>, s, P, kLnWarpThreads / 8, joined, ctas, st);                                           \
+      if (s.lanes == 32) return ln_go(ln_backward_kernel<T, AL, PIECE, NV, 32, KEEP8>, s, P, kLnWarpThreads / 32, joined, ctas, st);                       \
+      return ln_go(ln_backward_kernel<T, AL, PIECE, NV, 8, KEEP8>, s, P, kLnWarpThreads / 8, joined, ctas, st);                                           \
     }                                                                                                                                              \
   }
   TF_LN(1) TF_LN(2) TF_LN(4)
@@ -287,8 +288,10 @@ template <class T, int AL, bool KEEP8> cudaError_t ln_by_nv(const LnShape &s, co
 }
 template <class T> cudaError_t ln_by_align(const LnShape &s, const LnParams &P, int &ctas, cudaStream_t st) {
   constexpr int N = kLnN<T>;
-  if (P.codes) return s.al == N ? ln_by_nv<T, N, true>(s, P, ctas, st) : s.al == 2 ? ln_by_nv<T, 2, true>(s, P, ctas, st) : ln_by_nv<T, 1, true>(s, P, ctas, st);
-  return s.al == N ? ln_by_nv<T, N, false>(s, P, ctas, st) : s.al == 2 ? ln_by_nv<T, 2, false>(s, P, ctas, st) : ln_by_nv<T, 1, false>(s, P, ctas, st);
+  if (P.codes) return s.al == N ? ln_by_nv<T, N, N, true>(s, P, ctas, st) : s.al == 2 ? ln_by_nv<T, 2, N, true>(s, P, ctas, st) : ln_by_nv<T, 1, N, true>(s, P, ctas, st);
+  if (s.piece == N) return s.al == N ? ln_by_nv<T, N, N, false>(s, P, ctas, st) : ln_by_nv<T, 1, N, false>(s, P, ctas, st);
+  if (s.piece == 2) return s.al == 2 ? ln_by_nv<T, 2, 2, false>(s, P, ctas, st) : ln_by_nv<T, 1, 2, false>(s, P, ctas, st);
+  return ln_by_nv<T, 1, 1, false>(s, P, ctas, st);
 }
 
 }  // namespace
@@ -320,7 +323,7 @@ extern "C" int tf_layer_norm_bwd(const void *x, long long ld_x, const signed cha
   P.codes = const_cast<signed char *>(codes); P.ld_codes = ld_codes; P.exps = const_cast<unsigned char *>(exponents);
   P.dy = dy; P.ld_dy = ld_dy; P.dx = dx; P.ld_dx = ld_dx; P.part = sums ? work : nullptr;
   cudaStream_t st = (cudaStream_t)stream;
-  const LnShape s = ln_shape(ln_align(cols, bytes, {{codes ? nullptr : x, ld_x}, {dy, ld_dy}, {dx, ld_dx}}), cols, bytes);
+  const LnShape s = ln_shape(ln_pieces(cols, bytes, codes != nullptr, {{codes ? nullptr : x, ld_x}, {dy, ld_dy}, {dx, ld_dx}}), cols, bytes);
   int ctas = 0;
   cudaError_t e = cudaSuccess;
   if (rows > 0)

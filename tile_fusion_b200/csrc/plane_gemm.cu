@@ -280,15 +280,20 @@ plane_gemm_kernel(const __grid_constant__ CUtensorMap tm_ahi, const __grid_const
 #pragma unroll
           for (int c = 0; c < kCols; ++c) acc[c] = acc[c] * scale_a * scale_b;
           const long long at = (long long)row * P.ld_out + col;
-          const bool whole = P.ld_out * value_bytes(P.out_dtype) % 16 == 0 && (reinterpret_cast<uintptr_t>(P.out) & 15) == 0;
+          // (rows lie apart: whole sectors of 32 bytes at a time where they start on them)
+          const bool whole = P.ld_out * value_bytes(P.out_dtype) % 32 == 0 && (reinterpret_cast<uintptr_t>(P.out) & 31) == 0;
           if (P.out_dtype == TF_F32) {
             float *x = static_cast<float *>(P.out) + at;
 #pragma unroll
-            for (int c = 0; c < kCols; c += 4) {
-              if (whole && col + c + 3 < P.n) *reinterpret_cast<float4 *>(x + c) = make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
-              else {
+            for (int c = 0; c < kCols; c += 8) {
+              if (whole && col + c + 7 < P.n) {
+                Pack<float, 8> a;
 #pragma unroll
-                for (int q = 0; q < 4; ++q)
+                for (int q = 0; q < 8; ++q) a.v[q] = acc[c + q];
+                store_raw<float, 8>(x + c, a);
+              } else {
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
                   if (col + c + q < P.n) x[c + q] = acc[c + q];
               }
             }
@@ -296,15 +301,15 @@ plane_gemm_kernel(const __grid_constant__ CUtensorMap tm_ahi, const __grid_const
             unsigned short *x = static_cast<unsigned short *>(P.out) + at;
             const bool f16 = P.out_dtype == TF_F16;
 #pragma unroll
-            for (int c = 0; c < kCols; c += 8) {
-              unsigned u[4];
+            for (int c = 0; c < kCols; c += 16) {
+              Pack<unsigned, 8> a;
 #pragma unroll
-              for (int q = 0; q < 4; ++q) u[q] = pack_pair(acc[c + 2 * q], acc[c + 2 * q + 1], f16);
-              if (whole && col + c + 7 < P.n) *reinterpret_cast<uint4 *>(x + c) = make_uint4(u[0], u[1], u[2], u[3]);
+              for (int q = 0; q < 8; ++q) a.v[q] = pack_pair(acc[c + 2 * q], acc[c + 2 * q + 1], f16);
+              if (whole && col + c + 15 < P.n) store_raw<unsigned, 8>(reinterpret_cast<unsigned *>(x + c), a);
               else {
 #pragma unroll
-                for (int q = 0; q < 8; ++q)
-                  if (col + c + q < P.n) x[c + q] = (unsigned short)(u[q / 2] >> (q & 1) * 16);
+                for (int q = 0; q < 16; ++q)
+                  if (col + c + q < P.n) x[c + q] = (unsigned short)(a.v[q / 2] >> (q & 1) * 16);
               }
             }
           }

@@ -120,9 +120,10 @@ template <int PLANES, int W> __device__ __forceinline__ void wg_planes(float (&g
   }
 }
 
-// RING: G and the codes have nothing between their rows and the tile holds all columns, so that 16 rows are one run of bytes each (a
-// multiple of 16, whatever the width): one warp keeps bulk copies of them running ahead through a ring, and what the copies brought
-// is read from shared memory.  Else (more columns than a tile, strided rows) the teams read rows from memory themselves.
+// RING: G and the codes have nothing between their rows, so that 16 rows are one run of bytes each (a multiple of 16, whatever the
+// width): one warp keeps bulk copies of them running ahead through a ring, and what the copies brought is read from shared memory.
+// (Whole rows, of which a tile may use a part: 528 846 rows, 191 x 224 bf16.)  Else (strided rows, or a ring that does not fit four
+// slices) the teams read rows from memory themselves.
 template <class T, int PLANES, int MT, bool RING>
 __global__ void __launch_bounds__(wg_threads(RING), 1) weight_grad8_kernel(const WgParams P) {
   constexpr int NT = MT == 1 ? 256 : 128, kPlane = MT * 2 * kWgBlock, kStage = wg_stage_bytes(PLANES, MT);
@@ -399,7 +400,7 @@ template <class T, int PLANES> cudaError_t wg_run(const WgPlan &p, WgParams P, c
   P.ring = 0;
   P.g_bytes = kWgRows * P.na * (int)sizeof(T);
   P.ring_bytes = P.g_bytes + kWgRows * P.ld_codes + kWgRows * P.ld_codes / kPackGroup;
-  if (P.ld_g == P.na && p.tiles_a == 1 && p.tiles_b == 1 && P.ld_codes <= (p.mt == 1 ? 256 : 128) && whole(P.g) && whole(P.exps))
+  if (P.ld_g == P.na && whole(P.g) && whole(P.exps))
     P.ring = std::min(kWgMaxRing, (kWgSmem - kWgTeams * wg_stage_bytes(PLANES, p.mt)) / P.ring_bytes) / kWgTeams * kWgTeams;
   if (P.ring > 0) return p.mt == 1 ? wg_launch<T, PLANES, 1, true>(p, P, s) : wg_launch<T, PLANES, 2, true>(p, P, s);
   P.ring = 0;
