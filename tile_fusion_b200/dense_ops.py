@@ -29,7 +29,8 @@ row).  The loss is fp32.
 
 The operators take fp32, bf16 and fp16 CUDA tensors whose last dimension is contiguous or is made so, run on the current
 stream of the tensors' device, take their workspaces from torch's allocator, and can be captured into CUDA graphs.  They
-are differentiable once.
+are differentiable once.  (A captured backward pass belongs in ``torch.autograd.grad``, or to leaves of which no eager graph is
+alive: autograd accumulates into a leaf on the stream of the graph that made its accumulator, which a capture cannot wait for.)
 """
 from __future__ import annotations
 
@@ -68,6 +69,8 @@ def _rows(t):
     """t as [rows, columns] whose rows do not overlap and have their values side by side."""
     if t.dim() != 2:
         t = t.reshape(-1, t.shape[-1])
+    if t.shape[0] > 0x7fffffff or t.shape[1] > 0x7fffffff:
+        raise ValueError(f"sw_gcn: matrices of at most 2^31 - 1 rows and columns, not {tuple(t.shape)}")
     if t.is_contiguous():
         return t
     return t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] else t.contiguous()
