@@ -366,14 +366,9 @@ __global__ void __launch_bounds__(kFewThreads, 1) ce_few_kernel(const CeFewCall 
     constexpr int kMine = (kFewRows + kFewLoaders - 1) / kFewLoaders;  // rows of a warp: eight columns a lane
     const int col = lane * 8;
     using Raw = unsigned[kMine][PLANES * 4];  // rows as they lie in memory
-    auto fetch = [&](Raw &raw, const void *src, long long ld, long long row0, long long rows, const long long *target) {
+    auto fetch = [&](Raw &raw, const void *src, long long ld, long long row0, unsigned wanted) {
       constexpr int BYTES = DT == TF_F32 ? 4 : 2;
       const bool whole = P.cols % 8 == 0 && ld * BYTES % 16 == 0 && (reinterpret_cast<uintptr_t>(src) & 15) == 0;
-      // which of this warp's rows exist and count: lane i asks for the i-th
-      const int mine = lane * kFewLoaders + loader;
-      bool want = lane < kMine && mine < kFewRows && row0 + mine < rows;
-      if (want && target) want = __ldg(target + row0 + mine) != P.ignore;
-      const unsigned wanted = __ballot_sync(kFull, want);
       const char *p = static_cast<const char *>(src) + ((row0 + loader) * ld + col) * BYTES;
 #pragma unroll
       for (int i = 0; i < kMine; ++i, p += kFewLoaders * ld * BYTES) {
@@ -384,8 +379,9 @@ __global__ void __launch_bounds__(kFewThreads, 1) ce_few_kernel(const CeFewCall 
           if (in) {
 #pragma unroll
             for (int k = 0; k < PLANES; ++k) {
-              const uint4 q = __ldg(reinterpret_cast<const uint4 *>(p) + k);
-              raw[i][4 * k] = q.x; raw[i][4 * k + 1] = q.y; raw[i][4 * k + 2] = q.z; raw[i][4 * k + 3] = q.w;
+              // (volatile: issued here, a tile ahead, not where the values are used)
+              asm volatile("ld.global.nc.v4.b32 {%0, %1, %2, %3}, [%4];"
+                           : "=r"(raw[i][4 * k]), "=r"(raw[i][4 * k + 1]), "=r"(raw[i][4 * k + 2]), "=r"(raw[i][4 * k + 3]) : "l"(p + k * 16));
             }
           }
         } else if (DT == TF_F32) {
@@ -452,8 +448,19 @@ __global__ void __launch_bounds__(kFewThreads, 1) ce_few_kernel(const CeFewCall 
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // read next by the tensor core
     };
+    // Which of this warp's rows exist and count: lane i asks for the i-th, a tile before the rows themselves.
+    auto row_of = [&](int t) { return ((long long)blockIdx.x + (long long)t * gridDim.x) * kFewRows; };
+    const int mine = lane * kFewLoaders + loader;
+    bool there = false;
+    long long asked = 0;
+    auto ask = [&](int t) {
+      there = lane < kMine && mine < kFewRows && row_of(t) + mine < P.rows;
+      if (there) asm volatile("ld.global.nc.b64 %0, [%1];" : "=l"(asked) : "l"(P.target + row_of(t) + mine));
+    };
     auto fetch_tile = [&](Raw &raw, int t) {
-      fetch(raw, P.x, P.ld_x, ((long long)blockIdx.x + (long long)t * gridDim.x) * kFewRows, P.rows, P.target);
+      const unsigned wanted = __ballot_sync(kFull, there && asked != P.ignore);
+      fetch(raw, P.x, P.ld_x, row_of(t), wanted);
+      if (t + 1 < tiles) ask(t + 1);
     };
     auto put_tile = [&](const Raw &raw, int t) {
       // (where a wait has run out the waits end at once; no warp leaves, for the others would stay at the barrier in put())
@@ -463,7 +470,8 @@ __global__ void __launch_bounds__(kFewThreads, 1) ce_few_kernel(const CeFewCall 
     };
     Raw raw;
     if (tiles > 0) {
-      fetch(raw, P.w, P.ld_w, 0, P.vocab, nullptr);
+      ask(0);
+      fetch(raw, P.w, P.ld_w, 0, __ballot_sync(kFull, lane < kMine && mine < kFewRows && mine < P.vocab));
       put(raw, at_w, &s.unscale_w);
       few_arrive(&s.w_full);
       fetch_tile(raw, 0);

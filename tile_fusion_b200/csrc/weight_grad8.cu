@@ -254,13 +254,20 @@ __global__ void __launch_bounds__(wg_threads(RING), 1) weight_grad8_kernel(const
       auto gradient = [&](auto whole) {
 #pragma unroll 4
         for (int r = first_g; r < kWgRows; r += step_g) {
-          float g[W];
           const bool here = RING || r < rows;
+          const unsigned to = base + (unsigned)(to_g + r * 128 + ((at_g ^ r) & 7) * 16);
+          if constexpr (std::is_same<T, __nv_bfloat16>::value && decltype(whole)::value) {  // the operand as it lies in memory
+            uint4 q = wg_read<uint4>(pg + (here ? r : 0) * ld);
+            if (!here) q = make_uint4(0, 0, 0, 0);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(q.x), "r"(q.y), "r"(q.z), "r"(q.w));
+            continue;
+          }
+          float g[W];
           wg_load<T, decltype(whole)::value>(pg + (here ? r : 0) * ld, n_g, g);
           if (!here)
 #pragma unroll
             for (int k = 0; k < W; ++k) g[k] = 0.f;
-          wg_planes<PLANES, W>(g, base + (unsigned)(to_g + r * 128 + ((at_g ^ r) & 7) * 16), kPlane);
+          wg_planes<PLANES, W>(g, to, kPlane);
         }
       };
       if (P.whole_g) gradient(std::true_type());
