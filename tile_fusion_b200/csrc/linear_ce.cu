@@ -35,24 +35,28 @@ constexpr float kLn2 = 0.69314718055994531f;
 constexpr float kSlopeUnit = 16384.f;  // of fp16 slopes
 
 struct CeHeader {            // at the start of the workspace, zeroed by every call
-  unsigned top_x, top_w;     // bits of the largest finite |value| (fp32 operands)
   unsigned top_grad;         // bits of the largest finite |gradient of a row's loss|
   int counted;               // rows that count
   int error;                 // a bounded wait ran out
+  int joined;                // blocks whose losses are written
   float unscale_x, unscale_w, unscale_slope;
-  int pad[24];
+  int pad[25];
 };
+constexpr int kCeGrid = 148 * 8;       // blocks of a pass over the operands
+constexpr int kCeFewRows = 8192;       // rows up to which one block does what needs all of them, and a launch less is worth more
 
 struct CeOperand {
   const void *src; long long ld; int rows;
   unsigned short *hi, *lo;   // null: multiplied where they lie
-  unsigned *top; float *unscale;
+  unsigned *tops; float *unscale;  // tops: bits of the largest finite |value| that each block of ce_top_kernel saw (fp32 operands)
   const long long *target;   // rows whose target is `ignore` become zero; null: none
 };
 
-// The largest finite |value| of one operand (blockIdx.y chooses it).  The maximum of their bits does not depend on the order.
-__global__ void __launch_bounds__(256) ce_top_kernel(CeOperand a, CeOperand b, int cols, long long ignore) {
+// The largest finite |value| of one operand (blockIdx.y chooses it) among a block's; `zero`: the header, if this is the first launch of a call.
+__global__ void __launch_bounds__(256) ce_top_kernel(CeOperand a, CeOperand b, int cols, long long ignore, CeHeader *zero) {
+  __shared__ unsigned seen[8];
   const CeOperand o = blockIdx.y ? b : a;
+  if (zero && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x < sizeof(CeHeader) / 4) reinterpret_cast<int *>(zero)[threadIdx.x] = 0;
   const int quads = (cols + 3) / 4;
   const bool whole = cols % 4 == 0 && o.ld % 4 == 0 && (reinterpret_cast<uintptr_t>(o.src) & 15) == 0;
   const long long total = (long long)o.rows * quads, step = (long long)gridDim.x * blockDim.x;
@@ -74,7 +78,12 @@ __global__ void __launch_bounds__(256) ce_top_kernel(CeOperand a, CeOperand b, i
       for (int k = 0; k < 4 && c + k < cols; ++k) see(__ldg(x + k));
   }
   for (int k = 16; k; k >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, k));
-  if ((threadIdx.x & 31) == 0 && top) atomicMax(o.top, top);
+  if ((threadIdx.x & 31) == 0) seen[threadIdx.x >> 5] = top;
+  __syncthreads();
+  if (threadIdx.x) return;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) top = max(top, seen[k]);
+  o.tops[blockIdx.x] = top;
 }
 
 // 2^(14 - floor(log2 top)), at most 2^126
@@ -84,13 +93,21 @@ __device__ __forceinline__ float ce_power(int e) { return __uint_as_float((unsig
 // Planes [rows][ldp] of an operand: fp32 split, 16-bit values copied; zeros from `cols` on and in rows that do not count.
 __global__ void __launch_bounds__(256) ce_planes_kernel(CeOperand a, CeOperand b, int dtype, int cols, int ldp, long long ignore) {
   const CeOperand o = blockIdx.y ? b : a;
-  if (!o.hi) return;
+  if (!o.hi) return;  // (all threads of the block)
   const int eights = ldp / 8;
   const long long total = (long long)o.rows * eights, step = (long long)gridDim.x * blockDim.x;
   const bool whole = cols % 8 == 0 && o.ld * value_bytes(dtype) % 16 == 0 && (reinterpret_cast<uintptr_t>(o.src) & 15) == 0;
   float by = 1.f;
   if (dtype == TF_F32) {
-    const int e = ce_exponent(*o.top);
+    __shared__ unsigned seen[8];
+    unsigned top = 0;
+    for (int i = threadIdx.x; i < gridDim.x; i += blockDim.x) top = max(top, o.tops[i]);
+    for (int k = 16; k; k >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, k));
+    if ((threadIdx.x & 31) == 0) seen[threadIdx.x >> 5] = top;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 8; ++k) top = max(top, seen[k]);
+    const int e = ce_exponent(top);
     by = ce_power(max(e, -126));  // (e is at least -113)
     if (blockIdx.x == 0 && threadIdx.x == 0) *o.unscale = ce_power(-e);
   }
@@ -135,8 +152,8 @@ __global__ void __launch_bounds__(256) ce_planes_kernel(CeOperand a, CeOperand b
 // Joins a row's parts: lse2 = log2 sum exp, and the row's loss.  Eight threads to a row, 32 rows to a block.
 __global__ void __launch_bounds__(256) ce_join_kernel(const float2 *__restrict__ sums, int parts, int rows, const float *__restrict__ target_logit,
                                                       const long long *__restrict__ target, long long ignore, int vocab, float *__restrict__ lse2,
-                                                      float *__restrict__ row_loss, double *__restrict__ block_loss, int *__restrict__ block_count,
-                                                      const CeHeader *h) {
+                                                      float *__restrict__ row_loss, double *block_loss, int *block_count, CeHeader *h, int mean,
+                                                      float *total) {
   __shared__ float2 part[8][32];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, row = blockIdx.x * 32 + lane;
   float m = -INFINITY, s = 0.f;
@@ -173,6 +190,26 @@ __global__ void __launch_bounds__(256) ce_join_kernel(const float2 *__restrict__
     counts += __shfl_xor_sync(0xffffffffu, counts, k);
   }
   if (lane == 0) { block_loss[blockIdx.x] = loss; block_count[blockIdx.x] = counts; }
+  if (!total) return;
+  // few blocks: the last one adds them up, in their order
+  int last = 0;
+  if (lane == 0) {
+    __threadfence();
+    last = atomicAdd(&h->joined, 1) == (int)gridDim.x - 1;
+  }
+  if (!__shfl_sync(0xffffffffu, last, 0)) return;
+  __threadfence();
+  loss = 0.;
+  counts = 0;
+  for (int i = lane; i < (int)gridDim.x; i += 32) {
+    loss += *reinterpret_cast<volatile double *>(block_loss + i);
+    counts += *reinterpret_cast<volatile int *>(block_count + i);
+  }
+  for (int k = 16; k; k >>= 1) {
+    loss += __shfl_xor_sync(0xffffffffu, loss, k);
+    counts += __shfl_xor_sync(0xffffffffu, counts, k);
+  }
+  if (lane == 0) *total = (float)(mean ? loss / max(counts, 1) : loss);
 }
 
 // The blocks' losses in a fixed order, in 64 bits.
@@ -214,23 +251,54 @@ __global__ void __launch_bounds__(256) ce_count_kernel(const long long *__restri
   }
 }
 
-// row_scale: what a row's slope is multiplied by before it is rounded; unscale_slope: what the sums of slopes are multiplied by.
-// reduction 0: a gradient to each row, brought to at most one by a power of two; 1, 2: one gradient, which the sums take.
-__global__ void __launch_bounds__(256) ce_scale_kernel(const long long *__restrict__ target, const float *__restrict__ grad, int rows, long long ignore,
-                                                       int vocab, int reduction, float unit, float *__restrict__ row_scale, CeHeader *h) {
+// What a row's slope is multiplied by before it is rounded, and what the sums of slopes are multiplied by.  reduction 0: a gradient to
+// each row, brought to at most one by a power of two; 1, 2: one gradient, which the sums take.
+__device__ __forceinline__ float2 ce_scales(int reduction, float unit, unsigned top_grad, int counted, const float *grad) {
   float by = unit, back = 1.f / unit;
   if (reduction == 0) {
-    const int e = h->top_grad ? min(126, max(-126, -((int)(h->top_grad >> 23) - 126))) : 0;
+    const int e = top_grad ? min(126, max(-126, -((int)(top_grad >> 23) - 126))) : 0;
     by *= ce_power(e);
     back *= ce_power(-e);
-  } else back *= grad[0] / (reduction == 1 ? (float)max(h->counted, 1) : 1.f);
+  } else back *= grad[0] / (reduction == 1 ? (float)max(counted, 1) : 1.f);
+  return make_float2(by, back);
+}
+__device__ __forceinline__ float ce_row_scale(long long t, long long ignore, int vocab, int reduction, const float *grad, int i, float by) {
+  if (t == ignore) return 0.f;
+  return t < 0 || t >= vocab ? __int_as_float(0x7fc00000) : reduction == 0 ? grad[i] * by : by;
+}
+__global__ void __launch_bounds__(256) ce_scale_kernel(const long long *__restrict__ target, const float *__restrict__ grad, int rows, long long ignore,
+                                                       int vocab, int reduction, float unit, float *__restrict__ row_scale, CeHeader *h) {
+  const float2 scale = ce_scales(reduction, unit, h->top_grad, h->counted, grad);
   const int i = blockIdx.x * blockDim.x + threadIdx.x;
-  if (i == 0) h->unscale_slope = back;
-  if (i >= rows) return;
-  const long long t = target[i];
-  float v = t == ignore ? 0.f : reduction == 0 ? grad[i] * by : by;
-  if (t != ignore && (t < 0 || t >= vocab)) v = __int_as_float(0x7fc00000);
-  row_scale[i] = v;
+  if (i == 0) h->unscale_slope = scale.y;
+  if (i < rows) row_scale[i] = ce_row_scale(target[i], ignore, vocab, reduction, grad, i, scale.x);
+}
+
+// Both of these in one block, behind the zeroed header.
+__global__ void __launch_bounds__(1024) ce_prepare_kernel(const long long *__restrict__ target, const float *__restrict__ grad, int rows, long long ignore,
+                                                          int vocab, int reduction, float unit, float *__restrict__ row_scale, CeHeader *h) {
+  __shared__ int cs[32];
+  __shared__ unsigned ts[32];
+  if (threadIdx.x < sizeof(CeHeader) / 4) reinterpret_cast<int *>(h)[threadIdx.x] = 0;
+  int c = 0;
+  unsigned top = 0;
+  for (int i = threadIdx.x; i < rows; i += 1024) {
+    if (target[i] == ignore) continue;
+    ++c;
+    if (reduction == 0) {
+      const unsigned u = __float_as_uint(grad[i]) & 0x7fffffffu;
+      if (u < 0x7f800000u) top = max(top, u);
+    }
+  }
+  for (int k = 16; k; k >>= 1) { c += __shfl_xor_sync(0xffffffffu, c, k); top = max(top, __shfl_xor_sync(0xffffffffu, top, k)); }
+  if ((threadIdx.x & 31) == 0) { cs[threadIdx.x >> 5] = c; ts[threadIdx.x >> 5] = top; }
+  __syncthreads();
+  c = 0;
+  top = 0;
+  for (int k = 0; k < 32; ++k) { c += cs[k]; top = max(top, ts[k]); }
+  const float2 scale = ce_scales(reduction, unit, top, c, grad);
+  if (threadIdx.x == 0) h->unscale_slope = scale.y;
+  for (int i = threadIdx.x; i < rows; i += 1024) row_scale[i] = ce_row_scale(target[i], ignore, vocab, reduction, grad, i, scale.x);
 }
 
 // out = (part[0] + part[1] + ...) * scales, parts [splits][rows][ld]
@@ -276,6 +344,7 @@ long long up(long long v, long long to) { return (v + to - 1) / to * to; }
 // What the workspace holds, for the sizes of a call; `base` null: sizes only.
 struct CeSpace {
   CeHeader *h;
+  unsigned *tops = nullptr;  // [2][kCeGrid]
   unsigned short *x_hi = nullptr, *x_lo = nullptr, *w_hi = nullptr, *w_lo = nullptr;
   float2 *sums = nullptr; float *target_logit = nullptr; double *block_loss = nullptr; int *block_count = nullptr;
   float *row_scale = nullptr; unsigned short *slope_hi = nullptr, *slope_lo = nullptr; float *parts_x = nullptr, *parts_w = nullptr;
@@ -323,6 +392,7 @@ CeSpace ce_space(char *base, int rows, int cols, int vocab, int dtype, bool back
     return s;
   }
   s.ldp = (int)up(cols, 8);
+  if (f32) s.tops = (unsigned *)take(8ll * kCeGrid);
   s.copy_x = f32 || backward || !whole_x;
   s.copy_w = f32 || !whole_w;
   if (s.copy_x) s.x_hi = (unsigned short *)take(2ll * rows * s.ldp);
@@ -388,13 +458,13 @@ CeFewCall few_call(const CeSpace &sp, const void *x, long long ld_x, const void 
 
 // Planes of both operands, where they are not multiplied as they lie.
 cudaError_t ce_planes(const CeSpace &sp, const void *x, long long ld_x, const void *w, long long ld_w, int dtype, int rows, int cols, int vocab,
-                      const long long *target, long long ignore, cudaStream_t s) {
-  CeOperand ox = {x, ld_x, rows, sp.x_hi, sp.x_lo, &sp.h->top_x, &sp.h->unscale_x, target};
-  CeOperand ow = {w, ld_w, vocab, sp.w_hi, sp.w_lo, &sp.h->top_w, &sp.h->unscale_w, nullptr};
+                      const long long *target, long long ignore, CeHeader *zero, cudaStream_t s) {
+  CeOperand ox = {x, ld_x, rows, sp.x_hi, sp.x_lo, sp.tops, &sp.h->unscale_x, target};
+  CeOperand ow = {w, ld_w, vocab, sp.w_hi, sp.w_lo, sp.tops + kCeGrid, &sp.h->unscale_w, nullptr};
   if (!sp.copy_x && !sp.copy_w) return cudaSuccess;
   const long long most = (long long)std::max(sp.copy_x ? rows : 0, sp.copy_w ? vocab : 0) * sp.ldp / 8;
-  const dim3 grid((unsigned)std::min<long long>((most + 255) / 256, 148 * 8), 2);
-  if (dtype == TF_F32) ce_top_kernel<<<grid, 256, 0, s>>>(ox, ow, cols, ignore);
+  const dim3 grid((unsigned)std::min<long long>((most + 255) / 256, kCeGrid), 2);
+  if (dtype == TF_F32) ce_top_kernel<<<grid, 256, 0, s>>>(ox, ow, cols, ignore, zero);
   ce_planes_kernel<<<grid, 256, 0, s>>>(ox, ow, dtype, cols, sp.ldp, ignore);
   return cudaGetLastError();
 }
@@ -425,7 +495,9 @@ extern "C" int tf_linear_ce_fwd(const void *x, long long ld_x, const void *w, lo
     return e == cudaSuccess ? TF_OK : ce_fail(who, e);
   }
   const CeSpace sp = ce_space((char *)work, rows, cols, vocab, dtype, false, ce_whole(x, ld_x, dtype), ce_whole(w, ld_w, dtype));
-  cudaError_t e = cudaMemsetAsync(sp.h, 0, sizeof(CeHeader), s);
+  // (fp32: the first pass over the operands zeroes the header)
+  const bool zeroes = dtype == TF_F32 && !sp.few;
+  cudaError_t e = zeroes ? cudaSuccess : cudaMemsetAsync(sp.h, 0, sizeof(CeHeader), s);
   if (sp.few) {
     CeFewCall c = few_call(sp, x, ld_x, w, ld_w, dtype, target, rows, cols, vocab, ignore_index);
     c.lse2 = lse2;
@@ -438,7 +510,7 @@ extern "C" int tf_linear_ce_fwd(const void *x, long long ld_x, const void *w, lo
     }
     return e == cudaSuccess ? TF_OK : ce_fail(who, e);
   }
-  if (e == cudaSuccess) e = ce_planes(sp, x, ld_x, w, ld_w, dtype, rows, cols, vocab, target, ignore_index, s);
+  if (e == cudaSuccess) e = ce_planes(sp, x, ld_x, w, ld_w, dtype, rows, cols, vocab, target, ignore_index, zeroes ? sp.h : nullptr, s);
   if (e != cudaSuccess) return ce_fail(who, e);
   const bool f32 = dtype == TF_F32;
   PlaneGemmCall c;
@@ -455,8 +527,9 @@ extern "C" int tf_linear_ce_fwd(const void *x, long long ld_x, const void *w, lo
   if (rc != TF_OK) return rc;
   const int blocks = (rows + 31) / 32;
   ce_join_kernel<<<blocks, 256, 0, s>>>(sp.sums, plane_gemm_parts(rows, vocab), rows, sp.target_logit, target, ignore_index, vocab, lse2,
-                                        reduction ? nullptr : loss, reduction ? sp.block_loss : nullptr, sp.block_count, sp.h);
-  if (reduction) ce_total_kernel<<<1, 1024, 0, s>>>(sp.block_loss, sp.block_count, blocks, reduction == 1, loss);
+                                        reduction ? nullptr : loss, reduction ? sp.block_loss : nullptr, sp.block_count, sp.h, reduction == 1,
+                                        reduction && rows <= kCeFewRows ? loss : nullptr);
+  if (reduction && rows > kCeFewRows) ce_total_kernel<<<1, 1024, 0, s>>>(sp.block_loss, sp.block_count, blocks, reduction == 1, loss);
   e = cudaGetLastError();
   return e == cudaSuccess ? TF_OK : ce_fail(who, e);
 }
@@ -477,12 +550,17 @@ extern "C" int tf_linear_ce_bwd(const void *x, long long ld_x, const void *w, lo
   if (!dx && !dw) return TF_OK;
   const CeSpace sp = ce_space((char *)work, rows, cols, vocab, dtype, true, ce_whole(x, ld_x, dtype), ce_whole(w, ld_w, dtype));
   const bool f32 = dtype == TF_F32;
-  cudaError_t e = cudaMemsetAsync(sp.h, 0, sizeof(CeHeader), s);
-  if (e != cudaSuccess) return ce_fail(who, e);
-  if (reduction != 2)
-    ce_count_kernel<<<std::min((rows + 255) / 256, 148 * 4), 256, 0, s>>>(target, reduction ? nullptr : grad, rows, ignore_index, sp.h);
-  ce_scale_kernel<<<(rows + 255) / 256, 256, 0, s>>>(target, grad, rows, ignore_index, vocab, reduction, dtype == TF_BF16 ? 1.f : kSlopeUnit,
-                                                     sp.row_scale, sp.h);
+  const float unit = dtype == TF_BF16 ? 1.f : kSlopeUnit;
+  cudaError_t e = cudaSuccess;
+  if (rows <= kCeFewRows)
+    ce_prepare_kernel<<<1, 1024, 0, s>>>(target, grad, rows, ignore_index, vocab, reduction, unit, sp.row_scale, sp.h);
+  else {
+    e = cudaMemsetAsync(sp.h, 0, sizeof(CeHeader), s);
+    if (e != cudaSuccess) return ce_fail(who, e);
+    if (reduction != 2)
+      ce_count_kernel<<<std::min((rows + 255) / 256, 148 * 4), 256, 0, s>>>(target, reduction ? nullptr : grad, rows, ignore_index, sp.h);
+    ce_scale_kernel<<<(rows + 255) / 256, 256, 0, s>>>(target, grad, rows, ignore_index, vocab, reduction, unit, sp.row_scale, sp.h);
+  }
   if (sp.few) {
     CeFewCall c = few_call(sp, x, ld_x, w, ld_w, dtype, target, rows, cols, vocab, ignore_index);
     c.lse2 = const_cast<float *>(lse2);
@@ -495,7 +573,7 @@ extern "C" int tf_linear_ce_bwd(const void *x, long long ld_x, const void *w, lo
     }
     return e == cudaSuccess ? TF_OK : ce_fail(who, e);
   }
-  e = ce_planes(sp, x, ld_x, w, ld_w, dtype, rows, cols, vocab, target, ignore_index, s);
+  e = ce_planes(sp, x, ld_x, w, ld_w, dtype, rows, cols, vocab, target, ignore_index, nullptr, s);
   if (e != cudaSuccess) return ce_fail(who, e);
   const int sms = sm_count();
   const long long ld_sum = up(cols, 4), ld_w16 = sp.copy_w ? sp.ldp : ld_w;
