@@ -3,11 +3,11 @@
 //
 //   * The rows are cut into as many ranges as the device holds CTAs; each adds up a tile of 128 x 256 or 256 x 128 sums (which of
 //     the two: whatever reads less), and a second launch adds the ranges' tiles in order.
-//   * Four teams of four warps each turn 16 rows at a time into 16-bit operands in shared memory, row by row as they lie (MN-major,
+//   * Four teams of four warps (six for gradients in 16 bits) each turn 16 rows at a time into 16-bit operands in shared memory, row by row as they lie (MN-major,
 //     128-byte swizzle: nothing is transposed), while further rows are on their way; one warp issues tcgen05.mma.  (All warps on the
 //     same 32 rows wait for one another in every step: 500 009 rows, 47 x 256 bf16: 127 us.)  A value of X is seven bits and a power of two, exact in bf16.  G in fp32 is three bf16 planes (24 bits, exact), in
 //     fp16 two (exact), in bf16 one.  So products lose nothing.
-//   * The tensor core cuts off what it adds to an accumulator, 2e-8 of the sum each time: after 128 rows (at most 24 additions)
+//   * The tensor core cuts off what it adds to an accumulator, 2e-8 of the sum each time: for fp32 after 128 rows (24 additions)
 //     the accumulator, one of two, is read and added in registers, where sums round.
 // All waits are bounded: where one runs out the CTA's sums, and with them the result, become NaN.
 #include <algorithm>
@@ -22,18 +22,21 @@ namespace tfk {
 
 namespace {
 
-constexpr int kWgWarps = 16;
-__host__ __device__ constexpr int wg_threads(bool ring) { return 32 * (kWgWarps + (ring ? 2 : 1)); }
-constexpr int kWgTeams = 4, kWgTeam = 32 * kWgWarps / kWgTeams;  // teams of four warps, threads of one
+// Teams of four warps.  Gradients in 16 bits (one or two planes) leave their sums in tensor memory to the end: 2e-8 of the sum for each
+// of at most a few thousand additions is far below the 2^-9 or 2^-12 that the result is rounded to, and warps that hold no sums
+// are small enough for six teams.
+constexpr int kWgTeam = 128, kWgMaxTeams = 6;
+__host__ __device__ constexpr int wg_teams(int planes) { return planes == 3 ? 4 : 6; }
+__host__ __device__ constexpr int wg_threads(int planes, bool ring) { return kWgTeam * wg_teams(planes) + 32 * (ring ? 2 : 1); }
 constexpr int kWgRows = 16;                    // of a slice: a K step
-constexpr int kWgChain = 8;                    // slices added up in tensor memory, a multiple of the teams
+constexpr int kWgChain = 8;                    // (fp32) slices added up in tensor memory, a multiple of the teams
 constexpr int kWgBlock = kWgRows * 128;        // bytes of 64 columns of a slice
 constexpr int kWgMaxRing = 16;
 constexpr int kWgSmem = 224 * 1024;
 constexpr int kWgWaitLimit = 1 << 22;
 
 __host__ __device__ constexpr int wg_stage_bytes(int planes, int mt) { return planes * mt * 2 * kWgBlock + (mt == 1 ? 4 : 2) * kWgBlock; }
-static_assert(kWgTeams * wg_stage_bytes(3, 2) <= kWgSmem, "a stage to each team");
+static_assert(wg_teams(3) * wg_stage_bytes(3, 2) <= kWgSmem && wg_teams(2) * wg_stage_bytes(2, 2) <= kWgSmem, "a stage to each team");
 
 struct WgParams {
   const void *g; long long ld_g; int na;
@@ -46,7 +49,7 @@ struct WgParams {
 
 struct WgShared {
   unsigned long long raw_full[kWgMaxRing], raw_empty[kWgMaxRing];
-  unsigned long long full[kWgTeams], empty[kWgTeams], acc_full[2], acc_empty[2];
+  unsigned long long full[kWgMaxTeams], empty[kWgMaxTeams], acc_full[2], acc_empty[2];
   unsigned tmem_base;
   int dead;
 };
@@ -125,8 +128,10 @@ template <int PLANES, int W> __device__ __forceinline__ void wg_planes(float (&g
 // (Whole rows, of which a tile may use a part: 528 846 rows, 191 x 224 bf16.)  Else (strided rows, or a ring that does not fit four
 // slices) the teams read rows from memory themselves.
 template <class T, int PLANES, int MT, bool RING>
-__global__ void __launch_bounds__(wg_threads(RING), 1) weight_grad8_kernel(const WgParams P) {
+__global__ void __launch_bounds__(wg_threads(PLANES, RING), 1) weight_grad8_kernel(const WgParams P) {
   constexpr int NT = MT == 1 ? 256 : 128, kPlane = MT * 2 * kWgBlock, kStage = wg_stage_bytes(PLANES, MT);
+  constexpr int kTeams = wg_teams(PLANES), kWarps = 4 * kTeams, kTeamWarps = kWgTeam / 32;
+  constexpr bool STAY = PLANES < 3;  // sums stay in tensor memory
   constexpr int W = 16 / sizeof(T);  // values of G that a thread takes at a time; of X eight
   extern __shared__ char dyn[];
   __shared__ WgShared s;
@@ -139,13 +144,13 @@ __global__ void __launch_bounds__(wg_threads(RING), 1) weight_grad8_kernel(const
   const int slices = (int)((r1 - r0 + kWgRows - 1) / kWgRows);
 
   // columns beyond the operands' stay zero
-  for (int i = tid; i < kWgTeams * kStage / 16; i += wg_threads(RING)) reinterpret_cast<uint4 *>(smem)[i] = make_uint4(0, 0, 0, 0);
+  for (int i = tid; i < kTeams * kStage / 16; i += wg_threads(PLANES, RING)) reinterpret_cast<uint4 *>(smem)[i] = make_uint4(0, 0, 0, 0);
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   if (tid == 0) {
-    for (int i = 0; i < kWgTeams; ++i) { mbar_init(&s.full[i], kWgWarps / kWgTeams); mbar_init(&s.empty[i], 1); }
+    for (int i = 0; i < kTeams; ++i) { mbar_init(&s.full[i], kTeamWarps); mbar_init(&s.empty[i], 1); }
     if (RING)
-      for (int i = 0; i < P.ring; ++i) { mbar_init(&s.raw_full[i], 1); mbar_init(&s.raw_empty[i], kWgWarps / kWgTeams); }
-    for (int i = 0; i < 2; ++i) { mbar_init(&s.acc_full[i], 1); mbar_init(&s.acc_empty[i], kWgWarps); }
+      for (int i = 0; i < P.ring; ++i) { mbar_init(&s.raw_full[i], 1); mbar_init(&s.raw_empty[i], kTeamWarps); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&s.acc_full[i], 1); mbar_init(&s.acc_empty[i], kWarps); }
     s.dead = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -158,8 +163,8 @@ __global__ void __launch_bounds__(wg_threads(RING), 1) weight_grad8_kernel(const
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 
   const int whole = RING ? (int)((r1 - r0) / kWgRows) : 0;  // slices of the ring: those with all their rows
-  char *raw = smem + kWgTeams * kStage;
-  if (RING && warp == kWgWarps + 1) {
+  char *raw = smem + kTeams * kStage;
+  if (RING && warp == kWarps + 1) {
     // ---- copies ----
     int rs = 0, issued = 0;
     unsigned ph = 0;
@@ -186,21 +191,21 @@ __global__ void __launch_bounds__(wg_threads(RING), 1) weight_grad8_kernel(const
     if (!ok || s.dead)
       for (int i = 0; i < issued; ++i)
         for (int k = 0; k < kWgWaitLimit && !mbar_wait(&s.raw_full[i], i < rs ? ph : ph ^ 1u, 1); ++k) {}
-  } else if (warp == kWgWarps) {
+  } else if (warp == kWarps) {
     // ---- products ----
     const unsigned idesc = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (1u << 16) | ((unsigned)(n_pad >> 3) << 17) | ((unsigned)(128 >> 4) << 24);
     bool ok = true;
     auto wait = [&](unsigned long long *bar, unsigned parity) { return ok = __all_sync(kFull, pair_wait(bar, parity, s.dead, kWgWaitLimit)); };
     for (int sl = 0; sl < slices; ++sl) {
-      const int st = sl % kWgTeams;
-      const int chain = sl / kWgChain, buf = chain & 1, in = sl % kWgChain;
-      if (in == 0 && chain >= 2 && !wait(&s.acc_empty[buf], (unsigned)(chain / 2 - 1) & 1u)) break;
-      if (!wait(&s.full[st], (unsigned)(sl / kWgTeams) & 1u)) break;
+      const int st = sl % kTeams;
+      const int chain = STAY ? 0 : sl / kWgChain, buf = chain & 1, in = STAY ? sl : sl % kWgChain;
+      if (!STAY && in == 0 && chain >= 2 && !wait(&s.acc_empty[buf], (unsigned)(chain / 2 - 1) & 1u)) break;
+      if (!wait(&s.full[st], (unsigned)(sl / kTeams) & 1u)) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const unsigned base = smem_u32(smem + st * kStage);
       const unsigned long long a = wg_desc(base), b = wg_desc(base + PLANES * kPlane);
       const unsigned d = s.tmem_base + (unsigned)(buf * 256);
-      const bool last = in == kWgChain - 1 || sl == slices - 1;
+      const bool last = (!STAY && in == kWgChain - 1) || sl == slices - 1;
       if (elect_one()) {
 #pragma unroll
         for (int p = PLANES - 1; p >= 0; --p)  // the small products first
@@ -213,12 +218,13 @@ __global__ void __launch_bounds__(wg_threads(RING), 1) weight_grad8_kernel(const
       __syncwarp();
     }
   } else {
-    // ---- rows into operands, every fourth slice to a team; and the sums of the chain before out of tensor memory ----
-    const int team = warp / (kWgWarps / kWgTeams), in_team = tid % kWgTeam;
+    // ---- rows into operands, each team every so many slices; and (fp32) the sums of the chain before out of tensor memory ----
+    const int team = warp / kTeamWarps, in_team = tid % kWgTeam;
     const int quadrant = warp & 3, cols0 = (warp >> 2) * 64;  // this thread's row and columns of the accumulator
-    float acc[64];
+    float acc[STAY ? 1 : 64];
+    if (!STAY)
 #pragma unroll
-    for (int i = 0; i < 64; ++i) acc[i] = 0.f;
+      for (int i = 0; i < 64; ++i) acc[STAY ? 0 : i] = 0.f;
     bool ok = true;
     auto wait = [&](unsigned long long *bar, unsigned parity) { return ok = __all_sync(kFull, pair_wait(bar, parity, s.dead, kWgWaitLimit)); };
     auto drain = [&](int chain) {
@@ -231,7 +237,7 @@ __global__ void __launch_bounds__(wg_threads(RING), 1) weight_grad8_kernel(const
           float v[16];
           tmem_load16(v, s.tmem_base + ((unsigned)(quadrant * 32) << 16) + (unsigned)(buf * 256 + cols0 + c));
 #pragma unroll
-          for (int q = 0; q < 16; ++q) acc[c + q] += v[q];
+          for (int q = 0; q < 16; ++q) acc[STAY ? 0 : c + q] += v[q];
         }
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -299,7 +305,7 @@ __global__ void __launch_bounds__(wg_threads(RING), 1) weight_grad8_kernel(const
     int drained = 0, turn = 0, rs = team;
     unsigned raw_ph = 0;
     const unsigned stage = smem_u32(smem + team * kStage);
-    for (int sl = team; sl < slices && ok; sl += kWgTeams, ++turn) {
+    for (int sl = team; sl < slices && ok; sl += kTeams, ++turn) {
       if (turn && !wait(&s.empty[team], (unsigned)(turn - 1) & 1u)) break;
       const long long row = r0 + (long long)sl * kWgRows;
       if constexpr (RING) {
@@ -319,7 +325,7 @@ __global__ void __launch_bounds__(wg_threads(RING), 1) weight_grad8_kernel(const
         const unsigned place = ring_place(smem_u32(at));
         convert(stage, place, (unsigned)(P.na * sizeof(T)), place + P.g_bytes, place + P.g_bytes + kWgRows * P.ld_codes, kWgRows);
         arrive(&s.raw_empty[rs]);
-        if ((rs += kWgTeams) >= P.ring) { rs = team; raw_ph ^= 1u; }
+        if ((rs += kTeams) >= P.ring) { rs = team; raw_ph ^= 1u; }
       } else
         convert(stage, static_cast<const char *>(P.g) + row * P.ld_g * (long long)sizeof(T), P.ld_g * (long long)sizeof(T),
                 reinterpret_cast<const char *>(P.codes) + row * P.ld_codes, reinterpret_cast<const char *>(P.exps) + row * ld_e,
@@ -327,23 +333,36 @@ __global__ void __launch_bounds__(wg_threads(RING), 1) weight_grad8_kernel(const
       arrive(&s.full[team]);
       // this team's last slice of a chain: the chain before has been computed, or is about to be
       const int chain = sl / kWgChain;
-      if (sl % kWgChain >= kWgChain - kWgTeams && chain >= 1) { drain(chain - 1); ++drained; }
+      if (!STAY && sl % kWgChain >= kWgChain - kTeams && chain >= 1) { drain(chain - 1); ++drained; }
     }
-    while (ok && drained < chains) drain(drained++);
+    while (!STAY && ok && drained < chains) drain(drained++);
+    if (STAY && wait(&s.acc_full[0], 0)) asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const int t = MT == 2 ? cols0 / 128 : 0, col = b0 + (MT == 2 ? cols0 % 128 : cols0), row = a0 + t * 128 + quadrant * 32 + lane;
-    const bool lost = !ok || *reinterpret_cast<volatile int *>(&s.dead);
-    if (row < P.na) {
-      float *to = P.part + ((size_t)blockIdx.x * P.na + row) * P.nb + col;
-      const bool quads = P.nb % 4 == 0;
+    const bool lost = __any_sync(kFull, !ok || *reinterpret_cast<volatile int *>(&s.dead));
+    float *to = P.part + ((size_t)blockIdx.x * P.na + row) * P.nb + col;
+    const bool quads = P.nb % 4 == 0;
+    if (cols0 < 256) {  // (six teams: the first four have a part of the sums each)
 #pragma unroll
-      for (int c = 0; c < 64; c += 4) {
-        if (lost) acc[c] = acc[c + 1] = acc[c + 2] = acc[c + 3] = __int_as_float(0x7fc00000);
-        if (quads && col + c < P.nb) *reinterpret_cast<float4 *>(to + c) = make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
-        else {
+      for (int c = 0; c < 64; c += 16) {
+        float v[16];
+        if (STAY) {
+          if (!lost && (MT == 2 ? (cols0 & 127) < n_pad : cols0 < n_pad)) tmem_load16(v, s.tmem_base + ((unsigned)(quadrant * 32) << 16) + (unsigned)(cols0 + c));
+        } else
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (col + c + k < P.nb) to[c + k] = acc[c + k];
+          for (int q = 0; q < 16; ++q) v[q] = acc[STAY ? 0 : c + q];
+        if (row < P.na) {
+#pragma unroll
+          for (int k = 0; k < 16; k += 4) {
+            if (lost) v[k] = v[k + 1] = v[k + 2] = v[k + 3] = __int_as_float(0x7fc00000);
+            if (quads && col + c + k < P.nb) *reinterpret_cast<float4 *>(to + c + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+            else {
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+                if (col + c + k + q < P.nb) to[c + k + q] = v[k + q];
+            }
+          }
         }
+        __syncwarp();
       }
     }
   }
@@ -396,10 +415,10 @@ WgPlan wg_plan(int m, int na, int nb, int dtype) {
 
 template <class T, int PLANES, int MT, bool RING> cudaError_t wg_launch(const WgPlan &p, const WgParams &P, cudaStream_t s) {
   auto f = weight_grad8_kernel<T, PLANES, MT, RING>;
-  const int smem = kWgTeams * wg_stage_bytes(PLANES, MT) + P.ring * P.ring_bytes + 1024;
+  const int smem = wg_teams(PLANES) * wg_stage_bytes(PLANES, MT) + P.ring * P.ring_bytes + 1024;
   const cudaError_t e = cudaFuncSetAttribute((const void *)f, cudaFuncAttributeMaxDynamicSharedMemorySize, kWgSmem + 2048);
   if (e != cudaSuccess) return e;
-  f<<<dim3(p.parts, p.tiles_a, p.tiles_b), wg_threads(RING), smem, s>>>(P);
+  f<<<dim3(p.parts, p.tiles_a, p.tiles_b), wg_threads(PLANES, RING), smem, s>>>(P);
   return cudaGetLastError();
 }
 template <class T, int PLANES> cudaError_t wg_run(const WgPlan &p, WgParams P, cudaStream_t s) {
@@ -408,7 +427,7 @@ template <class T, int PLANES> cudaError_t wg_run(const WgPlan &p, WgParams P, c
   P.g_bytes = kWgRows * P.na * (int)sizeof(T);
   P.ring_bytes = P.g_bytes + kWgRows * P.ld_codes + kWgRows * P.ld_codes / kPackGroup;
   if (P.ld_g == P.na && whole(P.g) && whole(P.exps))
-    P.ring = std::min(kWgMaxRing, (kWgSmem - kWgTeams * wg_stage_bytes(PLANES, p.mt)) / P.ring_bytes) / kWgTeams * kWgTeams;
+    P.ring = std::min(kWgMaxRing, (kWgSmem - wg_teams(PLANES) * wg_stage_bytes(PLANES, p.mt)) / P.ring_bytes) / wg_teams(PLANES) * wg_teams(PLANES);
   if (P.ring > 0) return p.mt == 1 ? wg_launch<T, PLANES, 1, true>(p, P, s) : wg_launch<T, PLANES, 2, true>(p, P, s);
   P.ring = 0;
   return p.mt == 1 ? wg_launch<T, PLANES, 1, false>(p, P, s) : wg_launch<T, PLANES, 2, false>(p, P, s);
