@@ -83,3 +83,11 @@ def test_linear_ce(L):
     # the slope of a large vocabulary is held in pieces: 8 192 rows of 128 000 classes in bf16 are 2 GB, a piece 256 MB
     big = L.tf_linear_ce_work_bytes(8192, 4096, 128_000, 1, 1)
     assert C.c_longlong(big).value < 8192 * 128_000 * 2 / 2 + 3 * 128_000 * 4096
+
+
+def test_weight_grad8_of_a_very_long_side(L):
+    """A side of more than 2^20 would overflow a slice's count of bytes and the grid."""
+    grad = lambda **k: L.tf_weight_grad8(*{**dict(g=P, ld=8, t=0, na=8, c=P, ldc=64, e=P, nb=40, m=4, out=P, work=P, wn=1 << 40, s=None), **k}.values())  # noqa: E731
+    refused(grad(na=1 << 26, ld=1 << 26, nb=1, ldc=32), "side")
+    refused(grad(na=(1 << 20) + 1, ld=(1 << 20) + 1, nb=1, ldc=32), "side")
+    refused(grad(na=1, ld=1, nb=(1 << 20) + 1, ldc=(1 << 20) + 32), "side")

@@ -449,7 +449,9 @@ extern "C" int tf_weight_grad8(const void *g, long long ld_g, int dtype, int na,
   auto bad = [&](const char *what) { return tf::fail(TF_ERR_ARG, std::string("tf_weight_grad8: ") + what); };
   if (!known_dtype(dtype)) return bad("unknown type");
   if (m < 0 || na <= 0 || nb <= 0) return bad("bad size");
-  if ((long long)na * nb > (1 << 26)) return tf::fail(TF_ERR_UNSUPPORTED, "tf_weight_grad8: at most 2^26 entries");
+  // (the tiles of a side are a dimension of the grid, 65 535 at most, and a slice's bytes are counted in 32 bits)
+  if ((long long)na * nb > (1 << 26) || na > (1 << 20) || nb > (1 << 20))
+    return tf::fail(TF_ERR_UNSUPPORTED, "tf_weight_grad8: at most 2^26 entries, 2^20 to a side");
   if (!out || !work || (m > 0 && (!g || !codes || !exponents))) return bad("null argument");
   if (ld_g < na || ld_codes < nb) return bad("rows overlap");
   if (ld_codes % kPackGroup != 0 || (reinterpret_cast<uintptr_t>(codes) & 31) != 0) return bad("codes need rows of whole groups of 32 and 32-byte alignment");
