@@ -91,3 +91,15 @@ def test_weight_grad8_of_a_very_long_side(L):
     refused(grad(na=1 << 26, ld=1 << 26, nb=1, ldc=32), "side")
     refused(grad(na=(1 << 20) + 1, ld=(1 << 20) + 1, nb=1, ldc=32), "side")
     refused(grad(na=1, ld=1, nb=(1 << 20) + 1, ldc=(1 << 20) + 32), "side")
+
+
+def test_rows_next_to_2_31(L):
+    """A row's index and a step of the grid beyond it must fit 32 bits."""
+    n = 0x7f000001
+    refused(L.tf_layer_norm_fwd(P, 8, 0, None, None, 0, n, 8, 1e-5, P, 8, None, None, None, 0, None, None), "size")
+    refused(L.tf_layer_norm_bwd(P, 8, None, 0, None, 0, None, 0, n, 8, P, P, P, 8, P, 8, None, None, None, 0, None), "size")
+    refused(L.tf_pack8(P, 8, 0, n, 8, 0, P, 32, P, None), "size")
+    refused(L.tf_weight_grad8(P, 8, 0, 8, P, 32, P, 8, n, P, P, 1 << 40, None), "size")
+    refused(L.tf_linear_ce_fwd(P, 8, P, 8, 0, P, n, 8, 5, -100, 1, P, P, P, 1 << 40, None), "size")
+    refused(L.tf_linear_ce_fwd(P, 8, P, 8, 0, P, 4, 8, n, -100, 1, P, P, P, 1 << 40, None), "size")
+    assert L.tf_linear_ce_work_bytes(n, 8, 5, 0, 0) == 0 and L.tf_weight_grad8_work_floats(n, 8, 8, 0) == 0

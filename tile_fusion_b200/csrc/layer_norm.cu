@@ -207,7 +207,7 @@ template <class T> cudaError_t ln_by_align(const LnShape &s, const LnParams &P, 
 int ln_check(const char *who, int rows, int cols, int dtype, int w_dtype, const void *codes, int ld_codes, const void *exps) {
   auto bad = [&](const char *what) { return tf::fail(TF_ERR_ARG, std::string(who) + ": " + what); };
   if (!known_dtype(dtype) || !known_dtype(w_dtype)) return bad("unknown type");
-  if (rows < 0 || cols <= 0) return bad("bad size");
+  if (rows < 0 || rows > kMaxRows || cols <= 0) return bad("bad size");
   if (cols > kLnMaxCols) return tf::fail(TF_ERR_UNSUPPORTED, std::string(who) + ": at most " + std::to_string(kLnMaxCols) + " columns");
   if (codes && (!exps || ld_codes != (cols + kPackGroup - 1) / kPackGroup * kPackGroup || (reinterpret_cast<uintptr_t>(codes) & 31) != 0))
     return bad("codes need exponents, rows as long as the columns' groups of 32, and 32-byte alignment");

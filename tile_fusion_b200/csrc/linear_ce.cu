@@ -429,7 +429,7 @@ int ce_check(const char *who, const void *x, long long ld_x, const void *w, long
              int vocab, int reduction, const void *work) {
   auto bad = [&](const char *what) { return tf::fail(TF_ERR_ARG, std::string(who) + ": " + what); };
   if (!known_dtype(dtype)) return bad("unknown type");
-  if (rows < 0 || cols <= 0 || vocab <= 0) return bad("bad size");
+  if (rows < 0 || cols <= 0 || vocab <= 0 || rows > kMaxRows || cols > kMaxRows || vocab > kMaxRows) return bad("bad size");
   if (rows > 0 && (!x || !target)) return bad("null argument");
   if (!w || !work) return bad("null argument");
   if (ld_x < cols || ld_w < cols) return bad("rows overlap");
@@ -476,7 +476,7 @@ cudaError_t ce_planes(const CeSpace &sp, const void *x, long long ld_x, const vo
 using namespace tfk;
 
 extern "C" long long tf_linear_ce_work_bytes(int rows, int cols, int vocab, int dtype, int backward) {
-  if (rows < 0 || cols <= 0 || vocab <= 0 || !known_dtype(dtype)) return 0;
+  if (rows < 0 || cols <= 0 || vocab <= 0 || rows > kMaxRows || cols > kMaxRows || vocab > kMaxRows || !known_dtype(dtype)) return 0;
   return ce_space(nullptr, std::max(rows, 1), cols, vocab, dtype, backward != 0, false, false).bytes;
 }
 

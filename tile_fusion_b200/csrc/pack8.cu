@@ -182,7 +182,7 @@ int done(const char *who) {
 int check(const char *who, const void *values, long long ld, int dtype, int rows, int cols, const void *codes, int ld_codes, const void *exps) {
   auto bad = [&](const char *what) { return tf::fail(TF_ERR_ARG, std::string(who) + ": " + what); };
   if (!known_dtype(dtype)) return bad("unknown type");
-  if (rows < 0 || cols <= 0 || cols > (1 << 30)) return bad("bad size");
+  if (rows < 0 || rows > kMaxRows || cols <= 0 || cols > (1 << 30)) return bad("bad size");
   if (ld < cols || ld_codes < cols) return bad("rows overlap");
   if (ld_codes % kPackGroup != 0 || (reinterpret_cast<uintptr_t>(codes) & 31) != 0) return bad("codes need rows of whole groups of 32 and 32-byte alignment");
   if (rows > 0 && (!values || !codes || !exps)) return bad("null argument");

@@ -9,6 +9,7 @@
 
 namespace tfk {
 
+constexpr int kMaxRows = 0x7f000000;  // of rows, columns and classes: an index and a grid's step beyond it stay below 2^31
 __host__ __device__ constexpr int value_bytes(int dtype) { return dtype == TF_F32 ? 4 : 2; }
 __host__ __device__ constexpr bool known_dtype(int dtype) { return dtype == TF_F32 || dtype == TF_BF16 || dtype == TF_F16; }
 

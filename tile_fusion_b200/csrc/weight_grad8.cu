@@ -440,7 +440,7 @@ template <class T, int PLANES> cudaError_t wg_run(const WgPlan &p, WgParams P, c
 using namespace tfk;
 
 extern "C" long long tf_weight_grad8_work_floats(int m, int na, int nb, int dtype) {
-  if (m < 0 || na <= 0 || nb <= 0 || !known_dtype(dtype)) return 0;
+  if (m < 0 || m > kMaxRows || na <= 0 || nb <= 0 || na > kMaxRows || nb > kMaxRows || !known_dtype(dtype)) return 0;
   return (long long)wg_plan(m, na, nb, dtype).parts * na * nb;
 }
 
@@ -448,7 +448,7 @@ extern "C" int tf_weight_grad8(const void *g, long long ld_g, int dtype, int na,
                                const unsigned char *exponents, int nb, int m, void *out, float *work, long long work_floats, void *stream) {
   auto bad = [&](const char *what) { return tf::fail(TF_ERR_ARG, std::string("tf_weight_grad8: ") + what); };
   if (!known_dtype(dtype)) return bad("unknown type");
-  if (m < 0 || na <= 0 || nb <= 0) return bad("bad size");
+  if (m < 0 || m > kMaxRows || na <= 0 || nb <= 0) return bad("bad size");
   // (the tiles of a side are a dimension of the grid, 65 535 at most, and a slice's bytes are counted in 32 bits)
   if ((long long)na * nb > (1 << 26) || na > (1 << 20) || nb > (1 << 20))
     return tf::fail(TF_ERR_UNSUPPORTED, "tf_weight_grad8: at most 2^26 entries, 2^20 to a side");

@@ -40,6 +40,7 @@ from torch.autograd.function import once_differentiable
 from . import _lib
 
 _DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+_MOST = 0x7f000000
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 
 
@@ -69,8 +70,8 @@ def _rows(t):
     """t as [rows, columns] whose rows do not overlap and have their values side by side."""
     if t.dim() != 2:
         t = t.reshape(-1, t.shape[-1])
-    if t.shape[0] > 0x7fffffff or t.shape[1] > 0x7fffffff:
-        raise ValueError(f"sw_gcn: matrices of at most 2^31 - 1 rows and columns, not {tuple(t.shape)}")
+    if t.shape[0] > _MOST or t.shape[1] > _MOST:
+        raise ValueError(f"sw_gcn: matrices of at most {_MOST} rows and columns, not {tuple(t.shape)}")
     if t.is_contiguous():
         return t
     return t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] else t.contiguous()
