@@ -339,6 +339,17 @@ __global__ void __launch_bounds__(256) ce_few_sum_kernel(const float *__restrict
   store_value(out, dtype, i, v * *scale);
 }
 
+// Gradients of a call one of whose bounded waits ran out: NaN, as the forward's loss.
+__global__ void __launch_bounds__(256) ce_lost_kernel(const CeHeader *h, void *__restrict__ dx, long long nx, void *__restrict__ dw, long long nw, int dtype) {
+  if (!h->error) return;
+  const float nan = __int_as_float(0x7fc00000);
+  const long long i0 = blockIdx.x * (long long)blockDim.x + threadIdx.x, step = (long long)gridDim.x * blockDim.x;
+  if (dx)
+    for (long long i = i0; i < nx; i += step) store_value(dx, dtype, i, nan);
+  if (dw)
+    for (long long i = i0; i < nw; i += step) store_value(dw, dtype, i, nan);
+}
+
 long long up(long long v, long long to) { return (v + to - 1) / to * to; }
 
 // What the workspace holds, for the sizes of a call; `base` null: sizes only.
@@ -439,6 +450,11 @@ int ce_check(const char *who, const void *x, long long ld_x, const void *w, long
 }
 
 int ce_fail(const char *who, cudaError_t e) { return tf::fail(TF_ERR_CUDA, std::string(who) + ": " + cudaGetErrorString(e)); }
+
+cudaError_t ce_lost(const CeHeader *h, void *dx, long long nx, void *dw, long long nw, int dtype, cudaStream_t s) {
+  ce_lost_kernel<<<(unsigned)std::min<long long>((std::max(nx, nw) + 1023) / 1024, 148 * 4), 256, 0, s>>>(h, dx, nx, dw, nw, dtype);
+  return cudaGetLastError();
+}
 
 int sm_count() {
   int dev = 0, sms = 148;
@@ -571,6 +587,7 @@ extern "C" int tf_linear_ce_bwd(const void *x, long long ld_x, const void *w, lo
       ce_few_sum_kernel<<<(vocab * cols + 31) / 32, 256, 0, s>>>(sp.parts_w, ce_few_ctas(rows), vocab * cols, &sp.h->unscale_slope, dw, dtype);
       e = cudaGetLastError();
     }
+    if (e == cudaSuccess) e = ce_lost(sp.h, dx, (long long)rows * cols, dw, (long long)vocab * cols, dtype, s);
     return e == cudaSuccess ? TF_OK : ce_fail(who, e);
   }
   e = ce_planes(sp, x, ld_x, w, ld_w, dtype, rows, cols, vocab, target, ignore_index, nullptr, s);
@@ -641,6 +658,7 @@ extern "C" int tf_linear_ce_bwd(const void *x, long long ld_x, const void *w, lo
                                                                                              &sp.h->unscale_slope, f32 ? &sp.h->unscale_w : nullptr, dx, dtype);
   }
   e = cudaGetLastError();
+  if (e == cudaSuccess) e = ce_lost(sp.h, dx, (long long)rows * cols, dw, (long long)vocab * cols, dtype, s);
   return e == cudaSuccess ? TF_OK : ce_fail(who, e);
 }
 
