@@ -103,3 +103,25 @@ def test_rows_next_to_2_31(L):
     refused(L.tf_linear_ce_fwd(P, 8, P, 8, 0, P, n, 8, 5, -100, 1, P, P, P, 1 << 40, None), "size")
     refused(L.tf_linear_ce_fwd(P, 8, P, 8, 0, P, 4, 8, n, -100, 1, P, P, P, 1 << 40, None), "size")
     assert L.tf_linear_ce_work_bytes(n, 8, 5, 0, 0) == 0 and L.tf_weight_grad8_work_floats(n, 8, 8, 0) == 0
+
+
+def test_layer_that_keeps_8_bits_refuses(built_lib):
+    import torch
+    from tile_fusion_b200 import sw_gcn  # noqa: F401
+    ck8 = torch.ops.sw_gcn.fusedGeMMSpMM_ck8
+    i = torch.arange(5, dtype=torch.int32)
+    adj = torch.sparse_csr_tensor(i, i[:4], torch.ones(4), size=(4, 4))
+    with pytest.raises(ValueError, match="CUDA"):
+        ck8(adj, torch.ones(4, 8), torch.ones(2, 8), [], 1)
+    with pytest.raises(ValueError, match="chain"):
+        ck8(adj, torch.ones(4, 8), torch.ones(2, 7), [], 1)
+    wide = torch.sparse_csr_tensor(i[:4], i[:3], torch.ones(3), size=(3, 4))  # its gradient would read rows that are not there
+    with pytest.raises(ValueError, match="square"):
+        ck8(wide, torch.ones(4, 8), torch.ones(2, 8), [], 1)
+
+
+def test_8_bits_of_no_matrix(built_lib):
+    import torch
+    from tile_fusion_b200 import sw_gcn  # noqa: F401
+    with pytest.raises(ValueError, match="codes"):
+        torch.ops.sw_gcn.unpack8(torch.zeros((), dtype=torch.int8), torch.zeros(1, dtype=torch.uint8))

@@ -164,9 +164,9 @@ def unpack8(codes, exponents, dtype=None):
     dtype = torch.float32 if dtype is None else dtype
     if dtype not in _DTYPES:
         raise ValueError(f"sw_gcn.unpack8: dtype must be float32, bfloat16 or float16, not {dtype}")
-    n, d = codes.shape[0], codes.shape[-1]
+    d = codes.shape[-1] if codes.dim() else 0
     codes, exponents, ld = _packed("unpack8", codes, exponents)
-    return _unpack(codes, ld, exponents, dtype, n, d)
+    return _unpack(codes, ld, exponents, dtype, codes.shape[0], d)
 
 
 def weight_grad8(grad, codes, exponents):

@@ -160,10 +160,16 @@ class _FusedGeMMSpMMCk8(torch.autograd.Function):
 
 
 def _ck8(adj, feature, weight, schedule, num_threads, relu=False):
-    if feature.dim() != 2 or weight.dim() != 2 or feature.shape[1] != weight.shape[1] or adj.shape[1] != feature.shape[0]:
-        raise ValueError(f"sw_gcn.fusedGeMMSpMM_ck8: adj {tuple(adj.shape)}, feature {tuple(feature.shape)} and weight "
-                         f"{tuple(weight.shape)} do not chain")
-    return _FusedGeMMSpMMCk8.apply(adj, feature, weight, bool(relu))
+    name = "sw_gcn.fusedGeMMSpMM_ck8"
+    if feature.dim() != 2 or weight.dim() != 2 or feature.shape[1] != weight.shape[1] or tuple(adj.shape) != (feature.shape[0],) * 2:
+        raise ValueError(f"{name}: adj {tuple(adj.shape)}, feature {tuple(feature.shape)} and weight {tuple(weight.shape)} do not chain "
+                         "(the adjacency is square)")
+    if not feature.is_cuda or weight.device != feature.device:
+        raise ValueError(f"{name}: feature and weight must be CUDA tensors on one device, not {feature.device} and {weight.device}")
+    if not feature.is_floating_point() or not weight.is_floating_point():
+        raise ValueError(f"{name}: feature and weight must hold floating-point values, not {feature.dtype}, {weight.dtype}")
+    with torch.cuda.device(feature.device):
+        return _FusedGeMMSpMMCk8.apply(adj, feature, weight, bool(relu))
 
 
 class _CachedSpMMGeMM(torch.autograd.Function):
