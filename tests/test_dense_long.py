@@ -1,0 +1,120 @@
+"""The dense operators where offsets pass 32 bits: operands of more than 2^31 values.  Rows do not touch each other, so the last rows
+are compared with the same operator on a copy of them alone (which the other tests compare with the formulas), in their places; sums
+over rows have values in the first and the last rows only.
+
+Tolerances: rows on their own are the same operations in the same order (bit by bit); the loss of many rows and of few may cut its
+products differently, and sums over rows are added in another order: 2e-5 of the 2-norm, as for the sums of the other tests, and half a
+step of the type where a result was rounded to it once on either side.
+"""
+import math
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+U = {"float32": 2.0 ** -24, "bfloat16": 2.0 ** -8, "float16": 2.0 ** -11}
+
+
+def ends(t, k):
+    import torch
+    return torch.cat((t[:k], t[-k:]))
+
+
+def near(got, want, u):
+    off = (got.double() - want.double()).norm().item()
+    assert off <= (2 * u + 2e-5) * want.double().norm().item(), off / want.double().norm().item()
+
+
+@pytest.mark.parametrize("cols,checkpoint", [(2048, False), (250, True)])
+def test_layer_norm(built_lib, cols, checkpoint):
+    import torch
+    from tile_fusion_b200 import sw_gcn  # noqa: F401
+    ops = torch.ops.sw_gcn
+    n, k = 2 ** 31 // cols + 1000, 300
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    x = torch.empty(n, cols, device="cuda", dtype=torch.bfloat16).normal_(generator=gen)
+    g = torch.zeros_like(x)
+    g[:k].normal_(generator=gen)
+    g[-k:].normal_(generator=gen)
+    w, b = torch.randn(cols, generator=gen, device="cuda"), torch.randn(cols, generator=gen, device="cuda")
+
+    def run(x, g):
+        leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+        y = ops.layer_norm(*leaves, 1e-5, checkpoint)
+        return (y.detach(),) + torch.autograd.grad(y, leaves, g)
+
+    y, dx, dw, db = run(x, g)
+    want = run(ends(x, k), ends(g, k))
+    assert torch.equal(ends(y, k), want[0])
+    assert torch.equal(ends(dx, k), want[1])
+    assert not dx[k:-k:1000].any()
+    near(dw, want[2], U["float32"])
+    near(db, want[3], U["float32"])
+
+
+def test_8_bits(built_lib):
+    import torch
+    from tile_fusion_b200 import sw_gcn  # noqa: F401
+    ops = torch.ops.sw_gcn
+    d, k = 100, 500
+    n = 2 ** 31 // d + 1000
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    x = torch.empty(n, d, device="cuda", dtype=torch.float16).normal_(generator=gen)
+    codes, exponents = ops.pack8(x, True)
+    some = ops.pack8(ends(x, k), True)
+    assert torch.equal(ends(codes, k), some[0]) and torch.equal(ends(exponents, k), some[1])
+    back = ops.unpack8(codes, exponents, torch.bfloat16)
+    assert torch.equal(ends(back, k), ops.unpack8(*some, torch.bfloat16))
+    del back, x
+    g = torch.zeros(n, 104, device="cuda", dtype=torch.bfloat16)
+    g[:k].normal_(generator=gen)
+    g[-k:].normal_(generator=gen)
+    near(ops.weight_grad8(g, codes, exponents), ops.weight_grad8(ends(g, k), *some), U["bfloat16"])
+
+
+@pytest.mark.parametrize("d,v,dtype", [(256, 40, "bfloat16"), (2048, 300, "float16")])
+def test_loss_of_many_rows(built_lib, d, v, dtype):
+    import torch
+    from tile_fusion_b200 import sw_gcn  # noqa: F401
+    n, k = 2 ** 31 // d + 1000, 500
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    x = torch.empty(n, d, device="cuda", dtype=getattr(torch, dtype)).normal_(generator=gen)
+    w = (torch.randn(v, d, generator=gen, device="cuda") / math.sqrt(d)).to(x.dtype)
+    target = torch.full((n,), -100, device="cuda")
+    target[:k] = torch.randint(0, v, (k,), generator=gen, device="cuda")
+    target[-k:] = torch.randint(0, v, (k,), generator=gen, device="cuda")
+
+    def run(x, target):
+        x, p = x.detach().requires_grad_(), w.detach().requires_grad_()
+        loss = torch.ops.sw_gcn.linear_cross_entropy(x, p, target, -100, "none")
+        return (loss.detach(),) + torch.autograd.grad(loss.sum(), (x, p))
+
+    loss, dx, dw = run(x, target)
+    want = run(ends(x, k), ends(target, k))
+    near(ends(loss, k), want[0], U["float32"])
+    near(ends(dx, k), want[1], U[dtype])
+    near(dw, want[2], U[dtype])
+    assert not loss[k:-k].any() and not dx[k:-k:1000].any()
+
+
+def test_loss_of_many_classes(built_lib):
+    import torch
+    from tile_fusion_b200 import sw_gcn  # noqa: F401
+    n, d = 70, 4096
+    v = 2 ** 31 // d + 1000
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    w = (torch.empty(v, d, device="cuda", dtype=torch.bfloat16).normal_(generator=gen).mul_(1 / math.sqrt(d))).requires_grad_()
+    x = torch.randn(n, d, generator=gen, device="cuda").to(torch.bfloat16).requires_grad_()
+    target = torch.randint(v - 900, v, (n,), generator=gen, device="cuda")
+    loss = torch.ops.sw_gcn.linear_cross_entropy(x, w, target, -100, "mean")
+    dx, dw = torch.autograd.grad(loss, (x, w))
+    with torch.no_grad():
+        logits = torch.cat([x.double() @ p.double().t() for p in w.split(65536)], 1)
+        p = torch.softmax(logits, 1)
+        want = (torch.logsumexp(logits, 1) - logits.gather(1, target[:, None])[:, 0]).mean()
+        p[torch.arange(n, device="cuda"), target] -= 1
+        p /= n
+        assert abs(loss.item() - want.item()) <= 2e-5
+        near(dw[-1000:], p[:, -1000:].t() @ x.double(), U["bfloat16"])
+        near(dw[:1000], p[:, :1000].t() @ x.double(), U["bfloat16"])
+        near(dx, sum(q.double() @ c.double() for q, c in zip(p.split(65536, 1), w.split(65536))), U["bfloat16"])
