@@ -82,7 +82,6 @@ __global__ void __launch_bounds__(kLnWarpThreads) ln_forward_kernel(const LnPara
   LnPlace<T, LANES> at;
   const int t = at.t;
   const LnCols<T, PIECE> col = {t, LANES};
-  int slot = 0;
   float w[NV][N], b[NV][N];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -104,10 +103,10 @@ __global__ void __launch_bounds__(kLnWarpThreads) ln_forward_kernel(const LnPara
     fetch(at.row + at.step);
     auto x = [&](int i) { return now[i]; };
     float sum[1] = {ln_total<T, NV>(x)};
-    ln_sum<LANES, 1>(sum, nullptr, slot);
+    ln_sum<LANES, 1>(sum);
     const float mean = sum[0] * over;
     float var[1] = {ln_spread<T, NV, PIECE>(x, mean, P.cols, col)};
-    ln_sum<LANES, 1>(var, nullptr, slot);
+    ln_sum<LANES, 1>(var);
     const float rstd = 1.f / sqrtf(var[0] * over + P.eps);
     ln_write<T, AL, PIECE, NV, KEEP8>(P, x, at.row, in, mean, rstd, col, w, b);
     if (in && t == 0) {
@@ -123,7 +122,7 @@ template <class T, int AL, int PIECE, int NV, bool KEEP8>
 __global__ void __launch_bounds__(kLnRowThreads, 1) ln_forward_rows_kernel(const LnParams P) {
   constexpr int N = kLnN<T>, R = ln_rows_at_once<NV>(), AHEAD = ln_ahead<NV>();
   extern __shared__ float4 rows_smem[];
-  __shared__ float scratch[2][kLnRowThreads / 32][R];
+  __shared__ float scratch[2][kLnRowThreads / 32 * R];
   const int t = threadIdx.x, lanes = blockDim.x;
   Pack<T, N> *sx = reinterpret_cast<Pack<T, N> *>(rows_smem);
   const LnCols<T, PIECE> col = {t, lanes};
@@ -156,13 +155,13 @@ __global__ void __launch_bounds__(kLnRowThreads, 1) ln_forward_rows_kernel(const
     float sum[R], var[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) sum[r] = ln_total<T, NV>([&](int i) { return sx[at(turn, r, i)]; });
-    ln_sum<0, R>(sum, scratch, slot);
+    ln_sum_cta<R>(sum, scratch, slot);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       sum[r] *= over;  // the mean
       var[r] = ln_spread<T, NV, PIECE>([&](int i) { return sx[at(turn, r, i)]; }, sum[r], P.cols, col);
     }
-    ln_sum<0, R>(var, scratch, slot);
+    ln_sum_cta<R>(var, scratch, slot);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const bool in = row + r < P.rows;
@@ -182,15 +181,15 @@ template <class T, int AL, int PIECE, bool KEEP8> cudaError_t ln_by_nv(const LnS
   int ctas;
 #define TF_LN(NV)                                                                                                                              \
   if (s.nv == NV) {                                                                                                                            \
-    if (s.lanes == 0)                                                                                                                          \
+    if constexpr ((NV & (NV - 1)) == 0) if (s.lanes == 0)                                                                                                                          \
       return ln_go(ln_forward_rows_kernel<T, AL, PIECE, NV, KEEP8>, s, P, ln_rows_at_once<NV>(), (ln_ahead<NV>() + 1) * ln_turn_bytes<T, NV>(s.threads), ctas, st); \
+    if (s.lanes == 32) return ln_go(ln_forward_kernel<T, AL, PIECE, NV, 32, KEEP8>, s, P, s.threads / 32, 0, ctas, st);                         \
     if constexpr (NV <= 16 / kLnN<T>) {                                                                                                        \
-      if (s.lanes == 32) return ln_go(ln_forward_kernel<T, AL, PIECE, NV, 32, KEEP8>, s, P, kLnWarpThreads / 32, 0, ctas, st);                         \
       return ln_go(ln_forward_kernel<T, AL, PIECE, NV, 8, KEEP8>, s, P, kLnWarpThreads / 8, 0, ctas, st);                                             \
     }                                                                                                                                          \
   }
   TF_LN(1) TF_LN(2) TF_LN(4)
-  if constexpr (sizeof(T) == 4) { TF_LN(8) }
+  if constexpr (sizeof(T) == 4) { TF_LN(5) TF_LN(6) TF_LN(8) } else { TF_LN(3) }
 #undef TF_LN
   return cudaErrorInvalidValue;
 }
@@ -232,7 +231,7 @@ extern "C" int tf_layer_norm_fwd(const void *x, long long ld_x, int dtype, const
   P.rows = rows; P.cols = cols; P.eps = eps; P.y = y; P.ld_y = ld_y; P.mean = mean; P.rstd = rstd;
   P.codes = codes; P.ld_codes = ld_codes; P.exps = exponents;
   // (codes reach to the end of the columns' group)
-  const LnShape s = ln_shape(ln_pieces(cols, bytes, codes != nullptr, {{x, ld_x}, {y, ld_y}}), codes ? ld_codes : cols, bytes);
+  const LnShape s = ln_shape(ln_pieces(cols, bytes, codes != nullptr, {{x, ld_x}, {y, ld_y}}), codes ? ld_codes : cols, bytes, codes ? 768 : 1024);
   cudaStream_t st = (cudaStream_t)stream;
   const cudaError_t e = dtype == TF_F32 ? ln_by_align<float>(s, P, st) : dtype == TF_BF16 ? ln_by_align<__nv_bfloat16>(s, P, st) : ln_by_align<__half>(s, P, st);
   return e == cudaSuccess ? TF_OK : tf::fail(TF_ERR_CUDA, std::string("tf_layer_norm_fwd: ") + cudaGetErrorString(e));

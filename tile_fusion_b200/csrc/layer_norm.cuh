@@ -86,26 +86,41 @@ template <class T, int PIECE> __device__ __forceinline__ void ln_weight(const vo
   for (int k = 0; k < N; ++k) v[k] = w && cols_(i, k) < P.cols ? load_value(w, P.w_dtype, cols_(i, k)) : none;
 }
 
-// K sums over LANES lanes, or (LANES == 0) over the CTA; `slot` alternates between two scratch arrays.
-template <int LANES, int K> __device__ __forceinline__ void ln_sum(float (&v)[K], float (*scratch)[kLnRowThreads / 32][K], int &slot) {
+// K sums over LANES lanes.
+template <int LANES, int K> __device__ __forceinline__ void ln_sum(float (&v)[K]) {
 #pragma unroll
-  for (int k = (LANES ? LANES : 32) / 2; k; k >>= 1)
+  for (int k = LANES / 2; k; k >>= 1)
 #pragma unroll
     for (int i = 0; i < K; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], k);
-  if (LANES == 0 && blockDim.x > 32) {
-    const int warps = blockDim.x / 32, lane = threadIdx.x & (kLnRowThreads / 32 - 1);  // (both halves of a warp add up all warps)
-    if ((threadIdx.x & 31) == 0)
+}
+// K sums (a power of two) over the CTA; `slot` alternates between two scratch arrays.  A lane hands on half of its sums and adds
+// up the other half until it has one: 6 shuffles for four sums where one at a time would take 20.  Behind the barrier the lanes
+// of each warp add up the warps' sums in the same order.
+template <int K> __device__ __forceinline__ void ln_sum_cta(float (&v)[K], float (*scratch)[kLnRowThreads / 32 * K], int &slot) {
+  const int lane = threadIdx.x & 31, warps = blockDim.x / 32;
+  if (warps == 1) return ln_sum<32, K>(v);
 #pragma unroll
-      for (int i = 0; i < K; ++i) scratch[slot][threadIdx.x >> 5][i] = v[i];
-    __syncthreads();  // (one to a sum: the scratch array of the sum before last has been read by then)
+  for (int k = K / 2, o = 16; k; k >>= 1, o >>= 1) {
+    const bool upper = lane & o;
 #pragma unroll
-    for (int i = 0; i < K; ++i) v[i] = lane < warps ? scratch[slot][lane][i] : 0.f;
-#pragma unroll
-    for (int k = kLnRowThreads / 64; k; k >>= 1)
-#pragma unroll
-      for (int i = 0; i < K; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], k);
-    slot ^= 1;
+    for (int i = 0; i < k; ++i) {
+      const float given = upper ? v[i] : v[i + k], kept = upper ? v[i + k] : v[i];
+      v[i] = kept + __shfl_xor_sync(0xffffffffu, given, o);
+    }
   }
+#pragma unroll
+  for (int o = 16 / K; o; o >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+  if (lane % (32 / K) == 0) scratch[slot][(threadIdx.x >> 5) * K + lane / (32 / K)] = v[0];
+  __syncthreads();  // (one to a sum: the scratch array of the sum before last has been read by then)
+  float total = 0.f;
+#pragma unroll
+  for (int i = 0; i < kLnRowThreads / 32 * K; i += 32)
+    if (i + lane < warps * K) total += scratch[slot][i + lane];
+#pragma unroll
+  for (int o = 16; o >= K; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+#pragma unroll
+  for (int i = 0; i < K; ++i) v[i] = K == 1 ? total : __shfl_sync(0xffffffffu, total, i);
+  slot ^= 1;
 }
 
 // ---- a CTA to a row, several rows a turn, the rows of later turns on their way into shared memory ----
@@ -158,11 +173,11 @@ inline LnShape ln_pieces(int cols, int bytes, bool keep8, std::initializer_list<
 // Eight lanes to a row where they hold it with 16 values each, a warp where it does (512 columns), a CTA beyond: of as many threads as
 // hold it with one access each up to 256, with two, four or (fp32) eight up to 512 (16 384 x 4 096 bf16, forward and backward: 256
 // threads with two 67 and 98 us, 512 with one 74 and 108).
-inline LnShape ln_shape(LnShape s, int cols, int bytes) {
+inline LnShape ln_shape(LnShape s, int cols, int bytes, int warp_cols) {
   const int n = 16 / bytes, vecs = (cols + n - 1) / n, most = 16 / n;
-  auto least = [&](int lanes) { int nv = 1; while (lanes * nv < vecs) nv *= 2; return nv; };
-  if (vecs <= 8 * most) return {s.al, s.piece, least(8), 8, kLnWarpThreads};
-  if (vecs <= 32 * most) return {s.al, s.piece, least(32), 32, kLnWarpThreads};
+  auto least = [&](int lanes, int nv) { while (lanes * nv < vecs) nv += nv < most ? nv : 1; return nv == 7 ? 8 : nv; };
+  if (vecs <= 8 * most) return {s.al, s.piece, least(8, 1), 8, kLnWarpThreads};
+  if (cols <= warp_cols) { const int nv = least(32, 1); return {s.al, s.piece, nv, 32, nv <= most ? kLnWarpThreads : kLnWarpThreads / 2}; }
   int nv = 1;
   while ((vecs + nv - 1) / nv > (nv == 1 ? 256 : kLnRowThreads)) nv *= 2;
   return {s.al, s.piece, nv, 0, ((vecs + nv - 1) / nv + 31) / 32 * 32};

@@ -27,7 +27,6 @@ __global__ void __launch_bounds__(kLnWarpThreads) ln_backward_kernel(const LnPar
   extern __shared__ float joined[];  // [warps][2][cols]
   LnPlace<T, LANES> at;
   const LnCols<T, PIECE> col = {at.t, LANES};
-  int slot = 0;
   float w[NV][N], dw[NV][N], db[NV][N];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -76,7 +75,7 @@ __global__ void __launch_bounds__(kLnWarpThreads) ln_backward_kernel(const LnPar
       }
     }
     fetch(at.row + at.step);
-    ln_sum<LANES, 2>(sum, nullptr, slot);
+    ln_sum<LANES, 2>(sum);
     const float m0 = sum[0] * over, m1 = sum[1] * over;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -109,7 +108,7 @@ __global__ void __launch_bounds__(kLnWarpThreads) ln_backward_kernel(const LnPar
   __syncthreads();
   for (int c = threadIdx.x; c < 2 * P.cols; c += blockDim.x) {
     float s = 0.f;
-    for (int k = 0; k < kLnWarpThreads / 32; ++k) s += joined[k * 2 * P.cols + c];
+    for (int k = 0; k < blockDim.x / 32; ++k) s += joined[k * 2 * P.cols + c];
     part[c] = s;
   }
 }
@@ -123,7 +122,7 @@ template <class T, int AL, int PIECE, int NV, bool KEEP8>
 __global__ void __launch_bounds__(kLnRowThreads, 1) ln_backward_rows_kernel(const LnParams P) {
   constexpr int N = kLnN<T>, R = ln_grad_rows<NV>(), AHEAD = ln_ahead<NV>(), TURNS = AHEAD + 1;
   extern __shared__ float4 rows_smem[];
-  __shared__ float scratch[2][kLnRowThreads / 32][2 * R];
+  __shared__ float scratch[2][kLnRowThreads / 32 * 2 * R];
   using Kept = Pack<signed char, N>;
   const int t = threadIdx.x, lanes = blockDim.x;
   Pack<T, N> *sg = reinterpret_cast<Pack<T, N> *>(rows_smem);
@@ -189,6 +188,9 @@ __global__ void __launch_bounds__(kLnRowThreads, 1) ln_backward_rows_kernel(cons
 #pragma unroll
         for (int i = 0; i < NV; ++i) unit[r][i] = unpack8_step(next_e[r][i]);
     }
+    constexpr bool KEEP = NV == 1;
+    Pack<T, N> kept_g[KEEP ? R : 1];
+    float kept_x[KEEP ? R : 1][N];
     fetch_stats(row + step);
     fetch(row + AHEAD * step, turn == 0 ? AHEAD : turn - 1);  // (a thread has read its part of that turn)
     asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD) : "memory");
@@ -210,6 +212,11 @@ __global__ void __launch_bounds__(kLnRowThreads, 1) ln_backward_rows_kernel(cons
         float xh[N];
         hats(r, i, xh);
         const Pack<T, N> g = sg[at(turn, r, i)];
+        if (KEEP) {
+          kept_g[r] = g;
+#pragma unroll
+          for (int k = 0; k < N; ++k) kept_x[r][k] = xh[k];
+        }
 #pragma unroll
         for (int k = 0; k < N; ++k) {  // (dy is zero where there is no value, and xh finite)
           const float gk = to_float(g.v[k]), h = gk * w[i][k];
@@ -221,8 +228,8 @@ __global__ void __launch_bounds__(kLnRowThreads, 1) ln_backward_rows_kernel(cons
       }
     }
     if (P.dx) {
-      // (values are read and converted again rather than kept: registers bound the rows in flight)
-      ln_sum<0, 2 * R>(sum, scratch, slot);
+      // (with more than one access a thread its values are read and converted again rather than kept: registers bound the rows in flight)
+      ln_sum_cta<2 * R>(sum, scratch, slot);
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         const float m0 = sum[2 * r] * over, m1 = sum[2 * r + 1] * over;
@@ -230,8 +237,15 @@ __global__ void __launch_bounds__(kLnRowThreads, 1) ln_backward_rows_kernel(cons
         for (int i = 0; i < NV; ++i) {
           if (row + r >= P.rows || col(i, 0) >= P.cols) continue;
           float xh[N], d[N];
-          hats(r, i, xh);
-          const Pack<T, N> g = sg[at(turn, r, i)];
+          Pack<T, N> g;
+          if (KEEP) {
+            g = kept_g[r];
+#pragma unroll
+            for (int k = 0; k < N; ++k) xh[k] = kept_x[r][k];
+          } else {
+            hats(r, i, xh);
+            g = sg[at(turn, r, i)];
+          }
 #pragma unroll
           for (int k = 0; k < N; ++k) d[k] = rstd[r] * (to_float(g.v[k]) * w[i][k] - m0 - xh[k] * m1);
           ln_store<T, AL, PIECE>(static_cast<T *>(P.dx) + (row + r) * P.ld_dx, col, i, P.cols, d);
@@ -271,13 +285,13 @@ __global__ void __launch_bounds__(1024) ln_join_kernel(const float *__restrict__
 }
 
 template <class T, int AL, int PIECE, bool KEEP8> cudaError_t ln_by_nv(const LnShape &s, const LnParams &P, int &ctas, cudaStream_t st) {
-  const size_t joined = (size_t)kLnWarpThreads / 32 * 2 * P.cols * 4;
+  const size_t joined = (size_t)s.threads / 32 * 2 * P.cols * 4;
 #define TF_LN(NV)                                                                                                                                  \
   if (s.nv == NV) {                                                                                                                                \
     if (s.lanes == 0)                                                                                                                              \
       return ln_go(ln_backward_rows_kernel<T, AL, PIECE, NV, KEEP8>, s, P, ln_grad_rows<NV>(), (ln_ahead<NV>() + 1) * ln_turn_bytes<T, NV, KEEP8>(s.threads), ctas, st); \
     if constexpr (NV <= 16 / kLnN<T>) {                                                                                                            \
-      if (s.lanes == 32) return ln_go(ln_backward_kernel<T, AL, PIECE, NV, 32, KEEP8>, s, P, kLnWarpThreads / 32, joined, ctas, st);                       \
+      if (s.lanes == 32) return ln_go(ln_backward_kernel<T, AL, PIECE, NV, 32, KEEP8>, s, P, s.threads / 32, joined, ctas, st);                    \
       return ln_go(ln_backward_kernel<T, AL, PIECE, NV, 8, KEEP8>, s, P, kLnWarpThreads / 8, joined, ctas, st);                                           \
     }                                                                                                                                              \
   }
@@ -323,7 +337,7 @@ extern "C" int tf_layer_norm_bwd(const void *x, long long ld_x, const signed cha
   P.codes = const_cast<signed char *>(codes); P.ld_codes = ld_codes; P.exps = const_cast<unsigned char *>(exponents);
   P.dy = dy; P.ld_dy = ld_dy; P.dx = dx; P.ld_dx = ld_dx; P.part = sums ? work : nullptr;
   cudaStream_t st = (cudaStream_t)stream;
-  const LnShape s = ln_shape(ln_pieces(cols, bytes, codes != nullptr, {{codes ? nullptr : x, ld_x}, {dy, ld_dy}, {dx, ld_dx}}), cols, bytes);
+  const LnShape s = ln_shape(ln_pieces(cols, bytes, codes != nullptr, {{codes ? nullptr : x, ld_x}, {dy, ld_dy}, {dx, ld_dx}}), cols, bytes, 512);
   int ctas = 0;
   cudaError_t e = cudaSuccess;
   if (rows > 0)
