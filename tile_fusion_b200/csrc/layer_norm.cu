@@ -2,7 +2,8 @@
 //
 // Bound by the row read and the row written.  A row stays in registers or in shared memory between its sums and its use, so it is
 // read once; the variance is that of the centred values.  Threads walk the rows with the grid's stride and keep their columns'
-// weights.  Up to 512 columns a row belongs to eight lanes or a warp, and the next row is on its way in registers; wider ones to a CTA,
+// weights.  Up to 1 024 columns (768 with codes) a row belongs to eight lanes or a warp, and the next row is on its way in registers (50 021
+// x 602 fp32: 39 us, 64 with a CTA to a row; 60 000 x 1 024 bf16 51 and 65; 30 000 x 1 024 fp32 with codes 75 and 58); wider ones to a CTA,
 // R rows a turn so that a barrier serves them all, and the rows of two turns ahead are on their way into shared memory; a thread
 // copies what it alone reads, so copies need no barrier.  Statistics are fp32 whatever the values' type.
 //   The pass can leave its input in 8 bits on the way (pack8.cuh), which the backward pass then reads in its place.
@@ -18,9 +19,8 @@ namespace tfk {
 namespace {
 
 // One row whose statistics are known.
-template <class T, int AL, int PIECE, int NV, bool KEEP8, class Value>
-__device__ __forceinline__ void ln_write(const LnParams &P, Value x, long long row, bool in, float mean, float rstd, LnCols<T, PIECE> col, const float (&w)[NV][kLnN<T>],
-                                         const float (&b)[NV][kLnN<T>]) {
+template <class T, int AL, int PIECE, int NV, bool KEEP8, class Value, class Weights>
+__device__ __forceinline__ void ln_write(const LnParams &P, Value x, long long row, bool in, float mean, float rstd, LnCols<T, PIECE> col, Weights weights) {
   constexpr int N = kLnN<T>;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -37,8 +37,7 @@ __device__ __forceinline__ void ln_write(const LnParams &P, Value x, long long r
       }
     }
     if (!in || col(i, 0) >= P.cols) continue;
-#pragma unroll
-    for (int k = 0; k < N; ++k) v[k] = fmaf((v[k] - mean) * rstd, w[i][k], b[i][k]);
+    weights(i, [&](int k, float w, float b) { v[k] = fmaf((v[k] - mean) * rstd, w, b); });
     ln_store<T, AL, PIECE>(static_cast<T *>(P.y) + row * P.ld_y, col, i, P.cols, v);
   }
 }
@@ -75,19 +74,53 @@ template <class T, int NV, int PIECE, class Value> __device__ __forceinline__ fl
   return s;
 }
 
+// Weights of more than 16 values of a thread would take the registers of rows in flight where values are packed or make codes: they
+// lie in shared memory, and CTAs of 128 threads are held to 102 registers (80 000 x 768 bf16: 48 us, 58 with weights in registers;
+// 128 where every value is an access of its own, 50 021 x 999 bf16: 52 and 66).
+template <class T, int NV, bool KEEP8> __host__ __device__ constexpr bool ln_shares() { return NV * kLnN<T> > 16 && (KEEP8 || sizeof(T) == 2); }
+// A read that stays where it is: hoisted out of the loop over rows it would take the registers it is there to save.
+__device__ __forceinline__ float4 ln_shared4(const float4 *p) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"((unsigned)__cvta_generic_to_shared(p)));
+  return v;
+}
+
 // Eight lanes or a warp to a row.
 template <class T, int AL, int PIECE, int NV, int LANES, bool KEEP8>
-__global__ void __launch_bounds__(kLnWarpThreads) ln_forward_kernel(const LnParams P) {
+__global__ void __launch_bounds__(NV * kLnN<T> > 16 ? kLnWarpThreads / 2 : kLnWarpThreads, ln_shares<T, NV, KEEP8>() ? (PIECE > 1 ? 5 : 4) : 0) ln_forward_kernel(const LnParams P) {
   constexpr int N = kLnN<T>;
   LnPlace<T, LANES> at;
   const int t = at.t;
   const LnCols<T, PIECE> col = {t, LANES};
-  float w[NV][N], b[NV][N];
+  constexpr bool SHARED = ln_shares<T, NV, KEEP8>();
+  __shared__ float4 sw[SHARED ? NV * N / 4 : 1][SHARED ? 32 : 1], sb[SHARED ? NV * N / 4 : 1][SHARED ? 32 : 1];
+  float w[SHARED ? 1 : NV][N], b[SHARED ? 1 : NV][N];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    ln_weight<T, PIECE>(P.w, P, col, i, 1.f, w[i]);
-    ln_weight<T, PIECE>(P.b, P, col, i, 0.f, b[i]);
+    float(&wi)[N] = w[SHARED ? 0 : i], (&bi)[N] = b[SHARED ? 0 : i];
+    if (SHARED && threadIdx.x >= 32) break;
+    ln_weight<T, PIECE>(P.w, P, col, i, 1.f, wi);
+    ln_weight<T, PIECE>(P.b, P, col, i, 0.f, bi);
+    if constexpr (SHARED)
+#pragma unroll
+      for (int k = 0; k < N; k += 4) {
+        sw[(i * N + k) / 4][t] = make_float4(wi[k], wi[k + 1], wi[k + 2], wi[k + 3]);
+        sb[(i * N + k) / 4][t] = make_float4(bi[k], bi[k + 1], bi[k + 2], bi[k + 3]);
+      }
   }
+  if (SHARED) __syncthreads();
+  auto weights = [&](int i, auto f) {
+    if constexpr (SHARED) {
+#pragma unroll
+      for (int k = 0; k < N; k += 4) {
+        const float4 p = ln_shared4(&sw[(i * N + k) / 4][t]), q = ln_shared4(&sb[(i * N + k) / 4][t]);
+        f(k, p.x, q.x); f(k + 1, p.y, q.y); f(k + 2, p.z, q.z); f(k + 3, p.w, q.w);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < N; ++k) f(k, w[i][k], b[i][k]);
+    }
+  };
   const float over = 1.f / (float)P.cols;
   Pack<T, N> next[NV];
   auto fetch = [&](long long row) {
@@ -107,8 +140,8 @@ __global__ void __launch_bounds__(kLnWarpThreads) ln_forward_kernel(const LnPara
     const float mean = sum[0] * over;
     float var[1] = {ln_spread<T, NV, PIECE>(x, mean, P.cols, col)};
     ln_sum<LANES, 1>(var);
-    const float rstd = 1.f / sqrtf(var[0] * over + P.eps);
-    ln_write<T, AL, PIECE, NV, KEEP8>(P, x, at.row, in, mean, rstd, col, w, b);
+    const float rstd = rsqrtf(var[0] * over + P.eps);
+    ln_write<T, AL, PIECE, NV, KEEP8>(P, x, at.row, in, mean, rstd, col, weights);
     if (in && t == 0) {
       if (P.mean) P.mean[at.row] = mean;
       if (P.rstd) P.rstd[at.row] = rstd;
@@ -134,6 +167,10 @@ __global__ void __launch_bounds__(kLnRowThreads, 1) ln_forward_rows_kernel(const
     ln_weight<T, PIECE>(P.w, P, col, i, 1.f, w[i]);
     ln_weight<T, PIECE>(P.b, P, col, i, 0.f, b[i]);
   }
+  auto weights = [&](int i, auto f) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) f(k, w[i][k], b[i][k]);
+  };
   const float over = 1.f / (float)P.cols;
   const long long step = gridDim.x * (long long)R;
   auto fetch = [&](long long row, int turn) {
@@ -165,8 +202,8 @@ __global__ void __launch_bounds__(kLnRowThreads, 1) ln_forward_rows_kernel(const
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const bool in = row + r < P.rows;
-      const float rstd = 1.f / sqrtf(var[r] * over + P.eps);
-      ln_write<T, AL, PIECE, NV, KEEP8>(P, [&](int i) { return sx[at(turn, r, i)]; }, row + r, in, sum[r], rstd, col, w, b);
+      const float rstd = rsqrtf(var[r] * over + P.eps);
+      ln_write<T, AL, PIECE, NV, KEEP8>(P, [&](int i) { return sx[at(turn, r, i)]; }, row + r, in, sum[r], rstd, col, weights);
       if (in && t == 0) {
         if (P.mean) P.mean[row + r] = sum[r];
         if (P.rstd) P.rstd[row + r] = rstd;
@@ -181,9 +218,9 @@ template <class T, int AL, int PIECE, bool KEEP8> cudaError_t ln_by_nv(const LnS
   int ctas;
 #define TF_LN(NV)                                                                                                                              \
   if (s.nv == NV) {                                                                                                                            \
-    if constexpr ((NV & (NV - 1)) == 0) if (s.lanes == 0)                                                                                                                          \
+    if constexpr ((NV & (NV - 1)) == 0 && (NV > 1 || KEEP8 || sizeof(T) == 2)) if (s.lanes == 0)                                                                                                                          \
       return ln_go(ln_forward_rows_kernel<T, AL, PIECE, NV, KEEP8>, s, P, ln_rows_at_once<NV>(), (ln_ahead<NV>() + 1) * ln_turn_bytes<T, NV>(s.threads), ctas, st); \
-    if (s.lanes == 32) return ln_go(ln_forward_kernel<T, AL, PIECE, NV, 32, KEEP8>, s, P, s.threads / 32, 0, ctas, st);                         \
+    if constexpr (NV * kLnN<T> < 32 || !KEEP8) if (s.lanes == 32) return ln_go(ln_forward_kernel<T, AL, PIECE, NV, 32, KEEP8>, s, P, s.threads / 32, 0, ctas, st);                         \
     if constexpr (NV <= 16 / kLnN<T>) {                                                                                                        \
       return ln_go(ln_forward_kernel<T, AL, PIECE, NV, 8, KEEP8>, s, P, kLnWarpThreads / 8, 0, ctas, st);                                             \
     }                                                                                                                                          \

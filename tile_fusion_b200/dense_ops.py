@@ -8,8 +8,8 @@
     torch.ops.sw_gcn.linear_cross_entropy(x, weight, target, ignore_index=-100, reduction="mean")
 
 ``layer_norm`` is over the last dimension, with the gradients of x, weight and bias; weight and bias have x's type or
-another of the three.  With ``checkpoint`` it keeps x in 8 bits for the backward pass (x itself can be freed): y is the
-same, the gradients are those of the formula at the kept values.
+another of the three.  With ``checkpoint`` it keeps x in 8 bits for the backward pass (x itself can be freed): y is still
+that of x, the gradients are those of the formula at the kept values.
 
 ``pack8`` puts activations [rows, columns] into 8 bits: 32 neighbouring columns share a power of two, a value is a whole
 number of steps of its 64th part, the nearest one, at most 127 of them.  ``codes`` is int8 [rows, columns] with rows that
