@@ -118,3 +118,18 @@ def test_loss_of_many_classes(built_lib):
         near(dw[-1000:], p[:, -1000:].t() @ x.double(), U["bfloat16"])
         near(dw[:1000], p[:, :1000].t() @ x.double(), U["bfloat16"])
         near(dx, sum(q.double() @ c.double() for q, c in zip(p.split(65536, 1), w.split(65536))), U["bfloat16"])
+
+
+def test_weight_gradient_of_many_rows_of_one_sign(built_lib):
+    """The tensor core cuts off what it adds (2e-8 of the sum at a time), so an accumulator may not add up all rows: 10^8 equal products.
+    Tolerance: at most 4 096 additions to a sum, 1e-4, and the result's rounding."""
+    import torch
+    from tile_fusion_b200 import sw_gcn  # noqa: F401
+    n = 100_000_000
+    codes, exponents = torch.ops.sw_gcn.pack8(torch.ones(1, 1, device="cuda"))
+    g = torch.full((n, 8), 1 / 3000.5, device="cuda", dtype=torch.float16)
+    one = codes.new_full((n, 32), int(codes[0, 0]))
+    got = torch.ops.sw_gcn.weight_grad8(g, one, exponents[0, 0].expand(n, 1).contiguous())
+    want = n * g[0, 0].double().item()
+    off = (got.double() / want - 1).abs().max().item()
+    assert off <= U["float16"] + 1e-4, off

@@ -3,12 +3,15 @@
 //
 //   * The rows are cut into as many ranges as the device holds CTAs; each adds up a tile of 128 x 256 or 256 x 128 sums (which of
 //     the two: whatever reads less), and a second launch adds the ranges' tiles in order.
-//   * Four teams of four warps (six for gradients in 16 bits) each turn 16 rows at a time into 16-bit operands in shared memory, row by row as they lie (MN-major,
-//     128-byte swizzle: nothing is transposed), while further rows are on their way; one warp issues tcgen05.mma.  (All warps on the
-//     same 32 rows wait for one another in every step: 500 009 rows, 47 x 256 bf16: 127 us.)  A value of X is seven bits and a power of two, exact in bf16.  G in fp32 is three bf16 planes (24 bits, exact), in
-//     fp16 two (exact), in bf16 one.  So products lose nothing.
+//   * Four teams of four warps (six for gradients in 16 bits) each turn 16 rows at a time into 16-bit operands in shared memory, row by
+//     row as they lie (MN-major, 128-byte swizzle: nothing is transposed), while further rows are on their way; one warp issues
+//     tcgen05.mma.  (All warps on the same 32 rows wait for one another in every step: 500 009 rows, 47 x 256 bf16: 127 us.)
+//   * A value of X is seven bits and a power of two, exact in bf16.  G in fp32 is three bf16 planes (24 bits, exact), in fp16 two
+//     (exact), in bf16 one.  So products lose nothing.
 //   * The tensor core cuts off what it adds to an accumulator, 2e-8 of the sum each time: for fp32 after 128 rows (24 additions)
 //     the accumulator, one of two, is read and added in registers, where sums round.
+// Bound by the issue slots of the warps that make the operands.  500 009 rows, 47 x 256 bf16: 78 us, 2.3 TB/s; 2 449 029 rows, 256 x 100
+// fp32: 649 us, 4.3 TB/s (three planes of G to make).
 // All waits are bounded: where one runs out the CTA's sums, and with them the result, become NaN.
 #include <algorithm>
 #include <string>
@@ -23,8 +26,9 @@ namespace tfk {
 namespace {
 
 // Teams of four warps.  Gradients in 16 bits (one or two planes) leave their sums in tensor memory to the end: 2e-8 of the sum for each
-// of at most a few thousand additions is far below the 2^-9 or 2^-12 that the result is rounded to, and warps that hold no sums
+// of at most 4 096 additions (kWgStayRows) is 1e-4, where the result is rounded to 2^-8 or 2^-11 = 5e-4, and warps that hold no sums
 // are small enough for six teams.
+constexpr int kWgStayRows = 32768;
 constexpr int kWgTeam = 128, kWgMaxTeams = 6;
 __host__ __device__ constexpr int wg_teams(int planes) { return planes == 3 ? 4 : 6; }
 __host__ __device__ constexpr int wg_threads(int planes, bool ring) { return kWgTeam * wg_teams(planes) + 32 * (ring ? 2 : 1); }
@@ -407,7 +411,8 @@ WgPlan wg_plan(int m, int na, int nb, int dtype) {
              : wide.tiles_a * wide.tiles_b > tall.tiles_a * tall.tiles_b || read(tall) < read(wide) ? tall
                                                                                                        : wide;
   // one CTA to an SM; a range of fewer than 128 rows spends its time on the result
-  const int parts = std::max(1, std::min(148 / (p.tiles_a * p.tiles_b), (m + 127) / 128));
+  int parts = std::max(1, std::min(148 / (p.tiles_a * p.tiles_b), (m + 127) / 128));
+  if (dtype != TF_F32) parts = std::max(parts, (m + kWgStayRows - 1) / kWgStayRows);
   p.rows = ((m + parts - 1) / parts + kWgRows - 1) / kWgRows * kWgRows;
   p.parts = std::max(1, (m + p.rows - 1) / std::max(1, p.rows));
   return p;
