@@ -502,6 +502,13 @@ __global__ void __launch_bounds__(kFewThreads, 1) ce_few_kernel(const CeFewCall 
       P.cta_count[blockIdx.x] = tiles > 0 ? s.count[0] + s.count[1] : 0;
     }
   }
+  // (a wait ran out: the gradients of this CTA's rows are NaN, as its part of dW)
+  if (BACK && s.dead && P.dx)
+    for (int t = 0; t < tiles; ++t) {
+      const long long row0 = ((long long)blockIdx.x + (long long)t * gridDim.x) * kFewRows, at = row0 * P.cols;
+      const int n = (int)min((long long)kFewRows, P.rows - row0) * P.cols;
+      for (int i = tid; i < n; i += kFewThreads) store_value(P.dx, DT, at + i, __int_as_float(0x7fc00000));
+    }
   if (warp == 0) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(s.tmem_base), "n"(512) : "memory");

@@ -9,7 +9,7 @@
 //   Up to 64 classes and 256 columns have kernels of their own (ce_few.cu), which read x once a pass.
 //
 // Types.  bf16 and fp16 operands are multiplied as they are.  The slope is rounded to their type before its products, one
-// rounding of relative size 2^-9 (bf16) or 2^-12 (fp16) of each summand; the sums are fp32.  fp32 operands are split into two fp16
+// rounding of at most 2^-8 (bf16) or 2^-11 (fp16) of each summand; the sums are fp32.  fp32 operands are split into two fp16
 // planes behind a power of two that brings the largest finite value to [2^14, 2^15): 22 bits of every value within 2^-27 of the
 // largest, an absolute 2^-39 of the largest below.  The slope of fp32 operands is two planes too.
 // A slope lies in [-1, 1]; in fp16 it is held times 2^14, so that one of 2^-29 still has all its bits.
@@ -587,7 +587,6 @@ extern "C" int tf_linear_ce_bwd(const void *x, long long ld_x, const void *w, lo
       ce_few_sum_kernel<<<(vocab * cols + 31) / 32, 256, 0, s>>>(sp.parts_w, ce_few_ctas(rows), vocab * cols, &sp.h->unscale_slope, dw, dtype);
       e = cudaGetLastError();
     }
-    if (e == cudaSuccess) e = ce_lost(sp.h, dx, (long long)rows * cols, dw, (long long)vocab * cols, dtype, s);
     return e == cudaSuccess ? TF_OK : ce_fail(who, e);
   }
   e = ce_planes(sp, x, ld_x, w, ld_w, dtype, rows, cols, vocab, target, ignore_index, nullptr, s);
