@@ -426,7 +426,7 @@ CeSpace ce_space(char *base, int rows, int cols, int vocab, int dtype, bool back
     if (f32) s.slope_lo = (unsigned short *)take(2ll * rows * s.ld_slope);
     s.cut_x = ce_cut(rows, cols, s.piece, true);
     s.cut_w = ce_cut(s.piece, cols, rows, true);
-    const long long ld_sum = up(cols, 4);
+    const long long ld_sum = up(cols, 8);
     if (s.cut_x || pieces > 1) s.parts_x = (float *)take(4ll * plane_gemm_splits(s.piece, s.cut_x) * rows * ld_sum);
     if (s.cut_w) s.parts_w = (float *)take(4ll * plane_gemm_splits(rows, s.cut_w) * s.piece * ld_sum);
   }
@@ -592,7 +592,7 @@ extern "C" int tf_linear_ce_bwd(const void *x, long long ld_x, const void *w, lo
   e = ce_planes(sp, x, ld_x, w, ld_w, dtype, rows, cols, vocab, target, ignore_index, nullptr, s);
   if (e != cudaSuccess) return ce_fail(who, e);
   const int sms = sm_count();
-  const long long ld_sum = up(cols, 4), ld_w16 = sp.copy_w ? sp.ldp : ld_w;
+  const long long ld_sum = up(cols, 8), ld_w16 = sp.copy_w ? sp.ldp : ld_w;
   const unsigned short *w_hi = sp.copy_w ? sp.w_hi : (const unsigned short *)w;
   for (int v0 = 0; v0 < vocab; v0 += sp.piece) {
     const int nv = std::min(sp.piece, vocab - v0);

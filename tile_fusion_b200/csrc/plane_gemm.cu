@@ -273,7 +273,7 @@ plane_gemm_kernel(const __grid_constant__ CUtensorMap tm_ahi, const __grid_const
           const float *x = P.sum_in + ((size_t)tile.split * P.m + row) * P.ld_sum + col;
 #pragma unroll
           for (int c = 0; c < kCols; c += 4)
-            if (col + c < P.n) {  // (sums have rows of whole quads)
+            if (col + c < P.n) {  // (sums have rows of whole eights)
               const float4 q = *reinterpret_cast<const float4 *>(x + c);
               acc[c] += q.x; acc[c + 1] += q.y; acc[c + 2] += q.z; acc[c + 3] += q.w;
             }
@@ -281,8 +281,13 @@ plane_gemm_kernel(const __grid_constant__ CUtensorMap tm_ahi, const __grid_const
         if (EPI != kPgTurned && P.sum_out) {
           float *x = P.sum_out + ((size_t)tile.split * P.m + row) * P.ld_sum + col;
 #pragma unroll
-          for (int c = 0; c < kCols; c += 4)
-            if (col + c < P.n) *reinterpret_cast<float4 *>(x + c) = make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
+          for (int c = 0; c < kCols; c += 8)
+            if (col + c < P.n) {
+              Pack<float, 8> q;
+#pragma unroll
+              for (int k = 0; k < 8; ++k) q.v[k] = acc[c + k];
+              store_raw<float, 8>(x + c, q);
+            }
         } else {
 #pragma unroll
           for (int c = 0; c < kCols; ++c) acc[c] = acc[c] * scale_a * scale_b;

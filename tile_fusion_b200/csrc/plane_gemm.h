@@ -25,7 +25,8 @@ struct PlaneGemmCall {
   // D is multiplied by the powers of two at these addresses (device; null: 1)
   const float *scale_a = nullptr, *scale_b = nullptr;
   // kPlaneStore: out[m][ld_out] of out_dtype; sum_in: fp32 [m][ld_sum] added before scaling; sum_out: the unscaled sums go there
-  // instead of `out`.  split_slices > 0: K is cut every so many slices of 64, and cut s has the sums at s * m * ld_sum.
+  // instead of `out` (ld_sum a multiple of 8, 32-byte aligned).  split_slices > 0: K is cut every so many slices of 64, and cut s
+  // has the sums at s * m * ld_sum.
   void *out = nullptr;
   int out_dtype = 0;
   long long ld_out = 0;
