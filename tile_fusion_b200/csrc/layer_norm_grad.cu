@@ -6,8 +6,9 @@
 // thread's columns stay the same: the weight is read once, and the sums over rows of dw and db stay in registers until the end,
 // where they are joined in shared memory; a second launch adds the CTAs' sums in order, so results don't depend on scheduling.
 //   Up to 512 columns a row belongs to eight lanes or a warp, and the next row is on its way in registers.
-// Wider rows belong to a CTA (two sums to each column take the registers: 60 000 x 640 bf16 53 us, 130 with a warp to a row), R at a time so that a barrier serves them all, and come through
-// shared memory with asynchronous copies two turns ahead; a thread copies what it alone reads, so copies need no barrier.
+// Wider rows belong to a CTA (two sums to each column take the registers: 60 000 x 640 bf16 53 us, 130 with a warp to a row), R at a
+// time so that a barrier serves them all, and come through shared memory with asynchronous copies two turns ahead; a thread copies what
+// it alone reads, so copies need no barrier.
 // Sums are fp32 whatever the values' type.
 //   120 001 x 256 fp32: 66 us (5.6 TB/s); 16 384 x 4 096 bf16: 85 (4.7, issue slots); 50 021 x 602 fp32 from 8 bits: 66 (4.1).
 #include <algorithm>
