@@ -95,6 +95,23 @@ def test_pieces_and_reductions(built_lib, n, d, v, dtype, reduction):
     near(dw, ww, U[dtype])
 
 
+@pytest.mark.parametrize("n,d,v,dtype", [(20_000, 41, 7_000, "float32"), (20_000, 63, 15_000, "bfloat16"), (20_000, 300, 100, "float32"), (19_001, 129, 301, "float16")])
+def test_rows_of_gradients_that_start_anywhere(built_lib, n, d, v, dtype):
+    """Enough tiles that no sum is cut, so that the products store the gradients themselves; the first two in pieces of classes.
+
+    A mean over 19 001 rows makes gradients of 1e-6, below fp16's smallest normal number 2^-14, where its steps are 2^-24 whatever the
+    value: a result is off by half of that, 2^-25, besides its relative part; over all of them by 2^-25 sqrt(their number) at most."""
+    import torch
+    x, w, target = make(n, d, v, dtype)
+    got = run(x, w, target)
+    want = reference(x, w, target)
+    assert abs(got[0].item() - want[0].item()) <= 2e-5
+    for g, r in zip(got[1:], want[1:]):
+        off, steps = (g.double() - r).norm().item(), 2.0 ** -25 * math.sqrt(r.numel()) if dtype == "float16" else 0.0
+        assert off <= (2 * U[dtype] + 2e-5) * r.norm().item() + steps, off / r.norm().item()
+    torch.cuda.empty_cache()
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_rows_that_do_not_count_reach_nothing(built_lib, dtype):
     import torch
