@@ -133,3 +133,20 @@ def test_weight_gradient_of_many_rows_of_one_sign(built_lib):
     want = n * g[0, 0].double().item()
     off = (got.double() / want - 1).abs().max().item()
     assert off <= U["float16"] + 1e-4, off
+
+
+@pytest.mark.parametrize("cols", [256, 250])
+def test_mask_of_8_bits(built_lib, cols):
+    """More than 2^31 codes: the gradient behind a ReLU, and the layer's codes, at the first rows and the last."""
+    import torch
+    from tile_fusion_b200 import dense_ops, sw_gcn  # noqa: F401
+    n = 2 ** 31 // 256 + 1000
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    codes = torch.randint(-1, 2, (n, 256), generator=gen, device="cuda", dtype=torch.int8)
+    grad = torch.empty(n, cols, device="cuda", dtype=torch.bfloat16).normal_(generator=gen)
+    want = [torch.where(c[:, :cols] != 0, g, torch.zeros_like(g)) for c, g in zip(codes.split(1 << 20), grad.split(1 << 20))]
+    dense_ops.relu_grad8_(grad, codes)
+    for got, w in zip(grad.split(1 << 20), want):
+        assert torch.equal(got, w)
+    del want
+    torch.cuda.empty_cache()

@@ -172,3 +172,19 @@ def test_refusals(built_lib):
                     (ops.weight_grad8, (x[:4], codes, exps)), (ops.weight_grad8, (x.double(), codes, exps)), (ops.weight_grad8, (x, codes, exps.int()))):
         with pytest.raises(ValueError):
             f(*args)
+
+
+@pytest.mark.parametrize("dtype", list(U))
+@pytest.mark.parametrize("n,d", [(1, 1), (37, 33), (500, 32), (333, 602), (64, 256), (70_001, 30), (3, 5000)])
+def test_mask(built_lib, dtype, n, d):
+    """relu_grad8_ alone: a gradient stays, bit by bit, where the packed value was positive, and is zero elsewhere, infinities and NaN among both."""
+    import torch
+    from tile_fusion_b200 import dense_ops, sw_gcn  # noqa: F401
+    x, g = data(n, d, dtype, n), data(n, d, dtype, d)
+    x[n // 2, d // 2] = 1e-7  # (rounds to zero)
+    g[n // 2, d // 2], g[0, 0] = float("inf"), float("nan")
+    codes = torch.ops.sw_gcn.pack8(x, True)[0]
+    full = torch.as_strided(codes, (n, -(-d // 32) * 32), (-(-d // 32) * 32, 1))
+    want = torch.where(x > 0, g, torch.zeros_like(g))
+    got = dense_ops.relu_grad8_(g.clone(), full)
+    assert torch.equal(got.view(torch.uint8), want.view(torch.uint8))

@@ -146,7 +146,7 @@ unpack8_flat_kernel(const signed char *__restrict__ codes, int ld_codes, const u
 // grad (in place) where the packed value was positive, zero elsewhere.
 template <class T, int N>
 __global__ void __launch_bounds__(kPackThreads)
-mask8_kernel(const signed char *__restrict__ codes, int ld_codes, int rows, int cols, T *__restrict__ grad, long long ld) {
+mask8_kernel(const signed char *__restrict__ codes, long long ld_codes, int rows, int cols, T *__restrict__ grad, long long ld) {
   for (Walk<false> w(cols / N); w.in(rows);) {
     long long to[kPackUnroll];
     Pack<signed char, N> c[kPackUnroll];
