@@ -236,3 +236,21 @@ def test_refusals(built_lib):
     (g,) = torch.autograd.grad(loss, x, create_graph=True)
     with pytest.raises(RuntimeError):
         g.sum().backward()
+
+
+# the one class of a part, a part among others, all classes; few classes and many
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,d,v,first,last", [(300, 64, 40, 39, 40), (300, 64, 65, 64, 65), (300, 64, 129, 128, 129), (300, 64, 257, 256, 257), (200, 40, 1000, 64, 192),
+                                              (9000, 24, 20_001, 19_968, 20_001), (50, 48, 200, 0, 200)])
+def test_classes_that_are_nan_are_seen(built_lib, dtype, n, d, v, first, last):
+    """A NaN among a row's logits makes its loss NaN, wherever the row's target is; rows that do not count have none."""
+    import torch
+    from tile_fusion_b200 import sw_gcn  # noqa: F401
+    x, w, t = make(n, d, v, dtype)
+    t[t >= first] = 0
+    w[first:last] = float("nan")
+    loss = torch.ops.sw_gcn.linear_cross_entropy(x, w, t, -100, "none")
+    assert loss[t >= 0].isnan().all() and (loss[t < 0] == 0).all()
+    assert torch.ops.sw_gcn.linear_cross_entropy(x, w, t).isnan()
+    _, dx, _ = run(x, w, t)
+    assert dx[t >= 0].isnan().all()

@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(256) ce_join_kernel(const float2 *__restrict__
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, row = blockIdx.x * 32 + lane;
   float m = -INFINITY, s = 0.f;
   auto add = [&](float2 p) {
-    const float top = fmaxf(m, p.x);
+    const float top = max3(m, p.x, p.x);  // (a NaN stays one)
     if (top == -INFINITY) return;  // nothing yet
     s = s * exp2f(m - top) + p.y * exp2f(p.x - top);
     m = top;

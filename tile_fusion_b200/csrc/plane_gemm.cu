@@ -365,8 +365,9 @@ plane_gemm_kernel(const __grid_constant__ CUtensorMap tm_ahi, const __grid_const
           for (int c = 0; c < kCols; ++c) {
             acc[c] = acc[c] * to_logit * more;
             if (col + c >= P.n) acc[c] = -INFINITY;
-            top = fmaxf(top, acc[c]);
           }
+#pragma unroll
+          for (int c = 0; c < kCols; c += 2) top = max3(top, acc[c], acc[c + 1]);  // (a NaN if one of them is: a part of NaN alone is not an empty one)
           if (want >= 0) {
             float l = 0.f;
 #pragma unroll
@@ -376,7 +377,7 @@ plane_gemm_kernel(const __grid_constant__ CUtensorMap tm_ahi, const __grid_const
           }
           const float top2 = top * kLog2e;
           float sum[4] = {0.f, 0.f, 0.f, 0.f};
-          if (top > -INFINITY || top != top) {
+          if (top != -INFINITY) {
 #pragma unroll
             for (int c = 0; c < kCols; ++c) sum[c & 3] += ex2(fmaf(acc[c], kLog2e, -top2));
           }
