@@ -206,6 +206,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) ce_few_kernel(const CeFewCall 
     double loss = 0.;
     int count = 0, job = 0;
     float unscale_w = 1.f, unscale_p = 1.f;
+    const bool whole_dx = P.cols % 8 == 0 && (reinterpret_cast<uintptr_t>(P.dx) & (DT == TF_F32 ? 31 : 15)) == 0;  // (32 or 16 bytes a store)
     if (tiles > 0 && wait(&s.w_full, 0)) unscale_w = s.unscale_w;
     if (BACK) unscale_p = __ldg(P.unscale);
     float scale_of[2];
@@ -314,7 +315,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) ce_few_kernel(const CeFewCall 
 #pragma unroll
           for (int c = 0; c < 32; ++c) v[c] = v[c] * unscale_p * unscale_w;
           const long long at = row * P.cols + col;
-          if (P.cols % 8 == 0) {  // whole sectors at a time
+          if (whole_dx) {  // whole sectors at a time
 #pragma unroll
             for (int c = 0; c < 32; c += 8) {
               if (col + c >= P.cols) break;
