@@ -254,3 +254,25 @@ def test_classes_that_are_nan_are_seen(built_lib, dtype, n, d, v, first, last):
     assert torch.ops.sw_gcn.linear_cross_entropy(x, w, t).isnan()
     _, dx, _ = run(x, w, t)
     assert dx[t >= 0].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,v", [(100, 40), (100, 300), (9000, 40), (9000, 300)])
+@pytest.mark.parametrize("size", [1e-36, 1e-30])
+def test_tiny_gradients_of_rows(built_lib, dtype, n, v, size):
+    """A gradient to each row, all of them tiny and some zero: the power of two that brings the largest to one is held in the range.
+
+    fp32 and bf16: as elsewhere, in the types' normal range.  fp16: results are below half of its smallest number."""
+    import torch
+    x, w, t = make(n, 64, v, dtype)
+    g = size * torch.linspace(1, 4, n, device="cuda")
+    g[::7] = 0
+    _, dx, dw = run(x, w, t, "none", g)
+    _, wx, ww = reference(x, w, t, "none", g)
+    assert (dx[::7] == 0).all()
+    if dtype == "float16":
+        assert (dx == 0).all() and (dw == 0).all()
+    else:
+        scale = 1 / size  # (squares of 1e-36 are no numbers of fp32; the norms are fp64's)
+        near(dx.double() * scale, wx * scale, U[dtype])
+        near(dw.double() * scale, ww * scale, U[dtype])

@@ -34,7 +34,7 @@ namespace {
 constexpr long long kCeSlopeBytes = 256ll << 20;
 constexpr int kCeWaitLimit = 1 << 22;
 constexpr float kLn2 = 0.69314718055994531f;
-constexpr float kSlopeUnit = 16384.f;  // of fp16 slopes
+constexpr float kSlopeUnit = 16384.f;  // of fp16 slopes: 2^14
 
 struct CeHeader {            // at the start of the workspace, zeroed by every call
   unsigned top_grad;         // bits of the largest finite |gradient of a row's loss|
@@ -258,7 +258,8 @@ __global__ void __launch_bounds__(256) ce_count_kernel(const long long *__restri
 __device__ __forceinline__ float2 ce_scales(int reduction, float unit, unsigned top_grad, int counted, const float *grad) {
   float by = unit, back = 1.f / unit;
   if (reduction == 0) {
-    const int e = top_grad ? min(126, max(-126, -((int)(top_grad >> 23) - 126))) : 0;
+    // (unit * 2^e stays a number, or rows of zero gradients would become NaN)
+    const int e = top_grad ? min(unit == 1.f ? 126 : 112, max(-126, -((int)(top_grad >> 23) - 126))) : 0;
     by *= ce_power(e);
     back *= ce_power(-e);
   } else back *= grad[0] / (reduction == 1 ? (float)max(counted, 1) : 1.f);
