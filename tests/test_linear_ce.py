@@ -276,3 +276,18 @@ def test_tiny_gradients_of_rows(built_lib, dtype, n, v, size):
         scale = 1 / size  # (squares of 1e-36 are no numbers of fp32; the norms are fp64's)
         near(dx.double() * scale, wx * scale, U[dtype])
         near(dw.double() * scale, ww * scale, U[dtype])
+
+
+@pytest.mark.parametrize("v", [40, 300])
+def test_rows_of_zeros_beside_huge_ones(built_lib, v):
+    """fp32 operands of 2^100 and rows of zeros, whose logits are zero: their loss is log(classes), their gradient (1 / classes - onehot) @ w."""
+    import torch
+    x, w, t = make(64, 32, v, "float32", ignored=0)
+    x, w = x * 2.0 ** 100, w * 2.0 ** 100
+    x[::2] = 0
+    g = torch.zeros(64, device="cuda")
+    g[::2] = 1
+    loss, dx, _ = run(x, w, t, "none", g)
+    want, wx, _ = reference(x[::2], w, t[::2], "none", 1.0)
+    assert (loss[::2].double() - want).abs().max().item() <= 2e-5
+    near(dx[::2], wx, U["float32"])

@@ -260,12 +260,12 @@ __global__ void __launch_bounds__(kFewThreads, 1) ce_few_kernel(const CeFewCall 
         tmem_load16(v, lanes + b * 64 + side * 16);
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         few_arrive(&s.log_empty[b]);
-        const float in2 = unscale_x * unscale_w * kFewLog2e;  // (powers of two: their product may leave the range only where all logits do)
+        const float in2 = unscale_w * kFewLog2e;  // (one power of two at a time: a logit of zero stays zero where their product leaves the range)
         const int mine = in && target >= side * 16 && target < side * 16 + 16 ? (int)target - side * 16 : -1;
         const unsigned to = at_p + b * slope_bytes + in_tile * 128;
 #pragma unroll
         for (int c = 0; c < 16; ++c) {
-          const float e = few_ex2(fmaf(v[c], in2, -lse2)) - (c == mine ? 1.f : 0.f);
+          const float e = few_ex2(fmaf(PLANES == 2 ? v[c] * unscale_x : v[c], in2, -lse2)) - (c == mine ? 1.f : 0.f);
           v[c] = by == 0.f || side * 16 + c >= P.vocab ? 0.f : e * by;  // (a row that does not count stays zero whatever it holds)
         }
 #pragma unroll
