@@ -188,3 +188,37 @@ def test_mask(built_lib, dtype, n, d):
     want = torch.where(x > 0, g, torch.zeros_like(g))
     got = dense_ops.relu_grad8_(g.clone(), full)
     assert torch.equal(got.view(torch.uint8), want.view(torch.uint8))
+
+
+@pytest.mark.parametrize("dtype", list(U))
+@pytest.mark.parametrize("na,nb", [(20, 64), (47, 256), (300, 40)])
+def test_gradients_that_are_not_finite(built_lib, dtype, na, nb):
+    """An infinity in G makes the sums that it takes part in infinite (NaN where it meets a zero, another sign or a NaN), as the formula has it."""
+    import torch
+    from tile_fusion_b200 import sw_gcn  # noqa: F401
+    x, g = data(150, nb, "float32"), data(150, na, dtype, 1)
+    g[3, 2], g[7, 5], g[140, 5], g[60, 9], g[61, 10] = float("inf"), float("-inf"), float("inf"), float("nan"), float("inf")
+    x[61, :3] = 0
+    codes, exps = torch.ops.sw_gcn.pack8(x)
+    got = torch.ops.sw_gcn.weight_grad8(g, codes, exps).double()
+    want = g.double().t() @ torch.ops.sw_gcn.unpack8(codes, exps).double()
+    bad = ~want.isfinite()
+    assert bad.any(1).sum().item() == 4 and torch.equal(got.isnan(), want.isnan()) and torch.equal(got.isinf(), want.isinf())
+    assert torch.equal(got[want.isinf()], want[want.isinf()])
+    off = (got - want)[~bad].norm().item()
+    assert off <= (U[dtype] + 5e-6) * want[~bad].norm().item()
+
+
+def test_gradients_next_to_the_end_of_fp32(built_lib):
+    """Values beyond bf16's largest that are numbers."""
+    import torch
+    from tile_fusion_b200 import sw_gcn  # noqa: F401
+    x = data(40, 32, "float32").sign() * 2.0 ** -20
+    g = data(40, 20, "float32", 2)
+    g[:, 3] = torch.finfo(torch.float32).max
+    g[5, 4] = -3.4e38
+    codes, exps = torch.ops.sw_gcn.pack8(x)
+    got = torch.ops.sw_gcn.weight_grad8(g, codes, exps).double()
+    want = g.double().t() @ x.double()
+    for c in range(20):  # (columns of their own size each)
+        assert (got[c] - want[c]).norm().item() <= 5e-6 * 40 ** 0.5 * 2.0 ** -20 * g[:, c].double().norm().item()

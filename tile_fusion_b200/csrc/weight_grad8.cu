@@ -109,21 +109,43 @@ template <class T, bool WHOLE, class At> __device__ __forceinline__ void wg_load
 #pragma unroll
   for (int i = 0; i < W; ++i) v[i] = to_float(reinterpret_cast<const T &>(a.v[i]));
 }
-// They as bf16 operands, one plane after the other (each what the planes before leave).
-template <int PLANES, int W> __device__ __forceinline__ void wg_planes(float (&g)[W], unsigned to, int plane) {
+// They as bf16 operands, one plane after the other (each what the planes before leave).  FAR: some may be infinite or beyond bf16's largest
+// number: what the first plane keeps is cut off, not rounded, so that a number does not become an infinity, and an infinity leaves nothing.
+constexpr float kWgFar = 0x1.fep127f;
+template <int PLANES, int W, bool FAR = false> __device__ __forceinline__ void wg_planes(float (&g)[W], unsigned to, int plane) {
 #pragma unroll
   for (int p = 0; p < PLANES; ++p) {
     unsigned u[W / 2];
 #pragma unroll
     for (int k = 0; k < W / 2; ++k) {
-      u[k] = pack_pair(g[2 * k], g[2 * k + 1], false);
+      float a = g[2 * k], b = g[2 * k + 1];
+      if (FAR && p == 0) {
+        if (a == a) a = __uint_as_float(__float_as_uint(a) & 0xffff0000u);  // (a NaN stays one)
+        if (b == b) b = __uint_as_float(__float_as_uint(b) & 0xffff0000u);
+      }
+      u[k] = pack_pair(a, b, false);
       if (p < PLANES - 1) {
         g[2 * k] -= __uint_as_float(u[k] << 16);
         g[2 * k + 1] -= __uint_as_float(u[k] & 0xffff0000u);
+        if (FAR && p == 0) {
+          if (isinf(a)) g[2 * k] = 0.f;
+          if (isinf(b)) g[2 * k + 1] = 0.f;
+        }
       }
     }
     if constexpr (W == 8) asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + p * plane), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]));
     else asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(to + p * plane), "r"(u[0]), "r"(u[1]));
+  }
+}
+
+// A chunk's rows of a slice, some of them infinite or beyond bf16's largest number, as planes.
+template <class T, int PLANES, bool WHOLE, class At, class Ld>
+__device__ __noinline__ void wg_far_rows(At at, Ld ld, int rows, int first, int step, int n, unsigned to, int chunk, int plane) {
+#pragma unroll 1
+  for (int r = first; r < rows; r += step) {
+    float g[16 / sizeof(T)];
+    wg_load<T, WHOLE>(at + r * ld, n, g);
+    wg_planes<PLANES, 16 / (int)sizeof(T), true>(g, to + (unsigned)(r * 128 + ((chunk ^ r) & 7) * 16), plane);
   }
 }
 
@@ -262,6 +284,7 @@ __global__ void __launch_bounds__(wg_threads(PLANES, RING), 1) weight_grad8_kern
     auto convert = [&](unsigned base, auto pg, auto ld, auto pc, auto pe, int rows) {
       pg += (a0 + chunk_g * W) * (int)sizeof(T);
       auto gradient = [&](auto whole) {
+        float top = 0.f;
 #pragma unroll 4
         for (int r = first_g; r < kWgRows; r += step_g) {
           const bool here = RING || r < rows;
@@ -277,8 +300,14 @@ __global__ void __launch_bounds__(wg_threads(PLANES, RING), 1) weight_grad8_kern
           if (!here)
 #pragma unroll
             for (int k = 0; k < W; ++k) g[k] = 0.f;
+          if constexpr (PLANES > 1)
+#pragma unroll
+            for (int k = 0; k < W; k += 2) top = max3_abs_numbers(top, g[k], g[k + 1]);
           wg_planes<PLANES, W>(g, to, kPlane);
         }
+        // (rare: the rows again, in a call of its own, so that what they need takes no registers above)
+        if constexpr (PLANES > 1)
+          if (top > kWgFar) wg_far_rows<T, PLANES, decltype(whole)::value>(pg, ld, RING ? kWgRows : min(rows, kWgRows), first_g, step_g, n_g, base + to_g, at_g, kPlane);
       };
       if (P.whole_g) gradient(std::true_type());
       else gradient(std::false_type());
