@@ -222,3 +222,15 @@ def test_gradients_next_to_the_end_of_fp32(built_lib):
     want = g.double().t() @ x.double()
     for c in range(20):  # (columns of their own size each)
         assert (got[c] - want[c]).norm().item() <= 5e-6 * 40 ** 0.5 * 2.0 ** -20 * g[:, c].double().norm().item()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_positive_values_far_below_their_groups(built_lib, dtype):
+    """The smallest subnormals beside values of 2^8 and more: scaled, they are nothing, but they were positive."""
+    import torch
+    x = torch.zeros(6, 64, device="cuda", dtype=getattr(torch, dtype))
+    tiny = 2.0 ** (-149 if dtype == "float32" else -133)
+    for i, big in enumerate((1.0, 2.0 ** 7, 2.0 ** 8, 2.0 ** 30, 2.0 ** 126, 2.0 ** 127)):
+        x[i, 0], x[i, 1], x[i, 2], x[i, 33] = big, tiny, -tiny, tiny
+    check(x, True)
+    check(x, False)
