@@ -186,3 +186,25 @@ def test_refusals(built_lib):
             call(*args)
     with pytest.raises(_lib.TileFusionError, match="columns"):
         call(torch.zeros(2, 16_385, device="cuda"))
+
+
+def test_tangents_and_traces(built_lib):
+    """A forward-mode tangent is refused, not dropped, whether or not anything requires a gradient; a trace records the operator."""
+    import torch
+    from torch.autograd import forward_ad
+    from tile_fusion_b200 import sw_gcn  # noqa: F401
+    ops = torch.ops.sw_gcn
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    x, z = torch.randn(2, 30, 40, generator=gen, device="cuda")
+    w, b = torch.randn(2, 40, generator=gen, device="cuda")
+    y, yz = ops.layer_norm(x, w, b), ops.layer_norm(z, w, b)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for args in ((dual(x), w, b), (x, dual(w), b), (x, w, dual(b))):
+            with pytest.raises(RuntimeError):
+                ops.layer_norm(*args)
+            with pytest.raises(RuntimeError), torch.no_grad():
+                ops.layer_norm(*args)
+        assert torch.equal(ops.layer_norm(x, w, b), y)
+    traced = torch.jit.trace(lambda t: ops.layer_norm(t, w, b), (x,))
+    assert torch.equal(traced(x), y) and torch.equal(traced(z), yz)

@@ -291,3 +291,21 @@ def test_rows_of_zeros_beside_huge_ones(built_lib, v):
     want, wx, _ = reference(x[::2], w, t[::2], "none", 1.0)
     assert (loss[::2].double() - want).abs().max().item() <= 2e-5
     near(dx[::2], wx, U["float32"])
+
+
+def test_tangents_and_traces(built_lib):
+    """A forward-mode tangent is refused, not dropped; a trace records the operator."""
+    import torch
+    from torch.autograd import forward_ad
+    from tile_fusion_b200 import sw_gcn  # noqa: F401
+    call = torch.ops.sw_gcn.linear_cross_entropy
+    x, w, t = make(30, 40, 50, "float32")
+    z = make(30, 40, 50, "float32", seed=1)[0]
+    loss, other = call(x, w, t), call(z, w, t)
+    with forward_ad.dual_level():
+        for a, b in ((forward_ad.make_dual(x, torch.ones_like(x)), w), (x, forward_ad.make_dual(w, torch.ones_like(w)))):
+            with pytest.raises(RuntimeError):
+                call(a, b, t)
+        assert torch.equal(call(x, w, t), loss)
+    traced = torch.jit.trace(lambda a: call(a, w, t), (x,))
+    assert torch.equal(traced(x), loss) and torch.equal(traced(z), other)

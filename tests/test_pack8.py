@@ -234,3 +234,26 @@ def test_positive_values_far_below_their_groups(built_lib, dtype):
         x[i, 0], x[i, 1], x[i, 2], x[i, 33] = big, tiny, -tiny, tiny
     check(x, True)
     check(x, False)
+
+
+def test_tangents_and_traces(built_lib):
+    """These operators carry no graph: a forward-mode tangent is refused, not dropped.  A trace records the operators themselves."""
+    import torch
+    from torch.autograd import forward_ad
+    from tile_fusion_b200 import sw_gcn  # noqa: F401
+    ops = torch.ops.sw_gcn
+    x, g = data(20, 40, "float32"), data(20, 8, "float32", 1)
+    codes, exps = ops.pack8(x)
+    value, dw = ops.unpack8(codes, exps), ops.weight_grad8(g, codes, exps)
+    with forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="pack8"):
+            ops.pack8(forward_ad.make_dual(x, torch.ones_like(x)))
+        with pytest.raises(RuntimeError, match="weight_grad8"):
+            ops.weight_grad8(forward_ad.make_dual(g, torch.ones_like(g)), codes, exps)
+        assert torch.equal(ops.unpack8(*ops.pack8(x)), value) and torch.equal(ops.weight_grad8(g, codes, exps), dw)
+    z, h = data(20, 40, "float32", 2), data(20, 8, "float32", 3)
+    traced = torch.jit.trace(lambda x, g: (ops.unpack8(*ops.pack8(x)), ops.weight_grad8(g, *ops.pack8(x))), (x, g))
+    for a, b in ((x, g), (z, h)):
+        codes, exps = ops.pack8(a)
+        got = traced(a, b)
+        assert torch.equal(got[0], ops.unpack8(codes, exps)) and torch.equal(got[1], ops.weight_grad8(b, codes, exps))

@@ -29,12 +29,13 @@ row).  The loss is fp32.
 
 The operators take fp32, bf16 and fp16 CUDA tensors whose last dimension is contiguous or is made so, run on the current
 stream of the tensors' device, take their workspaces from torch's allocator, and can be captured into CUDA graphs.  They
-are differentiable once.  (A captured backward pass belongs in ``torch.autograd.grad``, or to leaves of which no eager graph is
+are differentiable once, backwards; a forward-mode tangent is refused.  (A captured backward pass belongs in ``torch.autograd.grad``, or to leaves of which no eager graph is
 alive: autograd accumulates into a leaf on the stream of the graph that made its accumulator, which a capture cannot wait for.)
 """
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -46,6 +47,16 @@ _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
+
+
+def _tangents():
+    """Whether forward-mode tangents may go with the tensors: autograd's functions refuse those, where plain calls would drop them."""
+    return forward_ad._current_level >= 0
+
+
+def _refuse_tangent(name, t):
+    if forward_ad.unpack_dual(t).tangent is not None:
+        raise RuntimeError(f"sw_gcn.{name} carries no graph: a forward-mode tangent would be lost")
 
 
 def _on_device_of_first(f):
@@ -155,6 +166,8 @@ def pack8(x, relu=False):
         _check_values("pack8", "x", x)
     if x.dim() != 2 or x.shape[1] == 0:
         raise ValueError(f"sw_gcn.pack8: x must be a matrix of at least one column, not {tuple(x.shape)}")
+    if _tangents():
+        _refuse_tangent("pack8", x)
     codes, exponents = _pack(_rows(x), relu)
     d = x.shape[1]
     return (codes if codes.shape[1] == d else codes[:, :d]), exponents
@@ -174,6 +187,8 @@ def weight_grad8(grad, codes, exponents):
     _check_values(name, "grad", grad)
     if grad.dim() != 2 or codes.dim() != 2 or grad.shape[0] != codes.shape[0] or grad.shape[1] == 0:
         raise ValueError(f"sw_gcn.{name}: grad {tuple(grad.shape)} and codes {tuple(codes.shape)} do not chain")
+    if _tangents():
+        _refuse_tangent(name, grad)
     nb = codes.shape[1]
     codes, exponents, ld = _packed(name, codes, exponents)
     _same_device(name, grad, codes)
@@ -256,7 +271,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, checkpoint=False):
     if not (_fine(x, d) and last and last[0] > 0 and (weight is None or (_fine(weight, d) and weight.shape == last))
             and (bias is None or (_fine(bias, d) and bias.shape == last and (weight is None or weight.dtype == bias.dtype)))):
         _refuse_layer_norm(x, weight, bias)
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
+    if _tangents() or torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
         return _LayerNorm.apply(x, weight, bias, eps, checkpoint)
     w = weight.contiguous() if weight is not None else None
     b = bias.contiguous() if bias is not None else None
@@ -335,7 +350,7 @@ def linear_cross_entropy(x, weight, target, ignore_index=-100, reduction="mean")
             and weight.dim() == 2 and x.dim() > 0 and x.shape[-1] == weight.shape[1] and weight.numel() > 0
             and target.dtype in (torch.int64, torch.int32) and target.shape == x.shape[:-1]):
         _refuse_linear_cross_entropy(x, weight, target, reduction)
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+    if _tangents() or torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
         return _LinearCrossEntropy.apply(x, weight, target, ignore_index, code)
     loss, _ = _loss_forward(_rows(x), _rows(weight), _classes(target), ignore_index, code)
     return loss if code or target.dim() == 1 else loss.view(target.shape)
