@@ -53,7 +53,7 @@ struct WgParams {
 
 struct WgShared {
   unsigned long long raw_full[kWgMaxRing], raw_empty[kWgMaxRing];
-  unsigned long long full[kWgMaxTeams], empty[kWgMaxTeams], acc_full[2], acc_empty[2];
+  unsigned long long full[kWgMaxTeams], empty[kWgMaxTeams], tail[kWgMaxTeams], acc_full[2], acc_empty[2];
   unsigned tmem_base;
   int dead;
 };
@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(wg_threads(PLANES, RING), 1) weight_grad8_kern
   for (int i = tid; i < kTeams * kStage / 16; i += wg_threads(PLANES, RING)) reinterpret_cast<uint4 *>(smem)[i] = make_uint4(0, 0, 0, 0);
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   if (tid == 0) {
-    for (int i = 0; i < kTeams; ++i) { mbar_init(&s.full[i], kTeamWarps); mbar_init(&s.empty[i], 1); }
+    for (int i = 0; i < kTeams; ++i) { mbar_init(&s.full[i], kTeamWarps); mbar_init(&s.empty[i], 1); mbar_init(&s.tail[i], kTeamWarps); }
     if (RING)
       for (int i = 0; i < P.ring; ++i) { mbar_init(&s.raw_full[i], 1); mbar_init(&s.raw_empty[i], kTeamWarps); }
     for (int i = 0; i < 2; ++i) { mbar_init(&s.acc_full[i], 1); mbar_init(&s.acc_empty[i], kWarps); }
@@ -347,13 +347,16 @@ __global__ void __launch_bounds__(wg_threads(PLANES, RING), 1) weight_grad8_kern
         if (all && !wait(&s.raw_full[rs], raw_ph)) break;
         if (!all) {  // the last rows: the team copies them itself, and zeros behind them (what was there it has read, once its warps have met)
           const int rows = (int)(r1 - row), per = P.ld_codes / kPackGroup;
-          asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(kWgTeam) : "memory");
+          // (its warps meet in bounded waits: one whose wait has run out does not come)
+          arrive(&s.tail[team]);
+          if (!wait(&s.tail[team], 0)) break;
           T *to = reinterpret_cast<T *>(at);
           for (int i = in_team; i < kWgRows * P.na; i += kWgTeam) to[i] = i < rows * P.na ? static_cast<const T *>(P.g)[row * P.na + i] : from_float<T>(0.f);
           for (int i = in_team; i < kWgRows * P.ld_codes; i += kWgTeam) at[P.g_bytes + i] = i < rows * P.ld_codes ? P.codes[row * P.ld_codes + i] : 0;
           for (int i = in_team; i < kWgRows * per; i += kWgTeam)
             at[P.g_bytes + kWgRows * P.ld_codes + i] = (char)(i < rows * per ? P.exps[row * per + i] : 127);
-          asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(kWgTeam) : "memory");
+          arrive(&s.tail[team]);
+          if (!wait(&s.tail[team], 1)) break;
         }
         const unsigned place = ring_place(smem_u32(at));
         convert(stage, place, (unsigned)(P.na * sizeof(T)), place + P.g_bytes, place + P.g_bytes + kWgRows * P.ld_codes, kWgRows);
