@@ -437,7 +437,7 @@ int tf_weight_grad8(const void *g, long long ld_g, int dtype, int na, const sign
  * add nothing to dw, whatever they hold.
  *   work: tf_linear_ce_work_bytes bytes, 256-byte aligned, of the caller's; two calls that may overlap need two.  The calls
  * only enqueue work on `stream`; they allocate nothing and can be captured.  tf_linear_ce_status waits for `stream` and says
- * whether a bounded wait of the last call with this work space ran out (the loss or the gradients are NaN then). */
+ * whether a bounded wait of the last call with this work space ran out (the losses and lse2, or the gradients, are NaN then). */
 long long tf_linear_ce_work_bytes(int rows, int cols, int vocab, int dtype, int backward);
 int tf_linear_ce_fwd(const void *x, long long ld_x, const void *w, long long ld_w, int dtype, const long long *target, int rows,
                      int cols, int vocab, long long ignore_index, int reduction, float *loss, float *lse2, void *work,
@@ -446,6 +446,9 @@ int tf_linear_ce_bwd(const void *x, long long ld_x, const void *w, long long ld_
                      int cols, int vocab, long long ignore_index, int reduction, const float *lse2, const float *grad, void *dx,
                      void *dw, void *work, long long work_bytes, void *stream);
 int tf_linear_ce_status(const void *work, void *stream);
+/* How often a kernel of tf_linear_ce_* or tf_weight_grad8 looks at what it waits for before it gives up: 4 194 304 unless set, 65 536 at
+ * least, or 0, with which every wait gives up at once (for tests of what follows); for the calls of all threads from then on. */
+int tf_dense_set_wait_limit(int polls);
 
 /* ------------------------------------------------------------------------- */
 /* Matrix files                                                               */

@@ -125,3 +125,9 @@ def test_8_bits_of_no_matrix(built_lib):
     from tile_fusion_b200 import sw_gcn  # noqa: F401
     with pytest.raises(ValueError, match="codes"):
         torch.ops.sw_gcn.unpack8(torch.zeros((), dtype=torch.int8), torch.zeros(1, dtype=torch.uint8))
+
+
+def test_wait_limit(L):
+    for polls in (-1, 1, 65535):
+        refused(L.tf_dense_set_wait_limit(polls), "polls")
+    assert L.tf_dense_set_wait_limit(65536) == 0 and L.tf_dense_set_wait_limit(0) == 0 and L.tf_dense_set_wait_limit(1 << 22) == 0

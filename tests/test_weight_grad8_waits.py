@@ -7,6 +7,8 @@ import re
 
 import pytest
 
+from tests.test_warp_waits import WAIT, _offences
+
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "tile_fusion_b200", "csrc")
 WARPS = 4
 
@@ -102,3 +104,11 @@ def test_no_barrier_without_a_limit_among_warps_that_may_leave():
         if n:
             found[name] = n
     assert found == {"ce_few.cu": 1}
+
+
+@pytest.mark.parametrize("source", ["plane_gemm.cu", "ce_few.cu", "weight_grad8.cu"])
+def test_a_warp_leaves_as_one(source):
+    """As for the other kernels (test_warp_waits.py): nothing is decided by a wait's result before the warp has voted on it."""
+    with open(os.path.join(CSRC, source)) as f:
+        text = f.read()
+    assert WAIT.search(text) and _offences(text) == []

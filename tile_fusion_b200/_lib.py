@@ -50,7 +50,7 @@ EXPORTS = [
     "tf_multi_exec", "tf_multi_status", "tf_multi_trace", "tf_partition_layout", "tf_read_matrix", "tf_read_dense_mtx",
     "tf_schedule_unfused_csr", "tf_schedule_reordered_adj", "tf_rcm_order", "tf_permute_csr",
     "tf_layer_norm_fwd", "tf_layer_norm_bwd", "tf_layer_norm_work_floats", "tf_pack8", "tf_unpack8", "tf_relu_grad8",
-    "tf_weight_grad8", "tf_weight_grad8_work_floats", "tf_linear_ce_work_bytes", "tf_linear_ce_fwd", "tf_linear_ce_bwd", "tf_linear_ce_status",
+    "tf_weight_grad8", "tf_weight_grad8_work_floats", "tf_linear_ce_work_bytes", "tf_linear_ce_fwd", "tf_linear_ce_bwd", "tf_linear_ce_status", "tf_dense_set_wait_limit",
 ]
 
 _lib = None
@@ -155,6 +155,7 @@ def lib() -> C.CDLL:
     L.tf_linear_ce_fwd.argtypes = [vp, ll, vp, ll, i, vp, i, i, i, ll, i, vp, vp, vp, ll, vp]
     L.tf_linear_ce_bwd.argtypes = [vp, ll, vp, ll, i, vp, i, i, i, ll, i, vp, vp, vp, vp, vp, ll, vp]
     L.tf_linear_ce_status.argtypes = [vp, vp]
+    L.tf_dense_set_wait_limit.argtypes = [i]
     L.tf_lattice_preview.argtypes = [C.POINTER(Csr), i, i, i, ip, C.POINTER(vp), C.POINTER(vp), C.POINTER(vp), ip]
     _lib = L
     return L

@@ -33,12 +33,11 @@ constexpr int kFewBlock = kFewRows * 128;  // bytes of 64 columns of a tile
 constexpr int kFewMmaWarp = 15;
 __host__ __device__ constexpr int few_drains(bool back) { return back ? 8 : 2; }
 __host__ __device__ constexpr int few_loaders(bool back) { return 15 - few_drains(back); }
-constexpr int kFewWaitLimit = 1 << 22;
 constexpr int kFewRegions = 3;             // accumulators of 128 columns behind two of 64 for the logits
 constexpr float kFewLog2e = 1.4426950408889634f, kFewLn2 = 0.69314718055994531f;
 
 struct FewShared {
-  unsigned long long x_full[2], x_empty[2], w_full, log_full[2], log_empty[2], p_full[2], job_full[kFewRegions], job_empty[kFewRegions];
+  unsigned long long x_full[2], x_empty[2], w_full, log_full[2], log_empty[2], p_full[2], job_full[kFewRegions], job_empty[kFewRegions], drained;
   unsigned top[2][few_loaders(false)];
   float unscale_x[2], unscale_w;
   double loss[2];
@@ -106,6 +105,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) ce_few_kernel(const CeFewCall 
       mbar_init(&s.p_full[i], kDrains);
     }
     mbar_init(&s.w_full, kFewLoaders);
+    mbar_init(&s.drained, 1);
     for (int i = 0; i < kFewRegions; ++i) { mbar_init(&s.job_full[i], 1); mbar_init(&s.job_empty[i], kDrains); }
     s.dead = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) ce_few_kernel(const CeFewCall 
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   bool ok = true;
-  auto wait = [&](unsigned long long *bar, unsigned parity) { return ok = __all_sync(kFull, pair_wait(bar, parity, s.dead, kFewWaitLimit)); };
+  auto wait = [&](unsigned long long *bar, unsigned parity) { return ok = __all_sync(kFull, pair_wait(bar, parity, s.dead, P.wait_limit)); };
 
   if (warp == kFewMmaWarp) {
     // ---- products ----
@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) ce_few_kernel(const CeFewCall 
         idle = 0;
       } else {
         __nanosleep(20);  // (the loop would take the issue slots of the warps that bring tiles)
-        if (++idle <= 64ll * kFewWaitLimit && !*reinterpret_cast<volatile int *>(&s.dead)) continue;
+        if (++idle <= 64ll * P.wait_limit && !*reinterpret_cast<volatile int *>(&s.dead)) continue;
         s.dead = 1;
         ok = false;
       }
@@ -195,6 +195,10 @@ __global__ void __launch_bounds__(kFewThreads, 1) ce_few_kernel(const CeFewCall 
     // the last arrivals on barriers that nobody waits for must be in before the CTA ends
     if (ok)
       for (int t = max(0, tiles - 2); t < tiles; ++t) wait(&s.x_empty[t & 1], (unsigned)(t / 2) & 1u);
+    if (!ok) {  // products still running read shared memory and write tensor memory
+      if (elect_one()) umma_commit(&s.drained);
+      mbar_wait(&s.drained, 0, kInFlightPolls);
+    }
   } else if (BACK ? (warp & 3) < 2 : warp < 2) {
     // ---- rows 32 (warp & 3) .. + 31 of a tile, and (backward) a quarter of the columns ----
     const int quadrant = warp & 3, side = warp >> 2, in_tile = quadrant * 32 + lane;
@@ -506,7 +510,14 @@ __global__ void __launch_bounds__(kFewThreads, 1) ce_few_kernel(const CeFewCall 
       P.cta_count[blockIdx.x] = tiles > 0 ? s.count[0] + s.count[1] : 0;
     }
   }
-  // (a wait ran out: the gradients of this CTA's rows are NaN, as its part of dW)
+  // (a wait ran out: the losses of this CTA's rows are NaN, or their gradients, as its part of dW)
+  if (!BACK && s.dead)
+    for (int t = 0; t < tiles; ++t) {
+      const long long row = ((long long)blockIdx.x + (long long)t * gridDim.x) * kFewRows + tid;
+      if (tid >= kFewRows || row >= P.rows) continue;
+      P.lse2[row] = __int_as_float(0x7fc00000);
+      if (P.row_loss) P.row_loss[row] = P.target[row] == P.ignore ? 0.f : __int_as_float(0x7fc00000);
+    }
   if (BACK && s.dead && P.dx)
     for (int t = 0; t < tiles; ++t) {
       const long long row0 = ((long long)blockIdx.x + (long long)t * gridDim.x) * kFewRows, at = row0 * P.cols;

@@ -13,6 +13,7 @@ struct CeFewCall {
   const long long *target = nullptr;
   long long ignore = 0;
   int *error = nullptr;
+  int wait_limit = 0;
   // forward
   float *lse2 = nullptr, *row_loss = nullptr;    // row_loss or, for each CTA, the sum of its rows' losses and their number
   double *cta_loss = nullptr;

@@ -20,6 +20,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <string>
 
 #include "ce_few.h"
@@ -32,7 +33,6 @@ namespace tfk {
 namespace {
 
 constexpr long long kCeSlopeBytes = 256ll << 20;
-constexpr int kCeWaitLimit = 1 << 22;
 constexpr float kLn2 = 0.69314718055994531f;
 constexpr float kSlopeUnit = 16384.f;  // of fp16 slopes: 2^14
 
@@ -175,13 +175,13 @@ __global__ void __launch_bounds__(256) ce_join_kernel(const float2 *__restrict__
   double loss = 0.;
   int counts = 0;
   if (row < rows) {
-    const float l2 = m + log2f(s);
+    const float l2 = h->error ? __int_as_float(0x7fc00000) : m + log2f(s);  // (a wait ran out: the gradients are lost with the loss)
     lse2[row] = l2;
     const long long t = target[row];
     float l = 0.f;
     if (t != ignore) {
       counts = 1;
-      l = t < 0 || t >= vocab || h->error ? __int_as_float(0x7fc00000) : l2 * kLn2 - target_logit[row];
+      l = t < 0 || t >= vocab ? __int_as_float(0x7fc00000) : l2 * kLn2 - target_logit[row];
     }
     if (row_loss) row_loss[row] = l;
     loss = l;
@@ -459,6 +459,8 @@ cudaError_t ce_lost(const CeHeader *h, void *dx, long long nx, void *dw, long lo
   return cudaGetLastError();
 }
 
+std::atomic<int> wait_limit{1 << 22};
+
 int sm_count() {
   int dev = 0, sms = 148;
   cudaGetDevice(&dev);
@@ -472,6 +474,7 @@ CeFewCall few_call(const CeSpace &sp, const void *x, long long ld_x, const void 
   c.x = x; c.w = w; c.ld_x = ld_x; c.ld_w = ld_w; c.dtype = dtype; c.rows = rows; c.cols = cols; c.vocab = vocab;
   c.target = target; c.ignore = ignore;
   c.error = &sp.h->error;
+  c.wait_limit = dense_wait_limit();
   return c;
 }
 
@@ -489,6 +492,8 @@ cudaError_t ce_planes(const CeSpace &sp, const void *x, long long ld_x, const vo
 }
 
 }  // namespace
+
+int dense_wait_limit() { return wait_limit.load(std::memory_order_relaxed); }
 
 }  // namespace tfk
 
@@ -542,7 +547,7 @@ extern "C" int tf_linear_ce_fwd(const void *x, long long ld_x, const void *w, lo
   if (f32) { c.scale_a = &sp.h->unscale_x; c.scale_b = &sp.h->unscale_w; }
   c.target = target;
   c.sums = sp.sums; c.target_logit = sp.target_logit;
-  rc = plane_gemm(c, &sp.h->error, kCeWaitLimit, sm_count(), s);
+  rc = plane_gemm(c, &sp.h->error, dense_wait_limit(), sm_count(), s);
   if (rc != TF_OK) return rc;
   const int blocks = (rows + 31) / 32;
   ce_join_kernel<<<blocks, 256, 0, s>>>(sp.sums, plane_gemm_parts(rows, vocab), rows, sp.target_logit, target, ignore_index, vocab, lse2,
@@ -611,7 +616,7 @@ extern "C" int tf_linear_ce_bwd(const void *x, long long ld_x, const void *w, lo
     c.target = target; c.col0 = v0;
     c.lse2 = lse2; c.row_scale = sp.row_scale;
     c.slope_hi = sp.slope_hi; c.slope_lo = sp.slope_lo; c.ld_slope = sp.ld_slope;
-    rc = plane_gemm(c, &sp.h->error, kCeWaitLimit, sms, s);
+    rc = plane_gemm(c, &sp.h->error, dense_wait_limit(), sms, s);
     if (rc != TF_OK) return rc;
     const bool last = v0 + nv == vocab;
     if (dx) {
@@ -628,7 +633,7 @@ extern "C" int tf_linear_ce_bwd(const void *x, long long ld_x, const void *w, lo
       if (v0) g.sum_in = sp.parts_x;
       if (!last || sp.cut_x) g.sum_out = sp.parts_x;
       g.out = dx; g.out_dtype = dtype; g.ld_out = cols;
-      rc = plane_gemm(g, &sp.h->error, kCeWaitLimit, sms, s);
+      rc = plane_gemm(g, &sp.h->error, dense_wait_limit(), sms, s);
       if (rc != TF_OK) return rc;
     }
     if (dw) {
@@ -645,7 +650,7 @@ extern "C" int tf_linear_ce_bwd(const void *x, long long ld_x, const void *w, lo
       if (sp.cut_w) g.sum_out = sp.parts_w;
       char *to = (char *)dw + (size_t)v0 * cols * value_bytes(dtype);
       g.out = to; g.out_dtype = dtype; g.ld_out = cols;
-      rc = plane_gemm(g, &sp.h->error, kCeWaitLimit, sms, s);
+      rc = plane_gemm(g, &sp.h->error, dense_wait_limit(), sms, s);
       if (rc != TF_OK) return rc;
       if (sp.cut_w) {
         const long long q = (long long)nv * ld_sum / 4;
@@ -662,6 +667,12 @@ extern "C" int tf_linear_ce_bwd(const void *x, long long ld_x, const void *w, lo
   e = cudaGetLastError();
   if (e == cudaSuccess) e = ce_lost(sp.h, dx, (long long)rows * cols, dw, (long long)vocab * cols, dtype, s);
   return e == cudaSuccess ? TF_OK : ce_fail(who, e);
+}
+
+extern "C" int tf_dense_set_wait_limit(int polls) {
+  if (polls != 0 && polls < kInFlightPolls) return tf::fail(TF_ERR_ARG, "tf_dense_set_wait_limit: 0, or 65 536 polls at least");
+  wait_limit.store(polls, std::memory_order_relaxed);
+  return TF_OK;
 }
 
 extern "C" int tf_linear_ce_status(const void *work, void *stream) {

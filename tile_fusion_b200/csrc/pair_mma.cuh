@@ -61,6 +61,11 @@ __device__ __forceinline__ void pair_commit(unsigned long long *bar) {
                    smem_u32(bar)), "h"((unsigned short)3) : "memory");
 }
 
+// Only this CTA's.
+__device__ __forceinline__ void pair_commit_own(unsigned long long *bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
 // x = hi + lo for the tensor core, which reads the first eleven bits of either.  hi is rounded to them by the addition (its last bits
 // need not be cleared); a NaN may be lost there, but not in lo.  lo is a power of two or has at most twelve bits: if the last of
 // them is set, lo / 2048 carries into the bit before (it is at least one unit there and less than two), if not, what it adds

@@ -180,7 +180,7 @@ plane_gemm_kernel(const __grid_constant__ CUtensorMap tm_ahi, const __grid_const
     // a copy still in flight must not outlive the pair (only after a wait ran out is one possible)
     if ((!ok || s.dead) && rank == 0)
       for (int i = 0; i < issued; ++i)
-        for (int k = 0; k < P.wait_limit && !mbar_wait(&s.full[i], i < st ? ph : ph ^ 1u, 1); ++k) {}
+        mbar_wait(&s.full[i], i < st ? ph : ph ^ 1u, kInFlightPolls);
   } else if (warp == kPgDrainWarps + 1) {
     // ---- products (even CTA) ----
     if (rank == 0) {
@@ -231,8 +231,8 @@ plane_gemm_kernel(const __grid_constant__ CUtensorMap tm_ahi, const __grid_const
         }
       }
       if (!ok) {  // products still running read shared memory of both CTAs
-        if (elect_one()) pair_commit(&s.drained);
-        mbar_wait(&s.drained, 0, P.wait_limit);
+        if (elect_one()) pair_commit_own(&s.drained);
+        mbar_wait(&s.drained, 0, kInFlightPolls);
       }
     }
   } else {

@@ -13,6 +13,10 @@ constexpr int kMaxRows = 0x7f000000;  // of rows, columns and classes: an index 
 __host__ __device__ constexpr int value_bytes(int dtype) { return dtype == TF_F32 ? 4 : 2; }
 __host__ __device__ constexpr bool known_dtype(int dtype) { return dtype == TF_F32 || dtype == TF_BF16 || dtype == TF_F16; }
 
+// Polls of a bounded wait (tf_dense_set_wait_limit), and after one has run out, for copies and products under way that take microseconds.
+int dense_wait_limit();
+constexpr int kInFlightPolls = 1 << 16;
+
 __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }

@@ -37,7 +37,6 @@ constexpr int kWgChain = 8;                    // (fp32) slices added up in tens
 constexpr int kWgBlock = kWgRows * 128;        // bytes of 64 columns of a slice
 constexpr int kWgMaxRing = 16;
 constexpr int kWgSmem = 224 * 1024;
-constexpr int kWgWaitLimit = 1 << 22;
 
 __host__ __device__ constexpr int wg_stage_bytes(int planes, int mt) { return planes * mt * 2 * kWgBlock + (mt == 1 ? 4 : 2) * kWgBlock; }
 static_assert(wg_teams(3) * wg_stage_bytes(3, 2) <= kWgSmem && wg_teams(2) * wg_stage_bytes(2, 2) <= kWgSmem, "a stage to each team");
@@ -47,13 +46,14 @@ struct WgParams {
   const signed char *codes; int ld_codes, nb; const unsigned char *exps;
   int m, rows;  // rows of a range
   bool whole_g;
+  int wait_limit;
   int ring, g_bytes, ring_bytes;  // slices as they lie in memory that are on their way, bytes of G and of all of one
   float *part;  // [range][na][nb]
 };
 
 struct WgShared {
   unsigned long long raw_full[kWgMaxRing], raw_empty[kWgMaxRing];
-  unsigned long long full[kWgMaxTeams], empty[kWgMaxTeams], tail[kWgMaxTeams], acc_full[2], acc_empty[2];
+  unsigned long long full[kWgMaxTeams], empty[kWgMaxTeams], tail[kWgMaxTeams], acc_full[2], acc_empty[2], drained;
   unsigned tmem_base;
   int dead;
 };
@@ -177,6 +177,7 @@ __global__ void __launch_bounds__(wg_threads(PLANES, RING), 1) weight_grad8_kern
     if (RING)
       for (int i = 0; i < P.ring; ++i) { mbar_init(&s.raw_full[i], 1); mbar_init(&s.raw_empty[i], kTeamWarps); }
     for (int i = 0; i < 2; ++i) { mbar_init(&s.acc_full[i], 1); mbar_init(&s.acc_empty[i], kWarps); }
+    mbar_init(&s.drained, 1);
     s.dead = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -196,7 +197,7 @@ __global__ void __launch_bounds__(wg_threads(PLANES, RING), 1) weight_grad8_kern
     unsigned ph = 0;
     bool ok = true;
     for (int sl = 0; sl < whole; ++sl) {
-      if (sl >= P.ring && !(ok = __all_sync(kFull, pair_wait(&s.raw_empty[rs], ph ^ 1u, s.dead, kWgWaitLimit)))) break;
+      if (sl >= P.ring && !(ok = __all_sync(kFull, pair_wait(&s.raw_empty[rs], ph ^ 1u, s.dead, P.wait_limit)))) break;
       if (elect_one()) {
         const long long row = r0 + (long long)sl * kWgRows;
         const unsigned to = smem_u32(raw + rs * P.ring_bytes), bar = smem_u32(&s.raw_full[rs]);
@@ -213,15 +214,13 @@ __global__ void __launch_bounds__(wg_threads(PLANES, RING), 1) weight_grad8_kern
       if (issued < P.ring) ++issued;
       if (++rs == P.ring) { rs = 0; ph ^= 1u; }
     }
-    // a copy still in flight must not outlive the CTA (only after a wait ran out is one possible)
-    if (!ok || s.dead)
-      for (int i = 0; i < issued; ++i)
-        for (int k = 0; k < kWgWaitLimit && !mbar_wait(&s.raw_full[i], i < rs ? ph : ph ^ 1u, 1); ++k) {}
+    // no copy may outlive the CTA (where a wait has run out some may be in flight)
+    for (int i = 0; i < issued; ++i) mbar_wait(&s.raw_full[i], i < rs ? ph : ph ^ 1u, kInFlightPolls);
   } else if (warp == kWarps) {
     // ---- products ----
     const unsigned idesc = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (1u << 16) | ((unsigned)(n_pad >> 3) << 17) | ((unsigned)(128 >> 4) << 24);
     bool ok = true;
-    auto wait = [&](unsigned long long *bar, unsigned parity) { return ok = __all_sync(kFull, pair_wait(bar, parity, s.dead, kWgWaitLimit)); };
+    auto wait = [&](unsigned long long *bar, unsigned parity) { return ok = __all_sync(kFull, pair_wait(bar, parity, s.dead, P.wait_limit)); };
     for (int sl = 0; sl < slices; ++sl) {
       const int st = sl % kTeams;
       const int chain = STAY ? 0 : sl / kWgChain, buf = chain & 1, in = STAY ? sl : sl % kWgChain;
@@ -243,6 +242,10 @@ __global__ void __launch_bounds__(wg_threads(PLANES, RING), 1) weight_grad8_kern
       }
       __syncwarp();
     }
+    if (!ok) {  // products still running read shared memory and write tensor memory
+      if (elect_one()) umma_commit(&s.drained);
+      mbar_wait(&s.drained, 0, kInFlightPolls);
+    }
   } else {
     // ---- rows into operands, each team every so many slices; and (fp32) the sums of the chain before out of tensor memory ----
     const int team = warp / kTeamWarps, in_team = tid % kWgTeam;
@@ -252,7 +255,7 @@ __global__ void __launch_bounds__(wg_threads(PLANES, RING), 1) weight_grad8_kern
 #pragma unroll
       for (int i = 0; i < 64; ++i) acc[STAY ? 0 : i] = 0.f;
     bool ok = true;
-    auto wait = [&](unsigned long long *bar, unsigned parity) { return ok = __all_sync(kFull, pair_wait(bar, parity, s.dead, kWgWaitLimit)); };
+    auto wait = [&](unsigned long long *bar, unsigned parity) { return ok = __all_sync(kFull, pair_wait(bar, parity, s.dead, P.wait_limit)); };
     auto drain = [&](int chain) {
       const int buf = chain & 1;
       if (!wait(&s.acc_full[buf], (unsigned)(chain / 2) & 1u)) return;
@@ -499,6 +502,7 @@ extern "C" int tf_weight_grad8(const void *g, long long ld_g, int dtype, int na,
   P.g = g; P.ld_g = ld_g; P.na = na; P.codes = codes; P.ld_codes = ld_codes; P.nb = nb; P.exps = exponents; P.m = m; P.rows = p.rows;
   P.whole_g = na % (16 / value_bytes(dtype)) == 0 && ld_g * value_bytes(dtype) % 16 == 0 && (reinterpret_cast<uintptr_t>(g) & 15) == 0;
   P.part = work;
+  P.wait_limit = dense_wait_limit();
   cudaStream_t s = (cudaStream_t)stream;
   cudaError_t e = cudaSuccess;
   if (m > 0) {
