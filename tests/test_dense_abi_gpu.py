@@ -122,3 +122,22 @@ def test_weight_gradients_whose_waits_run_out(no_waits, dtype, m, na, nb, stride
     with no_waits():
         assert ops.weight_grad8(g, codes, exps).isnan().all()
     assert torch.equal(ops.weight_grad8(g, codes, exps), want)
+
+
+@pytest.mark.parametrize("v", [40, 300])
+def test_status_of_a_call_of_no_rows(built_lib, v):
+    """The work space may hold anything before a call."""
+    import torch
+    L = _lib.lib()
+    x, w, t = make(4, 64, v, "float32")
+    for backward_ in (0, 1):
+        work = torch.full((L.tf_linear_ce_work_bytes(0, 64, v, _lib.F32, backward_),), 255, device="cuda", dtype=torch.uint8)
+        for reduction in (0, 1):
+            work.fill_(255)
+            if backward_:
+                dw = torch.ones_like(w)
+                backward(x[:0], w, t[:0], reduction, torch.empty(0, device="cuda"), torch.ones(1, device="cuda"), x[:0], dw, work)
+                assert (dw == 0).all()
+            else:
+                forward(x[:0], w, t[:0], reduction, work)
+            assert L.tf_linear_ce_status(work.data_ptr(), stream()) == _lib.TF_OK

@@ -514,8 +514,8 @@ extern "C" int tf_linear_ce_fwd(const void *x, long long ld_x, const void *w, lo
   if (work_bytes < tf_linear_ce_work_bytes(rows, cols, vocab, dtype, 0)) return tf::fail(TF_ERR_ARG, "tf_linear_ce_fwd: work space too small");
   cudaStream_t s = (cudaStream_t)stream;
   if (rows == 0) {
-    if (!reduction) return TF_OK;
-    const cudaError_t e = cudaMemsetAsync(loss, 0, 4, s);
+    cudaError_t e = cudaMemsetAsync(work, 0, sizeof(CeHeader), s);
+    if (e == cudaSuccess && reduction) e = cudaMemsetAsync(loss, 0, 4, s);
     return e == cudaSuccess ? TF_OK : ce_fail(who, e);
   }
   const CeSpace sp = ce_space((char *)work, rows, cols, vocab, dtype, false, ce_whole(x, ld_x, dtype), ce_whole(w, ld_w, dtype));
@@ -568,7 +568,8 @@ extern "C" int tf_linear_ce_bwd(const void *x, long long ld_x, const void *w, lo
   if (work_bytes < tf_linear_ce_work_bytes(rows, cols, vocab, dtype, 1)) return tf::fail(TF_ERR_ARG, "tf_linear_ce_bwd: work space too small");
   cudaStream_t s = (cudaStream_t)stream;
   if (rows == 0) {
-    const cudaError_t e = dw ? cudaMemsetAsync(dw, 0, (size_t)vocab * cols * value_bytes(dtype), s) : cudaSuccess;
+    cudaError_t e = cudaMemsetAsync(work, 0, sizeof(CeHeader), s);
+    if (e == cudaSuccess && dw) e = cudaMemsetAsync(dw, 0, (size_t)vocab * cols * value_bytes(dtype), s);
     return e == cudaSuccess ? TF_OK : ce_fail(who, e);
   }
   if (!dx && !dw) return TF_OK;
