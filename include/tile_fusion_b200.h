@@ -413,7 +413,8 @@ int tf_layer_norm_bwd(const void *x, long long ld_x, const signed char *codes, i
  * rounds to zero (it reads back as zero).
  *   tf_relu_grad8: grad (in place) becomes zero where the code is zero, i.e. where a value packed with relu was not positive.
  *   tf_weight_grad8: out[na][nb] = G^T X for G [m][na] and the packed X [m][nb], in G's type; products are exact, sums fp32;
- * work: tf_weight_grad8_work_floats floats of the caller's, 16-byte aligned; at most 2^26 entries, 2^20 to a side.
+ * work: tf_weight_grad8_work_floats floats of the caller's, 16-byte aligned; at most 2^26 entries, 2^20 to a side,
+ * and rows of codes at most 2^26 bytes apart.
  * Device pointers; the calls only enqueue work on `stream`. */
 int tf_pack8(const void *x, long long ld, int dtype, int rows, int cols, int relu, signed char *codes, int ld_codes,
              unsigned char *exponents, void *stream);

@@ -131,3 +131,12 @@ def test_wait_limit(L):
     for polls in (-1, 1, 65535):
         refused(L.tf_dense_set_wait_limit(polls), "polls")
     assert L.tf_dense_set_wait_limit(65536) == 0 and L.tf_dense_set_wait_limit(0) == 0 and L.tf_dense_set_wait_limit(1 << 22) == 0
+
+
+def test_weight_grad8_of_rows_far_apart(L):
+    """16 rows of codes more than 2^26 bytes apart overflow the 32 bits that a slice's bytes are counted in; and no work space for what is refused."""
+    grad = lambda **k: L.tf_weight_grad8(*{**dict(g=P, ld=8, t=0, na=8, c=P, ldc=64, e=P, nb=40, m=4, out=P, work=P, wn=1 << 40, s=None), **k}.values())  # noqa: E731
+    for ld in ((1 << 26) + 32, 1 << 27, 1 << 28, 0x7fffffe0):
+        refused(grad(ldc=ld), "apart")
+    assert L.tf_weight_grad8_work_floats(10, 1 << 20, 1 << 20, 0) == 0 and L.tf_weight_grad8_work_floats(10, (1 << 20) + 1, 1, 1) == 0
+    assert L.tf_weight_grad8_work_floats(10, 1 << 13, 1 << 13, 1) == 1 << 26

@@ -473,6 +473,10 @@ template <class T, int PLANES> cudaError_t wg_run(const WgPlan &p, WgParams P, c
   return p.mt == 1 ? wg_launch<T, PLANES, 1, false>(p, P, s) : wg_launch<T, PLANES, 2, false>(p, P, s);
 }
 
+// (the tiles of a side are a dimension of the grid, 65 535 at most, and a slice's bytes are counted in 32 bits)
+bool wg_fits(int na, int nb) { return (long long)na * nb <= (1 << 26) && na <= (1 << 20) && nb <= (1 << 20); }
+constexpr int kWgMaxLdCodes = 1 << 26;
+
 }  // namespace
 
 }  // namespace tfk
@@ -480,7 +484,7 @@ template <class T, int PLANES> cudaError_t wg_run(const WgPlan &p, WgParams P, c
 using namespace tfk;
 
 extern "C" long long tf_weight_grad8_work_floats(int m, int na, int nb, int dtype) {
-  if (m < 0 || m > kMaxRows || na <= 0 || nb <= 0 || na > kMaxRows || nb > kMaxRows || !known_dtype(dtype)) return 0;
+  if (m < 0 || m > kMaxRows || na <= 0 || nb <= 0 || !wg_fits(na, nb) || !known_dtype(dtype)) return 0;
   return (long long)wg_plan(m, na, nb, dtype).parts * na * nb;
 }
 
@@ -489,9 +493,8 @@ extern "C" int tf_weight_grad8(const void *g, long long ld_g, int dtype, int na,
   auto bad = [&](const char *what) { return tf::fail(TF_ERR_ARG, std::string("tf_weight_grad8: ") + what); };
   if (!known_dtype(dtype)) return bad("unknown type");
   if (m < 0 || m > kMaxRows || na <= 0 || nb <= 0) return bad("bad size");
-  // (the tiles of a side are a dimension of the grid, 65 535 at most, and a slice's bytes are counted in 32 bits)
-  if ((long long)na * nb > (1 << 26) || na > (1 << 20) || nb > (1 << 20))
-    return tf::fail(TF_ERR_UNSUPPORTED, "tf_weight_grad8: at most 2^26 entries, 2^20 to a side");
+  if (!wg_fits(na, nb)) return tf::fail(TF_ERR_UNSUPPORTED, "tf_weight_grad8: at most 2^26 entries, 2^20 to a side");
+  if (ld_codes > kWgMaxLdCodes) return tf::fail(TF_ERR_UNSUPPORTED, "tf_weight_grad8: rows of codes at most 2^26 bytes apart");
   if (!out || !work || (m > 0 && (!g || !codes || !exponents))) return bad("null argument");
   if (ld_g < na || ld_codes < nb) return bad("rows overlap");
   if (ld_codes % kPackGroup != 0 || (reinterpret_cast<uintptr_t>(codes) & 31) != 0) return bad("codes need rows of whole groups of 32 and 32-byte alignment");
