@@ -109,3 +109,21 @@ def test_training_step(built_lib):
         near(got, ref)
     again = step()
     assert torch.equal(again[0], loss) and all(torch.equal(s, t) for s, t in zip(again[4], grads))
+
+
+def test_weights_whose_gradient_is_refused(built_lib):
+    """2^27 entries: refused before anything is allocated, by the layer in its forward pass, not in the backward one."""
+    import torch
+    from tile_fusion_b200 import sw_gcn  # noqa: F401
+    ops = torch.ops.sw_gcn
+    i = torch.arange(5, dtype=torch.int32)
+    adj = torch.sparse_csr_tensor(i, i[:4], torch.ones(4), size=(4, 4)).cuda()
+    w = torch.zeros(1 << 14, 1 << 13, device="cuda").requires_grad_()
+    with pytest.raises(ValueError, match="entries"):
+        ops.fusedGeMMSpMM_ck8(adj, torch.ones(4, 1 << 13, device="cuda"), w, [], 1)
+    codes, exponents = ops.pack8(torch.ones(2, 1 << 20, device="cuda"))
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    with pytest.raises(ValueError, match="entries"):
+        ops.weight_grad8(torch.ones(2, 1 << 20, device="cuda"), codes, exponents)
+    assert torch.cuda.max_memory_allocated() < before + (1 << 31)

@@ -182,6 +182,12 @@ def unpack8(codes, exponents, dtype=None):
     return _unpack(codes, ld, exponents, dtype, codes.shape[0], d)
 
 
+def refuse_weight_grad8(name, na, nb):
+    """A weight gradient [na, nb] that the library does not take, before anything is allocated for it."""
+    if na * nb > 1 << 26 or max(na, nb) > 1 << 20:
+        raise ValueError(f"sw_gcn.{name}: a weight gradient from 8 bits has at most 2^26 entries, 2^20 to a side, not [{na}, {nb}]")
+
+
 def weight_grad8(grad, codes, exponents):
     name = "weight_grad8"
     _check_values(name, "grad", grad)
@@ -190,6 +196,7 @@ def weight_grad8(grad, codes, exponents):
     if _tangents():
         _refuse_tangent(name, grad)
     nb = codes.shape[1]
+    refuse_weight_grad8(name, grad.shape[1], nb)
     codes, exponents, ld = _packed(name, codes, exponents)
     _same_device(name, grad, codes)
     return _weight_grad(_rows(grad), codes, ld, exponents, nb)

@@ -168,6 +168,8 @@ def _ck8(adj, feature, weight, schedule, num_threads, relu=False):
         raise ValueError(f"{name}: feature and weight must be CUDA tensors on one device, not {feature.device} and {weight.device}")
     if not feature.is_floating_point() or not weight.is_floating_point():
         raise ValueError(f"{name}: feature and weight must hold floating-point values, not {feature.dtype}, {weight.dtype}")
+    if weight.requires_grad and torch.is_grad_enabled():
+        dense_ops.refuse_weight_grad8("fusedGeMMSpMM_ck8", *weight.shape)
     with torch.cuda.device(feature.device):
         return _FusedGeMMSpMMCk8.apply(adj, feature, weight, bool(relu))
 
