@@ -436,11 +436,15 @@ int tf_weight_grad8(const void *g, long long ld_g, int dtype, int na, const sign
  *   backward: grad[1] (reduction 1, 2) or grad[rows] (0) is the gradient of the loss; dx [rows][cols] and dw [vocab][cols],
  * contiguous, of the operands' type, are overwritten; either may be NULL.  Rows that do not count have a gradient of zero and
  * add nothing to dw, whatever they hold.
- *   work: tf_linear_ce_work_bytes bytes, 256-byte aligned, of the caller's; two calls that may overlap need two.  The calls
- * only enqueue work on `stream`; they allocate nothing and can be captured.  tf_linear_ce_status waits for `stream` and says
- * whether a bounded wait of the last call with this work space ran out (the losses and lse2, or the gradients, are NaN then);
- * a backward call that is asked for neither gradient leaves the work space as it was. */
+ *   work: tf_linear_ce_work_bytes bytes of the caller's, 256-byte aligned, or, where the operands are known,
+ * tf_linear_ce_work_bytes_for: less where 16-bit operands can be multiplied as they lie (16-byte aligned, rows a multiple of
+ * eight values apart).  Two calls that may overlap need two.  The calls only enqueue work on `stream`; they allocate nothing and
+ * can be captured.  tf_linear_ce_status waits for `stream` and says whether a bounded wait of the last call with this work space
+ * ran out (the losses and lse2, or the gradients, are NaN then); a backward call that is asked for neither gradient leaves the
+ * work space as it was. */
 long long tf_linear_ce_work_bytes(int rows, int cols, int vocab, int dtype, int backward);
+long long tf_linear_ce_work_bytes_for(const void *x, long long ld_x, const void *w, long long ld_w, int rows, int cols, int vocab, int dtype,
+                                      int backward);
 int tf_linear_ce_fwd(const void *x, long long ld_x, const void *w, long long ld_w, int dtype, const long long *target, int rows,
                      int cols, int vocab, long long ignore_index, int reduction, float *loss, float *lse2, void *work,
                      long long work_bytes, void *stream);

@@ -140,3 +140,23 @@ def test_weight_grad8_of_rows_far_apart(L):
         refused(grad(ldc=ld), "apart")
     assert L.tf_weight_grad8_work_floats(10, 1 << 20, 1 << 20, 0) == 0 and L.tf_weight_grad8_work_floats(10, (1 << 20) + 1, 1, 1) == 0
     assert L.tf_weight_grad8_work_floats(10, 1 << 13, 1 << 13, 1) == 1 << 26
+
+
+@pytest.mark.parametrize("dtype", [_lib.BF16, _lib.F16])
+def test_work_space_of_a_loss(L, dtype):
+    """Operands that are multiplied as they lie need no copy: 8 192 x 4 096 with 128 000 classes took 1 GB for one of the weights."""
+    n, d, v = 8192, 4096, 128_000
+    size = lambda x, ldx, w, ldw, back: L.tf_linear_ce_work_bytes_for(x, ldx, w, ldw, n, d, v, dtype, back)  # noqa: E731
+    weights, rows = 2 * v * d, 2 * n * d
+    for back in (0, 1):
+        most = L.tf_linear_ce_work_bytes(n, d, v, dtype, back)
+        assert size(P + 2, d, P + 2, d, back) == size(P, d + 4, P, d + 4, back) == most
+        assert most - size(P + 2, d, P, d, back) == weights
+        assert most - size(P, d, P + 2, d, back) == (0 if back else rows)  # (the backward pass clears rows that do not count in a copy)
+    assert size(P, d, P, d, 0) < weights // 8
+    assert size(P, d, P, d, 1) < 2 * rows + (600 << 20)
+    assert L.tf_linear_ce_work_bytes_for(P, d, P, d, n, d, v, _lib.F32, 0) == L.tf_linear_ce_work_bytes(n, d, v, _lib.F32, 0)
+    fwd = lambda need: L.tf_linear_ce_fwd(P, 64, P, 64, dtype, P, 4, 64, 300, -100, 1, P, P, P, need, None)  # noqa: E731
+    need = L.tf_linear_ce_work_bytes_for(P, 64, P, 64, 4, 64, 300, dtype, 0)
+    refused(fwd(need - 1), "work")
+    assert L.tf_linear_ce_work_bytes_for(P, 64, P, 64, 0x7f000001, 64, 300, dtype, 0) == 0

@@ -309,3 +309,21 @@ def test_tangents_and_traces(built_lib):
         assert torch.equal(call(x, w, t), loss)
     traced = torch.jit.trace(lambda a: call(a, w, t), (x,))
     assert torch.equal(traced(x), loss) and torch.equal(traced(z), other)
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:])
+def test_memory_of_a_large_vocabulary(built_lib, dtype):
+    """Beside the gradients: the piece of the slope, the copy of x and less; no copy of the weight."""
+    import torch
+    n, d, v = 64, 1024, 100_000
+    x, w, t = make(n, d, v, dtype)
+    run(x, w, t)
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    with torch.no_grad():
+        from tile_fusion_b200 import sw_gcn  # noqa: F401
+        torch.ops.sw_gcn.linear_cross_entropy(x, w, t)
+    assert torch.cuda.max_memory_allocated() - before < 2 * v * d // 8
+    torch.cuda.reset_peak_memory_stats()
+    run(x, w, t)
+    assert torch.cuda.max_memory_allocated() - before < 2 * v * d + (100 << 20)

@@ -50,7 +50,7 @@ EXPORTS = [
     "tf_multi_exec", "tf_multi_status", "tf_multi_trace", "tf_partition_layout", "tf_read_matrix", "tf_read_dense_mtx",
     "tf_schedule_unfused_csr", "tf_schedule_reordered_adj", "tf_rcm_order", "tf_permute_csr",
     "tf_layer_norm_fwd", "tf_layer_norm_bwd", "tf_layer_norm_work_floats", "tf_pack8", "tf_unpack8", "tf_relu_grad8",
-    "tf_weight_grad8", "tf_weight_grad8_work_floats", "tf_linear_ce_work_bytes", "tf_linear_ce_fwd", "tf_linear_ce_bwd", "tf_linear_ce_status", "tf_dense_set_wait_limit",
+    "tf_weight_grad8", "tf_weight_grad8_work_floats", "tf_linear_ce_work_bytes", "tf_linear_ce_work_bytes_for", "tf_linear_ce_fwd", "tf_linear_ce_bwd", "tf_linear_ce_status", "tf_dense_set_wait_limit",
 ]
 
 _lib = None
@@ -152,6 +152,8 @@ def lib() -> C.CDLL:
     L.tf_weight_grad8.argtypes = [vp, ll, i, i, vp, i, vp, i, i, vp, vp, ll, vp]
     L.tf_linear_ce_work_bytes.argtypes = [i, i, i, i, i]
     L.tf_linear_ce_work_bytes.restype = ll
+    L.tf_linear_ce_work_bytes_for.argtypes = [vp, ll, vp, ll, i, i, i, i, i]
+    L.tf_linear_ce_work_bytes_for.restype = ll
     L.tf_linear_ce_fwd.argtypes = [vp, ll, vp, ll, i, vp, i, i, i, ll, i, vp, vp, vp, ll, vp]
     L.tf_linear_ce_bwd.argtypes = [vp, ll, vp, ll, i, vp, i, i, i, ll, i, vp, vp, vp, vp, vp, ll, vp]
     L.tf_linear_ce_status.argtypes = [vp, vp]

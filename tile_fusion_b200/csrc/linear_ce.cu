@@ -504,6 +504,12 @@ extern "C" long long tf_linear_ce_work_bytes(int rows, int cols, int vocab, int 
   return ce_space(nullptr, std::max(rows, 1), cols, vocab, dtype, backward != 0, false, false).bytes;
 }
 
+extern "C" long long tf_linear_ce_work_bytes_for(const void *x, long long ld_x, const void *w, long long ld_w, int rows, int cols, int vocab, int dtype,
+                                                 int backward) {
+  if (rows < 0 || cols <= 0 || vocab <= 0 || rows > kMaxRows || cols > kMaxRows || vocab > kMaxRows || !known_dtype(dtype)) return 0;
+  return ce_space(nullptr, std::max(rows, 1), cols, vocab, dtype, backward != 0, ce_whole(x, ld_x, dtype), ce_whole(w, ld_w, dtype)).bytes;
+}
+
 extern "C" int tf_linear_ce_fwd(const void *x, long long ld_x, const void *w, long long ld_w, int dtype, const long long *target, int rows,
                                 int cols, int vocab, long long ignore_index, int reduction, float *loss, float *lse2, void *work,
                                 long long work_bytes, void *stream) {
@@ -511,7 +517,7 @@ extern "C" int tf_linear_ce_fwd(const void *x, long long ld_x, const void *w, lo
   int rc = ce_check(who, x, ld_x, w, ld_w, dtype, target, rows, cols, vocab, reduction, work);
   if (rc != TF_OK) return rc;
   if ((!loss && (reduction || rows)) || (!lse2 && rows)) return tf::fail(TF_ERR_ARG, "tf_linear_ce_fwd: null argument");
-  if (work_bytes < tf_linear_ce_work_bytes(rows, cols, vocab, dtype, 0)) return tf::fail(TF_ERR_ARG, "tf_linear_ce_fwd: work space too small");
+  if (work_bytes < tf_linear_ce_work_bytes_for(x, ld_x, w, ld_w, rows, cols, vocab, dtype, 0)) return tf::fail(TF_ERR_ARG, "tf_linear_ce_fwd: work space too small");
   cudaStream_t s = (cudaStream_t)stream;
   if (rows == 0) {
     cudaError_t e = cudaMemsetAsync(work, 0, sizeof(CeHeader), s);
@@ -565,7 +571,7 @@ extern "C" int tf_linear_ce_bwd(const void *x, long long ld_x, const void *w, lo
   int rc = ce_check(who, x, ld_x, w, ld_w, dtype, target, rows, cols, vocab, reduction, work);
   if (rc != TF_OK) return rc;
   if (rows > 0 && (!lse2 || !grad)) return tf::fail(TF_ERR_ARG, "tf_linear_ce_bwd: null argument");
-  if (work_bytes < tf_linear_ce_work_bytes(rows, cols, vocab, dtype, 1)) return tf::fail(TF_ERR_ARG, "tf_linear_ce_bwd: work space too small");
+  if (work_bytes < tf_linear_ce_work_bytes_for(x, ld_x, w, ld_w, rows, cols, vocab, dtype, 1)) return tf::fail(TF_ERR_ARG, "tf_linear_ce_bwd: work space too small");
   cudaStream_t s = (cudaStream_t)stream;
   if (rows == 0) {
     cudaError_t e = cudaMemsetAsync(work, 0, sizeof(CeHeader), s);

@@ -46,13 +46,8 @@ __device__ __forceinline__ unsigned pack_pair(float a, float b, bool f16) {
   return *reinterpret_cast<const unsigned *>(&h);
 }
 
-// N consecutive values (N a power of two, the address a multiple of their size) in one load or store.
+// N consecutive values (N a power of two, the address a multiple of their size) in one access.
 template <class T, int N> struct alignas(sizeof(T) * N) Pack { T v[N]; };
-template <class T, int N> __device__ __forceinline__ void load_pack(const T *p, float (&v)[N]) {
-  const Pack<T, N> a = *reinterpret_cast<const Pack<T, N> *>(p);
-#pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = to_float(a.v[i]);
-}
 template <class T, int N> __device__ __forceinline__ void store_pack(T *p, const float (&v)[N]) {
   Pack<T, N> a;
 #pragma unroll

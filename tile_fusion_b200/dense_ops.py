@@ -292,7 +292,7 @@ def _loss_forward(xr, w, t, ignore_index, reduction, stream):
     n, d, v, code = xr.shape[0], xr.shape[1], w.shape[0], _DTYPES[xr.dtype]
     loss = torch.empty(n if reduction == 0 else (), device=xr.device, dtype=torch.float32)
     lse = torch.empty(n, device=xr.device, dtype=torch.float32)
-    work = torch.empty(L.tf_linear_ce_work_bytes(n, d, v, code, 0), device=xr.device, dtype=torch.uint8)
+    work = torch.empty(L.tf_linear_ce_work_bytes_for(xr.data_ptr(), _ld(xr), w.data_ptr(), _ld(w), n, d, v, code, 0), device=xr.device, dtype=torch.uint8)
     _lib.check(L.tf_linear_ce_fwd(xr.data_ptr(), _ld(xr), w.data_ptr(), _ld(w), code, t.data_ptr(), n, d, v, ignore_index, reduction,
                                   loss.data_ptr(), lse.data_ptr(), work.data_ptr(), work.numel(), stream))
     return loss, lse
@@ -304,7 +304,7 @@ def _loss_backward(xr, w, t, lse, grad, ignore_index, reduction, want, stream):
     n, d, v, code = xr.shape[0], xr.shape[1], w.shape[0], _DTYPES[xr.dtype]
     dx = torch.empty((n, d), device=xr.device, dtype=xr.dtype) if want[0] else None
     dw = torch.empty((v, d), device=xr.device, dtype=xr.dtype) if want[1] else None
-    work = torch.empty(L.tf_linear_ce_work_bytes(n, d, v, code, 1), device=xr.device, dtype=torch.uint8)
+    work = torch.empty(L.tf_linear_ce_work_bytes_for(xr.data_ptr(), _ld(xr), w.data_ptr(), _ld(w), n, d, v, code, 1), device=xr.device, dtype=torch.uint8)
     _lib.check(L.tf_linear_ce_bwd(xr.data_ptr(), _ld(xr), w.data_ptr(), _ld(w), code, t.data_ptr(), n, d, v, ignore_index, reduction,
                                   lse.data_ptr(), grad.data_ptr(), _ptr(dx), _ptr(dw), work.data_ptr(), work.numel(), stream))
     return dx, dw
