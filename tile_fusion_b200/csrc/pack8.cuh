@@ -26,11 +26,12 @@ __device__ __forceinline__ int pack8_exponent(unsigned top) {
 }
 // A code in the low byte of the result, from x in steps of its group, at most 128 of them: adding 1.5 * 2^23 leaves the nearest whole
 // number in the last bits, ties to even (a conversion instruction runs at a quarter of the rate).
-// (RELU: `v`, the value itself, says whether it is positive: far below its group's largest its steps are zero.)
-template <bool RELU> __device__ __forceinline__ unsigned pack8_code(float steps, float v) {
+template <bool RELU> __device__ __forceinline__ unsigned pack8_code(float steps) {
   if (!RELU) return __float_as_uint(steps + 12582912.f);
-  return v > 0.f && steps <= 0.5f ? 0x80u : __float_as_uint(fmaxf(steps, 0.f) + 12582912.f);
+  return steps > 0.f && steps <= 0.5f ? 0x80u : __float_as_uint(fmaxf(steps, 0.f) + 12582912.f);
 }
+// A value in steps: exact but far below the group's largest, where a positive one (rounded up) does not become zero.
+__device__ __forceinline__ float pack8_steps(float v, float power) { return __fmul_ru(v, power); }
 __device__ __forceinline__ float unpack8_step(unsigned byte) {  // 2^(e - 6), NaN for 255
   return byte == 255 ? __int_as_float(0x7fc00000) : __uint_as_float((byte - 6) << 23);
 }
@@ -85,11 +86,11 @@ template <int N, bool RELU> __device__ __forceinline__ int pack8_lanes(const flo
     const float power = e == 127 ? pack8_power(6 - e) : 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      code[i] = e == 127 ? pack8_code<RELU>(fminf(fmaxf(v[i] * power, -127.f), 127.f), v[i]) : RELU && v[i] > 0.f ? 0x80u : 0u;
+      code[i] = e == 127 ? pack8_code<RELU>(fminf(fmaxf(pack8_steps(v[i], power), -127.f), 127.f)) : RELU && v[i] > 0.f ? 0x80u : 0u;
   } else {
     const float power = pack8_power(6 - e);
 #pragma unroll
-    for (int i = 0; i < N; ++i) code[i] = pack8_code<RELU>(v[i] * power, v[i]);
+    for (int i = 0; i < N; ++i) code[i] = pack8_code<RELU>(pack8_steps(v[i], power));
   }
   return e;
 }
