@@ -127,3 +127,31 @@ def test_weights_whose_gradient_is_refused(built_lib):
     with pytest.raises(ValueError, match="entries"):
         ops.weight_grad8(torch.ones(2, 1 << 20, device="cuda"), codes, exponents)
     assert torch.cuda.max_memory_allocated() < before + (1 << 31)
+
+
+@pytest.mark.parametrize("relu", [False, True])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "columns first"])
+def test_layer_of_other_features(built_lib, dtype, relu):
+    """Features in 16 bits, or whose columns lie apart, are the same as their copy in fp32, stay as they are, and are copied once."""
+    import torch
+    from tile_fusion_b200 import sw_gcn  # noqa: F401
+    ops = torch.ops.sw_gcn
+    adj, _ = graph(20_000)
+    n, k = adj.shape[0], 512
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(n, k, generator=gen, device="cuda")
+    x = (x.t().contiguous().t() if dtype == "columns first" else x.to(getattr(torch, dtype))).requires_grad_()
+    w = (torch.randn(24, k, generator=gen, device="cuda") / 6).requires_grad_()
+    g = torch.randn(n, 24, generator=gen, device="cuda")
+    before = x.detach().clone()
+    plain = x.detach().float().contiguous().requires_grad_()
+    y = ops.fusedGeMMSpMM_ck8(adj, plain, w, [], 4, relu)
+    want = (y.detach(),) + torch.autograd.grad(y, (plain, w), g)
+    del y, plain
+    torch.cuda.reset_peak_memory_stats()
+    held = torch.cuda.memory_allocated()
+    y = ops.fusedGeMMSpMM_ck8(adj, x, w, [], 4, relu)
+    assert torch.cuda.max_memory_allocated() - held < 1.5 * 4 * n * k  # the copy in fp32, its 8 bits
+    got = (y.detach(),) + torch.autograd.grad(y, (x, w), g)
+    assert torch.equal(x.detach(), before) and got[1].dtype == x.dtype
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1].to(x.dtype)) and torch.equal(got[2], want[2])

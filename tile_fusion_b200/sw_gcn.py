@@ -136,14 +136,15 @@ class _FusedGeMMSpMMCk8(torch.autograd.Function):
     @staticmethod
     def forward(ctx, adj, feature, weight, relu):
         x = feature.contiguous().float()
-        if relu:
-            x = torch.relu(x)
+        keep = ctx.needs_input_grad[2] or (relu and ctx.needs_input_grad[1])
+        kept = dense_ops._pack(x, relu) if keep else (None, None)
+        if relu:  # (a copy of the feature's own is not needed twice)
+            x = torch.relu(x) if x.data_ptr() == feature.data_ptr() else x.relu_()
         w = weight.contiguous().float()
         out = torch.empty((adj.shape[0], w.shape[0]), device=x.device, dtype=torch.float32)
         _plan(adj, x.shape[1], w.shape[0]).gemm_spmm(x, w, out, w_transposed=True)
         ctx.adj, ctx.relu = adj, relu
-        keep = ctx.needs_input_grad[2] or (relu and ctx.needs_input_grad[1])
-        ctx.save_for_backward(w, *(dense_ops._pack(feature.contiguous().float(), relu) if keep else (None, None)))
+        ctx.save_for_backward(w, *kept)
         return out
 
     @staticmethod
