@@ -160,3 +160,13 @@ def test_work_space_of_a_loss(L, dtype):
     need = L.tf_linear_ce_work_bytes_for(P, 64, P, 64, 4, 64, 300, dtype, 0)
     refused(fwd(need - 1), "work")
     assert L.tf_linear_ce_work_bytes_for(P, 64, P, 64, 0x7f000001, 64, 300, dtype, 0) == 0
+
+
+def test_work_space_of_a_weight_gradient(L):
+    """Of the result's size where that is large, however many rows: a million rows of 16-bit gradients for 2^26 entries took 31 times as much."""
+    for dtype in (_lib.F32, _lib.BF16, _lib.F16):
+        for m in (1, 100_000, 1_000_000, 0x7f000000):
+            assert L.tf_weight_grad8_work_floats(m, 1 << 13, 1 << 13, dtype) <= 2 << 26
+            assert L.tf_weight_grad8_work_floats(m, 47, 256, dtype) <= (64 << 20) + 2 * 47 * 256
+            assert L.tf_weight_grad8_work_floats(m, 1000, 700, dtype) <= (64 << 20) + 2 * 1000 * 700
+    assert L.tf_weight_grad8_work_floats(1_000_000, 256, 100, _lib.BF16) == 148 * 256 * 100

@@ -150,3 +150,27 @@ def test_mask_of_8_bits(built_lib, cols):
         assert torch.equal(got, w)
     del want
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dtype,na,nb", [("bfloat16", 2048, 2048), ("float16", 1900, 2100)])
+def test_weight_gradient_in_several_launches(built_lib, dtype, na, nb):
+    """More ranges of 32 768 rows than are summed in one launch: values in the first and last rows and on both sides of the launches' border."""
+    import torch
+    from tile_fusion_b200 import sw_gcn  # noqa: F401
+    ops = torch.ops.sw_gcn
+    n, k = 700_003, 200
+    border = 16 * 31_824  # 22 ranges, of 31 824 rows (whole sixteens) each, 2^26 sums or 16 of them a launch
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    some = torch.cat([torch.arange(a, b, device="cuda") for a, b in ((0, k), (border - k, border + k), (n - k, n))])
+    x = torch.empty(n, nb, device="cuda", dtype=getattr(torch, dtype)).normal_(generator=gen)
+    g = torch.zeros(n, na, device="cuda", dtype=x.dtype)
+    g[some] = torch.empty(len(some), na, device="cuda", dtype=x.dtype).normal_(generator=gen)
+    codes, exponents = ops.pack8(x)
+    got = ops.weight_grad8(g, codes, exponents)
+    kept = ops.unpack8(codes[some], exponents[some]).double()
+    near(got, g[some].double().t() @ kept, U[dtype])
+    assert torch.equal(got, ops.weight_grad8(g, codes, exponents))
+    for part in (slice(0, k), slice(k, 3 * k), slice(3 * k, 4 * k)):  # each of the three has its say
+        alone = torch.zeros_like(g)
+        alone[some[part]] = g[some[part]]
+        near(ops.weight_grad8(alone, codes, exponents), g[some[part]].double().t() @ kept[part], U[dtype])

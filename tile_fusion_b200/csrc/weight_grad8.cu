@@ -414,8 +414,10 @@ __global__ void __launch_bounds__(wg_threads(PLANES, RING), 1) weight_grad8_kern
   }
 }
 
-// out[i] = part[0][i] + part[1][i] + ..., in order; eight lanes share an element's parts and are added pairwise.
-__global__ void __launch_bounds__(256) wg_sum_kernel(const float *__restrict__ part, int parts, int n, void *__restrict__ out, int dtype) {
+// out[i] = part[0][i] + part[1][i] + ..., in order; eight lanes share an element's parts and are added pairwise.  before: the sums of the
+// launches before this one, added last; after: where they go if more follow, instead of out.
+__global__ void __launch_bounds__(256) wg_sum_kernel(const float *__restrict__ part, int parts, int n, const float *before, float *after, void *__restrict__ out,
+                                                     int dtype) {
   const int i = blockIdx.x * 32 + (threadIdx.x & 31), l = threadIdx.x >> 5;
   __shared__ float s[8][32];
   float v = 0.f;
@@ -427,10 +429,15 @@ __global__ void __launch_bounds__(256) wg_sum_kernel(const float *__restrict__ p
   if (l || i >= n) return;
 #pragma unroll
   for (int k = 1; k < 8; ++k) v += s[k][threadIdx.x];
-  store_value(out, dtype, i, v);
+  if (before) v += before[i];
+  if (after) after[i] = v;
+  else store_value(out, dtype, i, v);
 }
 
-struct WgPlan { int mt, tiles_a, tiles_b, parts, rows; };
+// parts: ranges of rows, `group` of them a launch.  Ranges of 32 768 rows at most (gradients in 16 bits) are more than fill the device where
+// there are many rows; those of a launch together hold 256 MB of sums at most, or as many as fill it.
+struct WgPlan { int mt, tiles_a, tiles_b, parts, rows, group; };
+constexpr long long kWgMaxFloats = 64ll << 20;
 WgPlan wg_plan(int m, int na, int nb, int dtype) {
   auto tiles = [&](int mt) {
     WgPlan p;
@@ -450,6 +457,7 @@ WgPlan wg_plan(int m, int na, int nb, int dtype) {
   if (dtype != TF_F32) parts = std::max(parts, (m + kWgStayRows - 1) / kWgStayRows);
   p.rows = ((m + parts - 1) / parts + kWgRows - 1) / kWgRows * kWgRows;
   p.parts = std::max(1, (m + p.rows - 1) / std::max(1, p.rows));
+  p.group = (int)std::min<long long>(p.parts, std::max<long long>(std::max(1, 148 / (p.tiles_a * p.tiles_b)), kWgMaxFloats / ((long long)na * nb)));
   return p;
 }
 
@@ -458,7 +466,7 @@ template <class T, int PLANES, int MT, bool RING> cudaError_t wg_launch(const Wg
   const int smem = wg_teams(PLANES) * wg_stage_bytes(PLANES, MT) + P.ring * P.ring_bytes + 1024;
   const cudaError_t e = cudaFuncSetAttribute((const void *)f, cudaFuncAttributeMaxDynamicSharedMemorySize, kWgSmem + 2048);
   if (e != cudaSuccess) return e;
-  f<<<dim3(p.parts, p.tiles_a, p.tiles_b), wg_threads(PLANES, RING), smem, s>>>(P);
+  f<<<dim3((P.m + p.rows - 1) / p.rows, p.tiles_a, p.tiles_b), wg_threads(PLANES, RING), smem, s>>>(P);
   return cudaGetLastError();
 }
 template <class T, int PLANES> cudaError_t wg_run(const WgPlan &p, WgParams P, cudaStream_t s) {
@@ -485,7 +493,8 @@ using namespace tfk;
 
 extern "C" long long tf_weight_grad8_work_floats(int m, int na, int nb, int dtype) {
   if (m < 0 || m > kMaxRows || na <= 0 || nb <= 0 || !wg_fits(na, nb) || !known_dtype(dtype)) return 0;
-  return (long long)wg_plan(m, na, nb, dtype).parts * na * nb;
+  const WgPlan p = wg_plan(m, na, nb, dtype);
+  return (p.group + (p.group < p.parts ? 1ll : 0ll)) * na * nb;
 }
 
 extern "C" int tf_weight_grad8(const void *g, long long ld_g, int dtype, int na, const signed char *codes, int ld_codes,
@@ -508,13 +517,19 @@ extern "C" int tf_weight_grad8(const void *g, long long ld_g, int dtype, int na,
   P.wait_limit = dense_wait_limit();
   cudaStream_t s = (cudaStream_t)stream;
   cudaError_t e = cudaSuccess;
-  if (m > 0) {
-    e = dtype == TF_F32 ? wg_run<float, 3>(p, P, s) : dtype == TF_F16 ? wg_run<__half, 2>(p, P, s) : wg_run<__nv_bfloat16, 1>(p, P, s);
-  }
-  if (e == cudaSuccess) {
-    const int n = na * nb;
-    wg_sum_kernel<<<(n + 31) / 32, 256, 0, s>>>(work, m > 0 ? p.parts : 0, n, out, dtype);
+  const int n = na * nb;
+  float *sums = work + (size_t)p.group * n;  // of the launches before (there is room where there are several)
+  long long row = 0;
+  do {
+    P.g = static_cast<const char *>(g) + row * ld_g * value_bytes(dtype);
+    P.codes = codes + row * ld_codes;
+    P.exps = exponents + row * (ld_codes / kPackGroup);
+    P.m = (int)std::min<long long>(m - row, (long long)p.group * p.rows);
+    if (m > 0) e = dtype == TF_F32 ? wg_run<float, 3>(p, P, s) : dtype == TF_F16 ? wg_run<__half, 2>(p, P, s) : wg_run<__nv_bfloat16, 1>(p, P, s);
+    if (e != cudaSuccess) break;
+    wg_sum_kernel<<<(n + 31) / 32, 256, 0, s>>>(work, m > 0 ? (P.m + p.rows - 1) / p.rows : 0, n, row ? sums : nullptr, row + P.m < m ? sums : nullptr, out, dtype);
     e = cudaGetLastError();
-  }
+    row += P.m;
+  } while (e == cudaSuccess && row < m);
   return e == cudaSuccess ? TF_OK : tf::fail(TF_ERR_CUDA, std::string("tf_weight_grad8: ") + cudaGetErrorString(e));
 }
