@@ -257,3 +257,15 @@ def test_tangents_and_traces(built_lib):
         codes, exps = ops.pack8(a)
         got = traced(a, b)
         assert torch.equal(got[0], ops.unpack8(codes, exps)) and torch.equal(got[1], ops.weight_grad8(b, codes, exps))
+
+
+def test_mask_refuses(built_lib):
+    import torch
+    from tile_fusion_b200 import dense_ops
+    g, c = torch.zeros(6, 40, device="cuda"), torch.zeros(6, 64, device="cuda", dtype=torch.int8)
+    for grad, codes in ((g.cpu(), c), (g, c.cpu()), (g.double(), c), (g, c.int()), (g[:, :8], c), (g, c[:5]), (g, c[:, :40]), (g, c[:, :32]), (g[:, 0], c),
+                        (torch.zeros(6, 70, device="cuda"), c)):
+        with pytest.raises(ValueError):
+            dense_ops.relu_grad8_(grad, codes)
+    assert dense_ops.relu_grad8_(torch.ones(6, 40, device="cuda"), c).sum() == 0
+    assert dense_ops.relu_grad8_(g[:0], c[:0]).shape == (0, 40)

@@ -138,11 +138,20 @@ def _weight_grad(g, codes, ld, exponents, nb, stream):
 
 
 @_on_device_of_first
-def relu_grad8_(grad, codes, stream):
-    """grad (a contiguous matrix, in place) where the packed value was positive, zero elsewhere."""
+def _relu_grad(grad, codes, stream):
     n, d = grad.shape
     _lib.check(_lib.lib().tf_relu_grad8(codes.data_ptr(), codes.shape[1], _DTYPES[grad.dtype], n, d, grad.data_ptr(), d, stream))
     return grad
+
+
+def relu_grad8_(grad, codes):
+    """grad (a contiguous matrix, in place) where the packed value was positive, zero elsewhere; codes: whole groups of 32, as they are packed."""
+    _check_values("relu_grad8_", "grad", grad)
+    if grad.dim() != 2 or not grad.is_contiguous():
+        raise ValueError(f"sw_gcn.relu_grad8_: grad must be a contiguous matrix, not {tuple(grad.shape)} with strides {grad.stride()}")
+    if codes.dtype != torch.int8 or codes.device != grad.device or not codes.is_contiguous() or codes.shape != (grad.shape[0], -(-grad.shape[1] // 32) * 32):
+        raise ValueError(f"sw_gcn.relu_grad8_: codes must be contiguous int8 on grad's device, [{grad.shape[0]}, {-(-grad.shape[1] // 32) * 32}], not {tuple(codes.shape)}")
+    return _relu_grad(grad, codes)
 
 
 def _packed(name, codes, exponents):
