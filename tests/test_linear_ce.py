@@ -327,3 +327,33 @@ def test_memory_of_a_large_vocabulary(built_lib, dtype):
     torch.cuda.reset_peak_memory_stats()
     run(x, w, t)
     assert torch.cuda.max_memory_allocated() - before < 2 * v * d + (100 << 20)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,d,v", [(1, 1, 2), (3, 1, 100), (2, 257, 2), (1, 300, 65), (5, 2, 20_000)])
+def test_smallest_sizes(built_lib, dtype, n, d, v):
+    """One row, one column: slopes are rounded to the type before products of one or two terms, so tolerances are taken of the summands, not of
+    their sum: 2 u of sum |P| |w|."""
+    import torch
+    x, w, t = make(n, d, v, dtype, ignored=0)
+    loss, dx, dw = run(x, w, t, "sum")
+    want, wx, ww = reference(x, w, t, "sum")
+    assert abs(loss.double() - want).item() <= 2e-5 * n
+    logp = torch.log_softmax(x.double() @ w.double().t(), 1)
+    p = logp.exp()
+    p[torch.arange(n, device="cuda"), t] -= 1
+    bound = 2 * U[dtype] + 2e-5
+    small = 2.0 ** -24 if dtype == "float16" else 0.0  # (its steps below 2^-14)
+    assert ((dx.double() - wx).abs() <= bound * (p.abs() @ w.double().abs()) + small).all()
+    assert ((dw.double() - ww).abs() <= bound * (p.abs().t() @ x.double().abs()) + small + 1e-6 * x.double().abs().sum(0)).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [8, 257])
+def test_one_class(built_lib, dtype, d):
+    """The loss over one class is zero whatever the logits, up to their rounding: 2^-23 of |logit| < 32."""
+    import torch
+    x, w, t = make(40, d, 1, dtype)
+    loss, dx, dw = run(x, w, t, "sum")
+    assert abs(loss.item()) <= 40 * 2.0 ** -18
+    assert dx.abs().max().item() <= 2.0 ** -18 * w.abs().max().item() and dw.abs().max().item() <= 40 * 2.0 ** -18 * x.abs().max().item()
