@@ -412,7 +412,8 @@ int tf_layer_norm_bwd(const void *x, long long ld_x, const signed char *codes, i
  * exponents [rows][ld_codes / 32].  relu: negative values become zero first, and -128 is the code of a positive value that
  * rounds to zero (it reads back as zero).
  *   tf_relu_grad8: grad (in place) becomes zero where the code is zero, i.e. where a value packed with relu was not positive.
- *   tf_weight_grad8: out[na][nb] = G^T X for G [m][na] and the packed X [m][nb], in G's type; products are exact, sums fp32;
+ *   tf_weight_grad8: out[na][nb] = G^T X for G [m][na] and the packed X [m][nb], in G's type; products are exact, sums fp32, infinities
+ * in G as the formula has them;
  * work: tf_weight_grad8_work_floats floats of the caller's, 16-byte aligned; at most 2^26 entries, 2^20 to a side,
  * and rows of codes at most 2^26 bytes apart.
  * Device pointers; the calls only enqueue work on `stream`. */
@@ -432,7 +433,10 @@ int tf_weight_grad8(const void *g, long long ld_g, int dtype, int na, const sign
  * memory.  x [rows][cols] (ld_x values from row to row) and w [vocab][cols] of one tf_dtype, all pointers on the device.
  * reduction 0: loss[rows], zero where a row does not count; 1: the mean over the rows that count (zero if none does);
  * 2: their sum; the sums are taken in 64 bits, in a fixed order.  lse2[rows] receives log2 of the sums for the backward call.
- *   A target outside [0, vocab) that is not `ignore_index` makes its row's loss NaN, and its gradients.
+ *   A target outside [0, vocab) that is not `ignore_index` makes its row's loss NaN, and its gradients; so does a NaN among a
+ * row's logits.  fp32 operands are multiplied with 22 bits of each value down to 2^-17 of the operand's largest finite one (over at
+ * most 64 classes and 256 columns: of 64 rows' largest, and the weight's), below that off by 2^-39 of it; an infinity in them may
+ * make its logits NaN.  Gradients of rows (reduction 0) far below the largest are off by 2^-39 of that in fp32 and fp16.
  *   backward: grad[1] (reduction 1, 2) or grad[rows] (0) is the gradient of the loss; dx [rows][cols] and dw [vocab][cols],
  * contiguous, of the operands' type, are overwritten; either may be NULL.  Rows that do not count have a gradient of zero and
  * add nothing to dw, whatever they hold.

@@ -11,8 +11,9 @@
 //   * Eight warps (forward two) turn logits into losses, or into the slope P = (exp(l - lse) - (class == target)) * row_scale as operand planes,
 //     write dX, and add up dW in registers: 24 additions in tensor memory, which cuts off, then one that rounds.
 //   * The CTAs' dW are added by a second launch, in order.
-// 120 001 rows, 256 columns, 47 classes, fp32: forward 55 us (2.2 TB/s), backward 106 (2.3 TB/s), bound by a tile's way through these stages:
-// neither memory nor the tensor cores nor the issue slots are busy for more than a third of the time.
+// 120 001 rows, 256 columns, 47 classes: the forward pass 55 us in fp32 and 33 in bf16, the backward pass 111 and 78, small launches before and
+// behind included, bound by a tile's way through these stages: neither memory (2.4 TB/s in fp32) nor the tensor cores (25 and 35 % of the time)
+// nor the schedulers (0.36 and 0.26 instructions a cycle) are busy for long.
 // All waits are bounded: the one that runs out sets the error flag, and every role leaves.
 #include "ce_few.h"
 

@@ -6,7 +6,8 @@
 // x 602 fp32: 39 us, 64 with a CTA to a row; 60 000 x 1 024 bf16 51 and 65; 30 000 x 1 024 fp32 with codes 75 and 58); wider ones to a CTA,
 // R rows a turn so that a barrier serves them all, and the rows of two turns ahead are on their way into shared memory; a thread
 // copies what it alone reads, so copies need no barrier.  Statistics are fp32 whatever the values' type.
-//   120 001 x 256 fp32: 36 us (6.8 TB/s, part of it into L2); 16 384 x 4 096 bf16: 60 (4.5, issue slots).
+//   120 001 x 256 fp32: 36 us (6.8 TB/s, part of it into L2); 16 384 x 4 096 bf16: 60 (4.5 TB/s; 0.63 instructions a cycle
+//   and scheduler, with two barriers a turn: nothing is at its limit).
 //   The pass can leave its input in 8 bits on the way (pack8.cuh), which the backward pass then reads in its place.
 #include <algorithm>
 #include <initializer_list>

@@ -10,7 +10,7 @@
 // time so that a barrier serves them all, and come through shared memory with asynchronous copies two turns ahead; a thread copies what
 // it alone reads, so copies need no barrier.
 // Sums are fp32 whatever the values' type.
-//   120 001 x 256 fp32: 66 us (5.6 TB/s); 16 384 x 4 096 bf16: 85 (4.7, issue slots); 50 021 x 602 fp32 from 8 bits: 66 (4.1).
+//   120 001 x 256 fp32: 66 us (5.6 TB/s); 16 384 x 4 096 bf16: 85 (4.7 TB/s at 0.65 instructions a cycle and scheduler); 50 021 x 602 fp32 from 8 bits: 66 (4.1).
 #include <algorithm>
 #include <initializer_list>
 #include <string>

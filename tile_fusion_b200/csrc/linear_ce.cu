@@ -3,18 +3,20 @@
 //   forward    logits tile by tile in tensor memory (plane_gemm.cu); a tile leaves the largest logit and the sum of
 //              exponentials of each row, in units of log2, and the target's logit.  A second kernel joins the parts.
 //   backward   the vocabulary in pieces: logits again, the slope P = exp(l - lse) - (column == target) of a piece as 16-bit
-//              planes (at most kCeSlopeBytes of them, however large the vocabulary), then dx += P W_piece and
+//              planes (at most kCeSlopeBytes of them, or 256 classes' where rows are many), then dx += P W_piece and
 //              dW_piece = P^T x.  Four products of 2 n d V operations in all where kept logits would need three.
 //
 //   Bound by the products: 4 096 rows, 2 048 columns, 50 021 classes in bf16, loss and gradients, 2 343 us, of which 2 285 are products
 //   (1 433 TFLOP/s over all).
-//   Up to 64 classes and 256 columns have kernels of their own (ce_few.cu), which read x once a pass.
+//   Up to 64 classes and 256 columns have kernels of their own (ce_few.cu), which read x once a pass; beyond, fp32 rows are read for their
+//   largest value, written as planes, and those read, in both passes.
 //
 // Types.  bf16 and fp16 operands are multiplied as they are.  The slope is rounded to their type before its products, one
 // rounding of at most 2^-8 (bf16) or 2^-11 (fp16) of each summand; the sums are fp32.  fp32 operands are split into two fp16
-// planes behind a power of two that brings the largest finite value to [2^14, 2^15): 22 bits of every value within 2^-27 of the
-// largest, an absolute 2^-39 of the largest below.  The slope of fp32 operands is two planes too.
-// A slope lies in [-1, 1]; in fp16 it is held times 2^14, so that one of 2^-29 still has all its bits.
+// planes behind a power of two that brings the operand's largest finite value to [2^14, 2^15): 22 bits of every value down to 2^-17 of
+// that value, where the second plane becomes subnormal; below, an absolute error of 2^-39 of it (at 2^-27 twelve bits are left).
+// An infinity's second plane is zero, and what it is multiplied with may make it a NaN.  The slope of fp32 operands is two planes too.
+// A slope lies in [-1, 1]; in fp16 it is held times 2^14: a first plane has its eleven bits down to 2^-28, both together (fp32) are off by 2^-39.
 // Rows that do not count (target == ignore_index) have a slope of zero, and the rows of x that dW is summed over are a copy in
 // which they are zero, so that what such rows hold -- padding, infinities, NaN -- reaches nothing.
 #include <cuda_runtime.h>

@@ -16,16 +16,16 @@ number of steps of its 64th part, the nearest one, at most 127 of them.  ``codes
 start on multiples of 32, ``exponents`` uint8 [rows, columns / 32 rounded up]; a group that holds an infinity or a NaN reads
 back as NaN.  With ``relu`` negative values become zero first, and a code of -128 is a positive value that rounds to zero, so
 that ``codes != 0`` says where the value was positive.  ``weight_grad8`` is the weight gradient of a layer whose input was
-packed, in grad's type.  These three carry no graph; ``fusedGeMMSpMM_ck8`` is the layer that uses them:
+packed, in grad's type, of at most 2^26 entries.  These three carry no graph; ``fusedGeMMSpMM_ck8`` is the layer that uses them:
 ``adj @ (h @ weight.T)`` with ``h = feature``, or with ``relu`` ``h = max(feature, 0)``, of which it keeps the 8 bits instead of
 the 32; the forward result and the gradient of feature are those of ``fusedGeMMSpMM``, the weight's gradient is taken at the
 kept values.
 
 ``linear_cross_entropy`` is the softmax cross entropy of ``x @ weight.T`` (weight stored ``[out, in]``, as in the layers)
-against class indices, without the logits in memory, with the gradients of both operands.  Rows whose target is
+against class indices, without the logits in memory, with the gradients of both operands, which have the same type.  Rows whose target is
 ``ignore_index`` do not count: they add nothing to the loss or to the weight's gradient and receive a gradient of zero,
 whatever they hold.  ``reduction``: "mean" over the rows that count (zero if none does), "sum", or "none" (a loss to each
-row).  The loss is fp32.
+row).  The loss is fp32.  fp32 operands are multiplied as two fp16 planes: 22 bits of values down to 2^-17 of their tensor's largest.
 
 The operators take fp32, bf16 and fp16 CUDA tensors whose last dimension is contiguous or is made so, run on the current
 stream of the tensors' device, take their workspaces from torch's allocator, and can be captured into CUDA graphs.  They
