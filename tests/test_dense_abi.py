@@ -170,3 +170,9 @@ def test_work_space_of_a_weight_gradient(L):
             assert L.tf_weight_grad8_work_floats(m, 47, 256, dtype) <= (64 << 20) + 2 * 47 * 256
             assert L.tf_weight_grad8_work_floats(m, 1000, 700, dtype) <= (64 << 20) + 2 * 1000 * 700
     assert L.tf_weight_grad8_work_floats(1_000_000, 256, 100, _lib.BF16) == 148 * 256 * 100
+
+
+def test_ranges_of_very_many_rows(L):
+    """A range's rows on top of 2^31 - 2^24 pass 32 bits: 16 ranges for 9 tiles became one, of a sixteenth of the rows."""
+    assert L.tf_weight_grad8_work_floats(0x7f000000, 300, 600, _lib.F32) == 16 * 300 * 600
+    assert L.tf_weight_grad8_work_floats(0x7f000000, 300, 300, _lib.F32) == 148 // 6 * 300 * 300

@@ -1,7 +1,5 @@
 """The C entry points of the dense operators on a GPU, where they allow more than tensors of torch show: results that start anywhere; and what a
 bounded wait that ran out leaves."""
-import ctypes as C
-
 import pytest
 
 from tile_fusion_b200 import _lib

@@ -439,6 +439,7 @@ __global__ void __launch_bounds__(256) wg_sum_kernel(const float *__restrict__ p
 // there are many rows; those of a launch together hold 256 MB of sums at most, or as many as fill it.
 struct WgPlan { int mt, tiles_a, tiles_b, parts, rows, group; };
 constexpr long long kWgMaxFloats = 64ll << 20;
+int wg_ranges(int m, int rows) { return (int)std::max(1ll, ((long long)m + rows - 1) / std::max(1, rows)); }
 WgPlan wg_plan(int m, int na, int nb, int dtype) {
   auto tiles = [&](int mt) {
     WgPlan p;
@@ -456,8 +457,8 @@ WgPlan wg_plan(int m, int na, int nb, int dtype) {
   // one CTA to an SM; a range of fewer than 128 rows spends its time on the result
   int parts = std::max(1, std::min(148 / (p.tiles_a * p.tiles_b), (m + 127) / 128));
   if (dtype != TF_F32) parts = std::max(parts, (m + kWgStayRows - 1) / kWgStayRows);
-  p.rows = ((m + parts - 1) / parts + kWgRows - 1) / kWgRows * kWgRows;
-  p.parts = std::max(1, (m + p.rows - 1) / std::max(1, p.rows));
+  p.rows = (int)(((long long)m + parts - 1) / parts + kWgRows - 1) / kWgRows * kWgRows;
+  p.parts = wg_ranges(m, p.rows);
   p.group = (int)std::min<long long>(p.parts, std::max<long long>(std::max(1, 148 / (p.tiles_a * p.tiles_b)), kWgMaxFloats / ((long long)na * nb)));
   return p;
 }
@@ -467,7 +468,7 @@ template <class T, int PLANES, int MT, bool RING> cudaError_t wg_launch(const Wg
   const int smem = wg_teams(PLANES) * wg_stage_bytes(PLANES, MT) + P.ring * P.ring_bytes + 1024;
   const cudaError_t e = cudaFuncSetAttribute((const void *)f, cudaFuncAttributeMaxDynamicSharedMemorySize, kWgSmem + 2048);
   if (e != cudaSuccess) return e;
-  f<<<dim3((P.m + p.rows - 1) / p.rows, p.tiles_a, p.tiles_b), wg_threads(PLANES, RING), smem, s>>>(P);
+  f<<<dim3(wg_ranges(P.m, p.rows), p.tiles_a, p.tiles_b), wg_threads(PLANES, RING), smem, s>>>(P);
   return cudaGetLastError();
 }
 template <class T, int PLANES> cudaError_t wg_run(const WgPlan &p, WgParams P, cudaStream_t s) {
@@ -528,7 +529,7 @@ extern "C" int tf_weight_grad8(const void *g, long long ld_g, int dtype, int na,
     P.m = (int)std::min<long long>(m - row, (long long)p.group * p.rows);
     if (m > 0) e = dtype == TF_F32 ? wg_run<float, 3>(p, P, s) : dtype == TF_F16 ? wg_run<__half, 2>(p, P, s) : wg_run<__nv_bfloat16, 1>(p, P, s);
     if (e != cudaSuccess) break;
-    wg_sum_kernel<<<(n + 31) / 32, 256, 0, s>>>(work, m > 0 ? (P.m + p.rows - 1) / p.rows : 0, n, row ? sums : nullptr, row + P.m < m ? sums : nullptr, out, dtype);
+    wg_sum_kernel<<<(n + 31) / 32, 256, 0, s>>>(work, m > 0 ? wg_ranges(P.m, p.rows) : 0, n, row ? sums : nullptr, row + P.m < m ? sums : nullptr, out, dtype);
     e = cudaGetLastError();
     row += P.m;
   } while (e == cudaSuccess && row < m);
